@@ -28,6 +28,7 @@ extern "C" {
 #define MSLK_AMD_DTYPE_BF16 0
 #define MSLK_AMD_DTYPE_F16 1
 #define MSLK_AMD_DTYPE_F32 2
+#define MSLK_AMD_DTYPE_E4M3FN 3 /* of a paged cache only */
 
 /* bias element types */
 #define MSLK_AMD_BIAS_NONE 0
@@ -301,6 +302,74 @@ int mslk_amd_f8f8bf16_rowwise_grouped_dynamic(const void* xq, const void* wq, co
 int mslk_amd_f8f8bf16_rowwise_batched(const void* xq, const void* wq, const float* x_scale, const float* w_scale,
                                       const void* bias, int bias_dtype, int64_t B, int64_t M, int64_t N,
                                       int64_t K, void* y, void* stream);
+
+/*
+ * Attention of a decoder layer that is served: prompts, and one new token per sequence over a paged cache.  No counterpart among
+ * the reference operators above; the package registers them as torch.ops.mslk.append_kv, attention_decode, attention_prompt.
+ *
+ * Rows of heads: element (token, head, channel) lies at data[token * token_stride + head * head_stride + channel], strides in
+ * elements.  Query head h reads KV head h / (Hq / Hkv).  D is a multiple of 8, at most 256; rows begin on 16-byte boundaries
+ * (base pointers and strides multiples of 8 elements).  `dtype` is MSLK_AMD_DTYPE_BF16 or _F16; sums, softmax and rotation run
+ * in fp32.
+ */
+typedef struct {
+  const void* data;
+  int64_t token_stride, head_stride;
+} mslk_amd_heads;
+
+/*
+ * A paged cache.  Key t of sequence b lies in slot t % page_size of page page_table[b * table_stride + t / page_size]; its row of
+ * head h begins at k + page * k_stride[0] + slot * k_stride[1] + h * k_stride[2] (elements), that of its value and, where the
+ * cache holds e4m3 codes, their fp32 scales alike.  Entries of the page table that no key needs are not used; a key whose entry
+ * is not in [0, pages), or lies beyond table_width, makes the attention of its sequence NaN.
+ */
+typedef struct {
+  void *k, *v;
+  float *k_scale, *v_scale; /* MSLK_AMD_DTYPE_E4M3FN only: value = code * scale */
+  int64_t k_stride[3], v_stride[3], k_scale_stride[3], v_scale_stride[3];
+  int64_t pages, page_size;
+  const int32_t* page_table; /* [sequences, table_width] */
+  int64_t table_width, table_stride;
+  const int32_t* kv_lens; /* [sequences] keys of each sequence, new ones included */
+  int dtype;              /* that of the queries, or MSLK_AMD_DTYPE_E4M3FN */
+} mslk_amd_paged_cache;
+
+/*
+ * Rotates queries and keys by their positions and writes keys and values into the cache.  The tokens of sequence b are
+ * cu_seqlens[b] ... cu_seqlens[b + 1] - 1 (NULL: one token per sequence, tokens == sequences) and take the last positions of its
+ * kv_lens[b] keys.
+ *   rotary   NULL, or [rotary_positions, rotary_dim] fp32: cosines, then sines of the angles; channel pairs (i, i + rotary_dim / 2),
+ *            with interleaved != 0 (2 i, 2 i + 1), become (a cos - b sin, b cos + a sin), the channels behind rotary_dim stay
+ *   q_out    [tokens, Hq, D] contiguous
+ * A token of no sequence, or whose position is negative, is padding: its query becomes zero and nothing is stored.  A token
+ * whose position lies beyond `rotary`, or has no page, stores nothing either; its query becomes NaN.
+ * e4m3 caches: scale = max(amax, 1e-12) / 448 and code = e4m3fn(x * (448 / max(amax, 1e-12))) of the row in fp32.
+ */
+int mslk_amd_append_kv(const mslk_amd_heads* q, const mslk_amd_heads* k, const mslk_amd_heads* v, int dtype, int64_t tokens,
+                       int64_t Hq, int64_t Hkv, int64_t D, const mslk_amd_paged_cache* cache, const int32_t* cu_seqlens,
+                       int64_t sequences, const float* rotary, int64_t rotary_positions, int64_t rotary_dim, int interleaved,
+                       void* q_out, void* stream);
+
+/*
+ * out[b, h] = sum_t softmax_t(scale q[b, h] . k[t]) v[t] over the kv_lens[b] keys of sequence b (q: one token per sequence), and
+ * lse[b, h] = log sum_t exp(scale q . k[t]).  No keys: zeros and -inf.  scale > 0.
+ *   out [sequences, Hq, D], lse [sequences, Hq], contiguous; workspace: mslk_amd_attention_decode_workspace_bytes() of it, 16-byte aligned.
+ */
+size_t mslk_amd_attention_decode_workspace_bytes(int64_t sequences, int64_t Hq, int64_t Hkv, int64_t D, int64_t table_width, int64_t page_size);
+int mslk_amd_attention_decode(const mslk_amd_heads* q, int dtype, int64_t sequences, int64_t Hq, int64_t Hkv, int64_t D,
+                              const mslk_amd_paged_cache* cache, float scale, void* out, float* lse, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/*
+ * The same for whole prompts packed one after the other: queries cu_seqlens[b] ... cu_seqlens[b + 1] - 1 of `tokens` over keys
+ * cu_seqlens_k[b] ... of `keys` (NULL: cu_seqlens).  causal != 0: the last query of a sequence sees its last key, the one before
+ * it all but that, and so on; queries in front of the first key, and tokens of no sequence, see nothing.
+ *   out [tokens, Hq, D], lse [tokens, Hq], contiguous.  tokens, keys < 2^30.
+ */
+int mslk_amd_attention_prompt(const mslk_amd_heads* q, const mslk_amd_heads* k, const mslk_amd_heads* v, int dtype, int64_t tokens,
+                              int64_t keys, int64_t Hq, int64_t Hkv, int64_t D, const int32_t* cu_seqlens,
+                              const int32_t* cu_seqlens_k, int64_t sequences, int causal, float scale, void* out, float* lse,
+                              void* stream);
 
 /*
  * Self-test helper: converts n fp32 values to e4m3fn with the same device routine the quantizer

@@ -17,6 +17,19 @@ TORCH_OPS_PATH = os.path.join(_HERE, "_torch_ops.so")
 
 _lib = None
 
+class Heads(ctypes.Structure):
+    """mslk_amd_heads"""
+    _fields_ = [("data", c_void_p), ("token_stride", c_int64), ("head_stride", c_int64)]
+
+
+class PagedCache(ctypes.Structure):
+    """mslk_amd_paged_cache"""
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+                ("k_stride", c_int64 * 3), ("v_stride", c_int64 * 3), ("k_scale_stride", c_int64 * 3), ("v_scale_stride", c_int64 * 3),
+                ("pages", c_int64), ("page_size", c_int64), ("page_table", c_void_p), ("table_width", c_int64),
+                ("table_stride", c_int64), ("kv_lens", c_void_p), ("dtype", c_int)]
+
+
 # name -> (restype, argtypes); mirrors include/mslk_amd.h one to one
 SIGNATURES = {
     "mslk_amd_version": (c_char_p, []),
@@ -60,6 +73,13 @@ SIGNATURES = {
                                                           c_int64, c_int64, c_int64, c_void_p, c_int, c_void_p]),
     "mslk_amd_f8f8bf16_rowwise_batched": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int64,
                                                   c_int64, c_int64, c_int64, c_void_p, c_void_p]),
+    "mslk_amd_append_kv": (c_int, [POINTER(Heads), POINTER(Heads), POINTER(Heads), c_int, c_int64, c_int64, c_int64, c_int64,
+                                   POINTER(PagedCache), c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p]),
+    "mslk_amd_attention_decode_workspace_bytes": (c_size_t, [c_int64] * 6),
+    "mslk_amd_attention_decode": (c_int, [POINTER(Heads), c_int, c_int64, c_int64, c_int64, c_int64, POINTER(PagedCache), c_float,
+                                          c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "mslk_amd_attention_prompt": (c_int, [POINTER(Heads), POINTER(Heads), POINTER(Heads), c_int, c_int64, c_int64, c_int64, c_int64,
+                                          c_int64, c_void_p, c_void_p, c_int64, c_int, c_float, c_void_p, c_void_p, c_void_p]),
     "mslk_amd_debug_cast_e4m3fn": (c_int, [c_void_p, c_int64, c_void_p, c_void_p]),
     "mslk_amd_debug_dispatch_name": (c_char_p, [c_int64, c_int64, c_int64, c_int, c_int, c_int, c_int]),
     "mslk_amd_debug_grouped_dispatch_name": (c_char_p, [c_int, c_int, c_int64, c_int64, c_int64]),

@@ -7,6 +7,7 @@
 #include <mutex>
 
 #include "../../include/mslk_amd.h"
+#include "attention.h"
 #include "kernels.h"
 
 namespace {
@@ -57,6 +58,66 @@ int scratch_of_current_device(void** out) {
 }  // namespace
 
 using namespace mslk_amd;
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------------------------------
+// attention: checks shared by its entry points
+// ---------------------------------------------------------------------------------------------------------------------
+constexpr int64_t kMaxTokens = int64_t(1) << 30;
+
+bool aligned(const void* p, uintptr_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; }
+
+int check_heads(const char* op, int dtype, int64_t tokens, int64_t Hq, int64_t Hkv, int64_t D) {
+  if (dtype != MSLK_AMD_DTYPE_BF16 && dtype != MSLK_AMD_DTYPE_F16) return fail("%s: bf16 or fp16 expected (dtype code %d)", op, dtype);
+  if (tokens < 0 || tokens >= kMaxTokens) return fail("%s: token counts must be in [0, 2^30) (got %lld)", op, (long long)tokens);
+  if (Hq <= 0 || Hkv <= 0 || Hq > 65535 || Hq % Hkv != 0)
+    return fail("%s: the query heads (%lld, at most 65535) must be a multiple of the KV heads (%lld)", op, (long long)Hq, (long long)Hkv);
+  if (D <= 0 || D > kMaxHeadDim || D % 8 != 0) return fail("%s: the head dimension must be a multiple of 8, at most 256 (got %lld)", op, (long long)D);
+  return 0;
+}
+int check_rows(const char* op, const char* what, const mslk_amd_heads* h, HeadRows& out) {
+  if (h == nullptr || h->data == nullptr) return fail("%s: null pointer (%s)", op, what);
+  // (offsets inside a tile of 64 rows are 32-bit numbers of bytes)
+  if (h->token_stride < 0 || h->head_stride < 0 || h->token_stride >= (int64_t(1) << 25)) return fail("%s: stride of %s out of range", op, what);
+  if (!aligned(h->data, 16) || h->token_stride % 8 != 0 || h->head_stride % 8 != 0) return fail("%s: rows of %s must begin on 16-byte boundaries", op, what);
+  out = HeadRows{(const uint16_t*)h->data, h->token_stride, h->head_stride};
+  return 0;
+}
+int check_cache(const char* op, const mslk_amd_paged_cache* c, int dtype, int64_t sequences, PagedCache& out) {
+  if (c == nullptr) return fail("%s: null pointer (cache)", op);
+  if (c->dtype != dtype && c->dtype != MSLK_AMD_DTYPE_E4M3FN) return fail("%s: the cache must hold the type of the queries or e4m3 codes (dtype code %d)", op, c->dtype);
+  if (sequences < 0 || sequences > 65535) return fail("%s: at most 65535 sequences (got %lld)", op, (long long)sequences);
+  if (c->pages < 0 || c->pages > kIntMax || c->page_size <= 0 || c->page_size >= kMaxTokens || c->table_width < 0 || c->table_width >= kMaxTokens)
+    return fail("%s: pages, page_size or table_width out of range", op);
+  const bool fp8 = c->dtype == MSLK_AMD_DTYPE_E4M3FN;
+  if (sequences > 0 && ((c->table_width > 0 && !c->page_table) || !c->kv_lens)) return fail("%s: null pointer (page_table, kv_lens)", op);
+  if (c->pages > 0 && (!c->k || !c->v || (fp8 && (!c->k_scale || !c->v_scale)))) return fail("%s: null pointer (cache)", op);
+  const uintptr_t row = fp8 ? 8 : 16;
+  bool fits = aligned(c->k, row) && aligned(c->v, row);
+  for (int i = 0; i < 3; ++i) {
+    out.k_stride[i] = c->k_stride[i];
+    out.v_stride[i] = c->v_stride[i];
+    out.k_scale_stride[i] = c->k_scale_stride[i];
+    out.v_scale_stride[i] = c->v_scale_stride[i];
+    fits = fits && c->k_stride[i] % 8 == 0 && c->v_stride[i] % 8 == 0;
+  }
+  if (!fits) return fail("%s: rows of the cache must begin on %d-byte boundaries", op, (int)row);
+  out.k = c->k;
+  out.v = c->v;
+  out.k_scale = c->k_scale;
+  out.v_scale = c->v_scale;
+  out.pages = (int)c->pages;
+  out.page_size = divider((uint32_t)c->page_size);
+  out.table = c->page_table;
+  out.table_width = (int)c->table_width;
+  out.table_stride = c->table_stride;
+  out.lens = c->kv_lens;
+  return 0;
+}
+bool good_scale(float scale) { return scale > 0.f && scale <= 3.0e38f; }
+
+}  // namespace
 
 extern "C" {
 
@@ -438,6 +499,101 @@ int mslk_amd_f8f8bf16_rowwise_batched(const void* xq, const void* wq, const floa
   DeviceGroups p{(const uint8_t*)xq, (const uint8_t*)wq, x_scale, w_scale, bias, (uint16_t*)y, nullptr, (int)B,
                  (int)M, (int)N, (int)K, bias_dtype, 0};
   return check_hip(launch_device_groups(p, kGroupsUniform, s), "batched launch");
+}
+
+int mslk_amd_append_kv(const mslk_amd_heads* q, const mslk_amd_heads* k, const mslk_amd_heads* v, int dtype, int64_t tokens,
+                       int64_t Hq, int64_t Hkv, int64_t D, const mslk_amd_paged_cache* cache, const int32_t* cu_seqlens,
+                       int64_t sequences, const float* rotary, int64_t rotary_positions, int64_t rotary_dim, int interleaved,
+                       void* q_out, void* stream) {
+  const char* op = "append_kv";
+  AppendArgs p{};
+  if (int rc = check_heads(op, dtype, tokens, Hq, Hkv, D)) return rc;
+  if (int rc = check_cache(op, cache, dtype, sequences, p.cache)) return rc;
+  if (cu_seqlens == nullptr && sequences != tokens)
+    return fail("%s: without cu_seqlens there is one token per sequence (%lld tokens, %lld sequences)", op, (long long)tokens, (long long)sequences);
+  if (rotary != nullptr && (rotary_positions < 0 || rotary_dim < 2 || rotary_dim > D || rotary_dim % 2 != 0))
+    return fail("%s: rotary_dim must be even and at most the head dimension (got %lld)", op, (long long)rotary_dim);
+  if (tokens == 0) return 0;
+  if (int rc = check_rows(op, "q", q, p.q)) return rc;
+  if (int rc = check_rows(op, "k", k, p.k)) return rc;
+  if (int rc = check_rows(op, "v", v, p.v)) return rc;
+  if (!q_out || !aligned(q_out, 16)) return fail("%s: q_out must not be null and be 16-byte aligned", op);
+  p.q_out = (uint16_t*)q_out;
+  p.cu_seqlens = cu_seqlens;
+  p.rotary = rotary;
+  p.rotary_positions = rotary_positions;
+  p.rotary_dim = rotary != nullptr ? (int)rotary_dim : 0;
+  p.interleaved = interleaved != 0;
+  p.tokens = tokens;
+  p.sequences = (int)sequences;
+  p.Hq = (int)Hq; p.Hkv = (int)Hkv; p.D = (int)D; p.dtype = dtype;
+  p.fp8 = cache->dtype == MSLK_AMD_DTYPE_E4M3FN;
+  return check_hip(launch_append_kv(p, (hipStream_t)stream), "append_kv launch");
+}
+
+size_t mslk_amd_attention_decode_workspace_bytes(int64_t sequences, int64_t Hq, int64_t Hkv, int64_t D, int64_t table_width, int64_t page_size) {
+  if (sequences <= 0 || sequences > 65535 || Hq <= 0 || Hkv <= 0 || Hq > 65535 || Hq % Hkv != 0 || D <= 0 || D > kMaxHeadDim || table_width < 0 ||
+      table_width >= kMaxTokens || page_size <= 0 || page_size >= kMaxTokens)
+    return 0;
+  return decode_workspace_bytes(sequences, Hq, Hkv, D, table_width * page_size);
+}
+
+int mslk_amd_attention_decode(const mslk_amd_heads* q, int dtype, int64_t sequences, int64_t Hq, int64_t Hkv, int64_t D,
+                              const mslk_amd_paged_cache* cache, float scale, void* out, float* lse, void* workspace,
+                              size_t workspace_bytes, void* stream) {
+  const char* op = "attention_decode";
+  DecodeArgs p{};
+  if (int rc = check_heads(op, dtype, sequences, Hq, Hkv, D)) return rc;
+  if (int rc = check_cache(op, cache, dtype, sequences, p.cache)) return rc;
+  if (!good_scale(scale)) return fail("%s: scale must be positive and finite", op);
+  if (sequences == 0) return 0;
+  if (int rc = check_rows(op, "q", q, p.q)) return rc;
+  if (!out || !lse || !aligned(out, 16)) return fail("%s: out and lse must not be null and out be 16-byte aligned", op);
+  // keys without a page are read from page 0, and what they give is dropped: there has to be one
+  if (cache->pages == 0) return fail("%s: the cache must hold at least one page", op);
+  const size_t need = mslk_amd_attention_decode_workspace_bytes(sequences, Hq, Hkv, D, cache->table_width, cache->page_size);
+  if (need > 0 && (!workspace || workspace_bytes < need || !aligned(workspace, 16)))
+    return fail("%s: needs a 16-byte aligned workspace of %zu bytes (got %zu)", op, need, workspace ? workspace_bytes : (size_t)0);
+  p.out = (uint16_t*)out;
+  p.lse = lse;
+  p.partial = (float*)workspace;
+  p.sequences = (int)sequences;
+  p.Hq = (int)Hq; p.Hkv = (int)Hkv; p.D = (int)D; p.dtype = dtype;
+  p.fp8 = cache->dtype == MSLK_AMD_DTYPE_E4M3FN;
+  p.scale = scale;
+  return check_hip(launch_attention_decode(p, (hipStream_t)stream), "attention_decode launch");
+}
+
+int mslk_amd_attention_prompt(const mslk_amd_heads* q, const mslk_amd_heads* k, const mslk_amd_heads* v, int dtype, int64_t tokens,
+                              int64_t keys, int64_t Hq, int64_t Hkv, int64_t D, const int32_t* cu_seqlens,
+                              const int32_t* cu_seqlens_k, int64_t sequences, int causal, float scale, void* out, float* lse,
+                              void* stream) {
+  const char* op = "attention_prompt";
+  PromptArgs p{};
+  if (int rc = check_heads(op, dtype, tokens, Hq, Hkv, D)) return rc;
+  if (keys < 0 || keys >= kMaxTokens) return fail("%s: token counts must be in [0, 2^30) (got %lld)", op, (long long)keys);
+  if (sequences < 0 || sequences >= kMaxTokens) return fail("%s: sequences out of range (got %lld)", op, (long long)sequences);
+  if (cu_seqlens_k == nullptr && keys != tokens) return fail("%s: without cu_seqlens_k there are as many keys as queries (%lld, %lld)", op, (long long)keys, (long long)tokens);
+  if (!good_scale(scale)) return fail("%s: scale must be positive and finite", op);
+  if (tokens == 0) return 0;
+  if (!cu_seqlens) return fail("%s: null pointer (cu_seqlens)", op);
+  if (int rc = check_rows(op, "q", q, p.q)) return rc;
+  if (keys > 0) {
+    if (int rc = check_rows(op, "k", k, p.k)) return rc;
+    if (int rc = check_rows(op, "v", v, p.v)) return rc;
+  }
+  if (!out || !lse || !aligned(out, 16)) return fail("%s: out and lse must not be null and out be 16-byte aligned", op);
+  p.out = (uint16_t*)out;
+  p.lse = lse;
+  p.cu_q = cu_seqlens;
+  p.cu_k = cu_seqlens_k != nullptr ? cu_seqlens_k : cu_seqlens;
+  p.tokens = tokens;
+  p.keys = keys;
+  p.sequences = (int)sequences;
+  p.Hq = (int)Hq; p.Hkv = (int)Hkv; p.D = (int)D; p.dtype = dtype;
+  p.causal = causal != 0;
+  p.scale = scale;
+  return check_hip(launch_attention_prompt(p, (hipStream_t)stream), "attention_prompt launch");
 }
 
 int mslk_amd_debug_cast_e4m3fn(const float* in, int64_t n, void* out, void* stream) {

@@ -17,6 +17,7 @@
 #include <dlfcn.h>
 #include <torch/library.h>
 
+#include <cmath>
 #include <cstring>
 #include <optional>
 #include <string>
@@ -52,7 +53,11 @@ constexpr auto kF8 = at::kFloat8_e4m3fn;
   X(mslk_amd_quantize_f8f8bf16_rowwise_supported)                                                                      \
   X(mslk_amd_f8f8bf16_rowwise_grouped)                                                                                 \
   X(mslk_amd_f8f8bf16_rowwise_grouped_stacked)                                                                         \
-  X(mslk_amd_f8f8bf16_rowwise_grouped_mm)
+  X(mslk_amd_f8f8bf16_rowwise_grouped_mm)                                                                              \
+  X(mslk_amd_append_kv)                                                                                                \
+  X(mslk_amd_attention_decode_workspace_bytes)                                                                         \
+  X(mslk_amd_attention_decode)                                                                                         \
+  X(mslk_amd_attention_prompt)
 
 struct Api {
 #define X(name) decltype(&::name) name = nullptr;
@@ -554,6 +559,184 @@ Tensor grouped_mm_op(const Tensor& XQ, const Tensor& WQ, const Tensor& x_scale, 
   return output;
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// attention
+// ---------------------------------------------------------------------------------------------------------------------
+// [tokens, heads, channels] with rows that the kernels can read as they are (itself if it is that, a copy otherwise).
+struct HeadsArg {
+  c10::MaybeOwned<Tensor> keep;
+  mslk_amd_heads view{};
+};
+HeadsArg heads_of(const Tensor& t) {
+  HeadsArg h;
+  // (the stride of a dimension of size 0 or 1 has no meaning)
+  const bool fits = aligned16(t) && (t.size(2) <= 1 || t.stride(2) == 1) && (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) < (1 << 25))) &&
+                    (t.size(1) <= 1 || t.stride(1) % 8 == 0);
+  h.keep = fits ? c10::MaybeOwned<Tensor>::borrowed(t) : c10::MaybeOwned<Tensor>::owned(t.clone(at::MemoryFormat::Contiguous));
+  const Tensor& u = *h.keep;
+  h.view = {u.const_data_ptr(), u.size(0) <= 1 ? 0 : u.stride(0), u.size(1) <= 1 ? 0 : u.stride(1)};
+  return h;
+}
+void check_heads(const char* op, const Tensor& q, const Tensor& k, const Tensor& v) {
+  TORCH_CHECK(q.dim() == 3 && k.dim() == 3 && v.dim() == 3, op, ": q, k and v must have shape [tokens, heads, channels]");
+  TORCH_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf, op, ": q must be bfloat16 or float16, got ", q.scalar_type());
+  TORCH_CHECK(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(), op, ": q, k and v must have the same dtype");
+  TORCH_CHECK(q.is_cuda() && k.device() == q.device() && v.device() == q.device(), op, ": q, k and v must be GPU tensors on one device");
+  TORCH_CHECK(k.sizes() == v.sizes(), op, ": k and v must have the same shape");
+  TORCH_CHECK(k.size(2) == q.size(2), op, ": q, k and v must have the same number of channels, got ", q.size(2), " and ", k.size(2));
+}
+void check_head_counts(const char* op, int64_t Hq, int64_t Hkv, int64_t D) {
+  TORCH_CHECK(Hq > 0 && Hkv > 0 && Hq % Hkv == 0, op, ": the query heads (", Hq, ") must be a multiple of the KV heads (", Hkv, ")");
+  TORCH_CHECK(D > 0 && D <= 256 && D % 8 == 0, op, ": the head dimension must be a multiple of 8, at most 256, got ", D);
+}
+const int32_t* int32_of(const char* op, const char* name, const Tensor& t, const Tensor& like) {
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.device() == like.device(), op, ": ", name, " must be an int32 tensor on the device of q");
+  return t.const_data_ptr<int32_t>();
+}
+// cu_seqlens: offsets of the sequences, one more than there are
+int64_t sequences_of(const char* op, const char* name, const Tensor& cu) {
+  TORCH_CHECK(cu.dim() == 1 && cu.is_contiguous() && cu.size(0) >= 1, op, ": ", name, " must be a contiguous 1-D tensor of at least one offset");
+  return cu.size(0) - 1;
+}
+float scale_of(const char* op, std::optional<double> scale, int64_t D) {
+  const double s = scale.value_or(1.0 / std::sqrt((double)D));
+  TORCH_CHECK((float)s > 0.f && std::isfinite((float)s), op, ": scale must be positive and finite, got ", s);
+  return (float)s;
+}
+
+mslk_amd_paged_cache cache_of(const char* op, const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table,
+                              const Tensor& kv_lens, const OptTensor& k_scale, const OptTensor& v_scale) {
+  TORCH_CHECK(k_cache.dim() == 4 && k_cache.sizes() == v_cache.sizes(), op, ": k_cache and v_cache must have one shape [pages, page_size, kv_heads, channels]");
+  TORCH_CHECK(k_cache.scalar_type() == v_cache.scalar_type() && (k_cache.scalar_type() == q.scalar_type() || k_cache.scalar_type() == kF8), op,
+              ": the cache must have the dtype of q or torch.float8_e4m3fn, got ", k_cache.scalar_type(), " and ", v_cache.scalar_type());
+  TORCH_CHECK(k_cache.device() == q.device() && v_cache.device() == q.device(), op, ": the cache must be on the device of q");
+  TORCH_CHECK(k_cache.size(3) == q.size(-1), op, ": q and the cache must have the same number of channels, got ", q.size(-1), " and ", k_cache.size(3));
+  TORCH_CHECK(k_cache.size(1) > 0, op, ": pages must hold at least one key");
+  const bool fp8 = k_cache.scalar_type() == kF8;
+  mslk_amd_paged_cache c{};
+  const auto strides = [&](const Tensor& t, int64_t* out, int64_t unit, const char* name) {
+    for (int i = 0; i < 3; ++i) {
+      out[i] = t.size(i) <= 1 ? 0 : t.stride(i);
+      TORCH_CHECK(out[i] % unit == 0, op, ": rows of ", name, " must begin on ", fp8 ? 8 : 16, "-byte boundaries");
+    }
+  };
+  for (const Tensor* t : {&k_cache, &v_cache})
+    TORCH_CHECK(t->stride(3) == 1 && reinterpret_cast<uintptr_t>(t->const_data_ptr()) % (fp8 ? 8 : 16) == 0, op,
+                ": the channels of the cache must be contiguous and its rows begin on ", fp8 ? 8 : 16, "-byte boundaries");
+  c.k = const_cast<void*>(k_cache.const_data_ptr());
+  c.v = const_cast<void*>(v_cache.const_data_ptr());
+  strides(k_cache, c.k_stride, 8, "k_cache");
+  strides(v_cache, c.v_stride, 8, "v_cache");
+  const bool scaled = k_scale.has_value() && k_scale->defined(), v_scaled = v_scale.has_value() && v_scale->defined();
+  TORCH_CHECK(scaled == fp8 && v_scaled == fp8, op, ": k_scale and v_scale belong to a float8_e4m3fn cache, and both to it");
+  if (fp8) {
+    for (const Tensor* t : {&*k_scale, &*v_scale})
+      TORCH_CHECK(t->scalar_type() == at::kFloat && t->device() == q.device() && t->dim() == 3 && t->sizes() == k_cache.sizes().slice(0, 3), op,
+                  ": k_scale and v_scale must be float32 tensors [pages, page_size, kv_heads] on the device of q");
+    c.k_scale = const_cast<float*>(k_scale->const_data_ptr<float>());
+    c.v_scale = const_cast<float*>(v_scale->const_data_ptr<float>());
+    strides(*k_scale, c.k_scale_stride, 1, "k_scale");
+    strides(*v_scale, c.v_scale_stride, 1, "v_scale");
+  }
+  c.pages = k_cache.size(0);
+  c.page_size = k_cache.size(1);
+  c.dtype = fp8 ? MSLK_AMD_DTYPE_E4M3FN : float_code(q.scalar_type());
+  c.page_table = int32_of(op, "page_table", page_table, q);
+  TORCH_CHECK(page_table.dim() == 2 && (page_table.size(1) <= 1 || page_table.stride(1) == 1), op, ": page_table must have shape [sequences, width] with unit column stride");
+  c.table_width = page_table.size(1);
+  c.table_stride = page_table.size(0) <= 1 ? 0 : page_table.stride(0);
+  c.kv_lens = int32_of(op, "kv_lens", kv_lens, q);
+  TORCH_CHECK(kv_lens.dim() == 1 && kv_lens.is_contiguous() && kv_lens.size(0) == page_table.size(0), op, ": kv_lens must be contiguous and hold one length per row of page_table (",
+              page_table.size(0), "), got ", kv_lens.sizes());
+  return c;
+}
+
+Tensor append_kv(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table,
+                 const Tensor& kv_lens, const OptTensor& cu_seqlens, const OptTensor& rotary, bool interleaved, const OptTensor& k_scale,
+                 const OptTensor& v_scale) {
+  const char* op = "append_kv";
+  check_heads(op, q, k, v);
+  const int64_t T = q.size(0), Hq = q.size(1), Hkv = k.size(1), D = q.size(2);
+  TORCH_CHECK(k.size(0) == T, op, ": q, k and v must hold the same tokens, got ", T, " and ", k.size(0));
+  check_head_counts(op, Hq, Hkv, D);
+  const mslk_amd_paged_cache cache = cache_of(op, q, k_cache, v_cache, page_table, kv_lens, k_scale, v_scale);
+  TORCH_CHECK(k_cache.size(2) == Hkv, op, ": the cache holds ", k_cache.size(2), " KV heads, k ", Hkv);
+  const int64_t sequences = page_table.size(0);
+  const int32_t* cu = nullptr;
+  if (cu_seqlens.has_value() && cu_seqlens->defined()) {
+    cu = int32_of(op, "cu_seqlens", *cu_seqlens, q);
+    TORCH_CHECK(sequences_of(op, "cu_seqlens", *cu_seqlens) == sequences, op, ": cu_seqlens must hold one offset more than page_table has rows (", sequences, ")");
+  } else {
+    TORCH_CHECK(sequences == T, op, ": without cu_seqlens there is one token per sequence, got ", T, " tokens and ", sequences, " sequences");
+  }
+  const float* turn = nullptr;
+  int64_t positions = 0, rotary_dim = 0;
+  if (rotary.has_value() && rotary->defined()) {
+    TORCH_CHECK(rotary->scalar_type() == at::kFloat && rotary->device() == q.device() && rotary->dim() == 2 && rotary->is_contiguous(), op,
+                ": rotary must be a contiguous float32 tensor [positions, rotated channels] on the device of q");
+    positions = rotary->size(0);
+    rotary_dim = rotary->size(1);
+    TORCH_CHECK(rotary_dim >= 2 && rotary_dim % 2 == 0 && rotary_dim <= D, op, ": the rotated channels must be even in number and at most ", D, ", got ", rotary_dim);
+    TORCH_CHECK(positions > 0, op, ": rotary must hold at least one position");
+    turn = rotary->const_data_ptr<float>();
+  }
+  Tensor out = empty_on(q.sizes(), q.scalar_type(), q);
+  if (T == 0) return out;
+  const c10::DeviceGuard guard(q.device());
+  const HeadsArg hq = heads_of(q), hk = heads_of(k), hv = heads_of(v);
+  check_rc(api.mslk_amd_append_kv(&hq.view, &hk.view, &hv.view, float_code(q.scalar_type()), T, Hq, Hkv, D, &cache, cu, sequences, turn, positions,
+                                  rotary_dim, interleaved, out.mutable_data_ptr(), stream_of(q)));
+  return out;
+}
+
+std::tuple<Tensor, Tensor> attention_decode(const Tensor& q, const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table,
+                                            const Tensor& kv_lens, const OptTensor& k_scale, const OptTensor& v_scale, std::optional<double> scale) {
+  const char* op = "attention_decode";
+  TORCH_CHECK(q.dim() == 3, op, ": q must have shape [sequences, heads, channels]");
+  TORCH_CHECK(q.scalar_type() == at::kBFloat16 || q.scalar_type() == at::kHalf, op, ": q must be bfloat16 or float16, got ", q.scalar_type());
+  TORCH_CHECK(q.is_cuda(), op, ": q must be a GPU tensor");
+  const mslk_amd_paged_cache cache = cache_of(op, q, k_cache, v_cache, page_table, kv_lens, k_scale, v_scale);
+  const int64_t B = q.size(0), Hq = q.size(1), D = q.size(2), Hkv = k_cache.size(2);
+  check_head_counts(op, Hq, Hkv, D);
+  TORCH_CHECK(page_table.size(0) == B, op, ": page_table must have a row per sequence (", B, "), got ", page_table.size(0));
+  const float s = scale_of(op, scale, D);
+  Tensor out = empty_on(q.sizes(), q.scalar_type(), q), lse = empty_on({B, Hq}, at::kFloat, q);
+  if (B == 0) return {out, lse};
+  const c10::DeviceGuard guard(q.device());
+  const HeadsArg hq = heads_of(q);
+  const size_t bytes = api.mslk_amd_attention_decode_workspace_bytes(B, Hq, Hkv, D, cache.table_width, cache.page_size);
+  Tensor workspace;
+  if (bytes > 0) workspace = empty_on({(int64_t)bytes}, at::kByte, q);
+  check_rc(api.mslk_amd_attention_decode(&hq.view, float_code(q.scalar_type()), B, Hq, Hkv, D, &cache, s, out.mutable_data_ptr(),
+                                         lse.mutable_data_ptr<float>(), bytes > 0 ? workspace.mutable_data_ptr() : nullptr, bytes, stream_of(q)));
+  return {out, lse};
+}
+
+std::tuple<Tensor, Tensor> attention_prompt(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_seqlens, const OptTensor& cu_seqlens_k,
+                                            bool causal, std::optional<double> scale) {
+  const char* op = "attention_prompt";
+  check_heads(op, q, k, v);
+  const int64_t T = q.size(0), Hq = q.size(1), Hkv = k.size(1), D = q.size(2), S = k.size(0);
+  check_head_counts(op, Hq, Hkv, D);
+  const int32_t* cu = int32_of(op, "cu_seqlens", cu_seqlens, q);
+  const int64_t sequences = sequences_of(op, "cu_seqlens", cu_seqlens);
+  const int32_t* cu_k = nullptr;
+  if (cu_seqlens_k.has_value() && cu_seqlens_k->defined()) {
+    cu_k = int32_of(op, "cu_seqlens_k", *cu_seqlens_k, q);
+    TORCH_CHECK(sequences_of(op, "cu_seqlens_k", *cu_seqlens_k) == sequences, op, ": cu_seqlens_k must hold as many offsets as cu_seqlens");
+  } else {
+    TORCH_CHECK(S == T, op, ": without cu_seqlens_k there are as many keys as queries, got ", S, " and ", T);
+  }
+  const float s = scale_of(op, scale, D);
+  Tensor out = empty_on(q.sizes(), q.scalar_type(), q), lse = empty_on({T, Hq}, at::kFloat, q);
+  if (T == 0) return {out, lse};
+  const c10::DeviceGuard guard(q.device());
+  const HeadsArg hq = heads_of(q), hk = heads_of(k), hv = heads_of(v);
+  check_rc(api.mslk_amd_attention_prompt(&hq.view, &hk.view, &hv.view, float_code(q.scalar_type()), T, S, Hq, Hkv, D, cu, cu_k, sequences, causal, s,
+                                         out.mutable_data_ptr(), lse.mutable_data_ptr<float>(), stream_of(q)));
+  return {out, lse};
+}
+
 // Registered as boxed functions, one operator at a time and when the package asks for it.  A library loaded earlier may have
 // defined an operator (the package then only replaces its GPU kernel): a kernel registered with its C++ type is refused where
 // that library's own kernels take, say, Tensor by value instead of by reference, and an exception in a static initializer
@@ -587,6 +770,9 @@ const Kernel kernels[] = {
     kernel<grouped_cat_op>("mslk", "f8f8bf16_rowwise_grouped_cat"),
     kernel<grouped_stacked_op>("mslk", "f8f8bf16_rowwise_grouped_stacked"),
     kernel<grouped_mm_op>("mslk", "f8f8bf16_rowwise_grouped_mm"),
+    kernel<append_kv>("mslk", "append_kv"),
+    kernel<attention_decode>("mslk", "attention_decode"),
+    kernel<attention_prompt>("mslk", "attention_prompt"),
 };
 
 }  // namespace
