@@ -58,7 +58,8 @@ struct DecodeArgs {
   PagedCache cache;
   uint16_t* out;                         // [sequences, Hq, D]
   float* lse;                            // [sequences, Hq]
-  float* partial;                        // workspace
+  float* partial;                        // workspace: the pieces of divided head blocks, ...
+  int* ends;                             // ... and the first and last of each
   int sequences, Hq, Hkv, D, dtype, fp8;
   float scale;
 };

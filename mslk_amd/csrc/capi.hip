@@ -101,6 +101,11 @@ int check_cache(const char* op, const mslk_amd_paged_cache* c, int dtype, int64_
     out.k_scale_stride[i] = c->k_scale_stride[i];
     out.v_scale_stride[i] = c->v_scale_stride[i];
     fits = fits && c->k_stride[i] % 8 == 0 && c->v_stride[i] % 8 == 0;
+    // (the kernels count pieces of eight channels, and scales, of a page in 32 bits)
+    const int64_t most = int64_t(1) << 32;
+    if (c->k_stride[i] < 0 || c->v_stride[i] < 0 || c->k_scale_stride[i] < 0 || c->v_scale_stride[i] < 0 || c->k_stride[i] >= 8 * most ||
+        c->v_stride[i] >= 8 * most || c->k_scale_stride[i] >= most || c->v_scale_stride[i] >= most)
+      return fail("%s: stride of the cache out of range", op);
   }
   if (!fits) return fail("%s: rows of the cache must begin on %d-byte boundaries", op, (int)row);
   out.k = c->k;
@@ -549,6 +554,9 @@ int mslk_amd_attention_decode(const mslk_amd_heads* q, int dtype, int64_t sequen
   if (sequences == 0) return 0;
   if (int rc = check_rows(op, "q", q, p.q)) return rc;
   if (!out || !lse || !aligned(out, 16)) return fail("%s: out and lse must not be null and out be 16-byte aligned", op);
+  const int64_t blocks = sequences * Hkv * ((Hq / Hkv + 15) / 16);
+  if (blocks * (cache->table_width * cache->page_size / 32 + 1) >= (int64_t(1) << 31))
+    return fail("%s: the page tables have room for too many keys (at most 2^31 tiles of 32, over sequences and KV heads)", op);
   // keys without a page are read from page 0, and what they give is dropped: there has to be one
   if (cache->pages == 0) return fail("%s: the cache must hold at least one page", op);
   const size_t need = mslk_amd_attention_decode_workspace_bytes(sequences, Hq, Hkv, D, cache->table_width, cache->page_size);
