@@ -17,8 +17,6 @@ from typing import Optional, Tuple, Union
 
 import torch
 
-from .gemm import _op
-
 _library = torch.library.Library("mslk", "FRAGMENT")
 
 
@@ -44,6 +42,9 @@ for _name, (_schema, _fake) in _OPS.items():
     if not hasattr(torch.ops.mslk, _name):
         _library.define(_name + _schema)
         torch.library.register_fake(f"mslk::{_name}", _fake, lib=_library)
+    # Outside of autograd: without a derivative its fallback would make the results part of the graph of any input that requires a
+    # gradient.  (Calling under no_grad() instead costs 1.5 us, a quarter of a small call.)
+    _library.impl(_name, torch.library.fallthrough_kernel, "Autograd")
 
 
 def _check_gpu(name: str, q: torch.Tensor) -> None:
@@ -65,7 +66,7 @@ def append_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.
     Tokens of no sequence and positions below zero are padding: a query of zeros, nothing stored.  A position beyond `rotary` or
     without a page stores nothing and gives a query of NaN."""
     _check_gpu("append_kv", q)
-    return _op("append_kv", q, k, v, k_cache, v_cache, page_table, kv_lens, cu_seqlens, rotary, interleaved, k_scale, v_scale)
+    return torch.ops.mslk.append_kv(q, k, v, k_cache, v_cache, page_table, kv_lens, cu_seqlens, rotary, interleaved, k_scale, v_scale)
 
 
 def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, kv_lens: torch.Tensor,
@@ -76,7 +77,7 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     Returns out [sequences, Hq, D] and, with `return_lse`, log sum exp of the scaled scores [sequences, Hq] (fp32).  `scale` is
     1 / sqrt(D) unless given.  A sequence without keys gives zeros and -inf; one whose keys lack a page gives NaN."""
     _check_gpu("attention_decode", q)
-    out, lse = _op("attention_decode", q, k_cache, v_cache, page_table, kv_lens, k_scale, v_scale, scale)
+    out, lse = torch.ops.mslk.attention_decode(q, k_cache, v_cache, page_table, kv_lens, k_scale, v_scale, scale)
     return (out, lse) if return_lse else out
 
 
@@ -89,5 +90,5 @@ def attention_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     `causal`: the last query of a sequence sees its last key, each one before it a key less.  Queries that see nothing, and tokens
     of no sequence, give zeros and -inf.  Returns as `attention_decode`."""
     _check_gpu("attention_prompt", q)
-    out, lse = _op("attention_prompt", q, k, v, cu_seqlens, cu_seqlens_k, causal, scale)
+    out, lse = torch.ops.mslk.attention_prompt(q, k, v, cu_seqlens, cu_seqlens_k, causal, scale)
     return (out, lse) if return_lse else out

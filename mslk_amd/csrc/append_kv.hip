@@ -6,35 +6,43 @@
 // row.
 //
 // A team of eight lanes holds a row in registers, two vectors of VEC channels per lane and unit: the two partners of VEC
-// rotations (half of the rotated part apart, or neighbours with `interleaved`), or the next 2 VEC unrotated channels.
+// rotations (half of the rotated part apart, or neighbours with `interleaved`), or the next 2 VEC unrotated channels.  A workgroup
+// takes 32 consecutive rows: it asks for them and looks up the places of their tokens meanwhile, one lane a token (the sequence,
+// its length, the page: loads that wait for one another).
 #include "attention.h"
 #include "rows.h"
 
 namespace mslk_amd {
 namespace {
 
-constexpr int kTeam = 8, kThreads = 256, kRowsPerBlock = kThreads / kTeam;
+constexpr int kTeam = 8, kThreads = 256, kBlockRows = kThreads / kTeam;
+constexpr int kBlockTokens = kBlockRows / 3 + 2;   // a token has at least three rows
 
 // VEC consecutive 16-bit channels.
-template <bool F16, int VEC>
-MSLK_AMD_DEVINL void load_vec(const uint16_t* src, float* x) {
-  using E = Elem<F16>;
-  if constexpr (VEC == 1) {
-    x[0] = E::lo(*src);
-  } else {
+template <int VEC> struct Raw {
+  static constexpr int kWords = VEC == 1 ? 1 : VEC / 2;
+  uint32_t w[kWords];
+};
+template <int VEC>
+MSLK_AMD_DEVINL Raw<VEC> load_raw(const uint16_t* src) {
+  Raw<VEC> r;
+  if constexpr (VEC == 1) r.w[0] = *src;
+  else if constexpr (VEC == 2) r.w[0] = *reinterpret_cast<const uint32_t*>(src);
+  else {
     typedef uint32_t words __attribute__((ext_vector_type(VEC / 2)));
-    uint32_t w[VEC / 2];
-    if constexpr (VEC == 2) w[0] = *reinterpret_cast<const uint32_t*>(src);
-    else {
-      const words v = *reinterpret_cast<const words*>(src);
+    const words v = __builtin_nontemporal_load(reinterpret_cast<const words*>(src));
 #pragma unroll
-      for (int i = 0; i < VEC / 2; ++i) w[i] = v[i];
-    }
+    for (int i = 0; i < VEC / 2; ++i) r.w[i] = v[i];
+  }
+  return r;
+}
+template <bool F16, int VEC>
+MSLK_AMD_DEVINL void to_floats(const Raw<VEC>& r, float* x) {
+  using E = Elem<F16>;
 #pragma unroll
-    for (int i = 0; i < VEC / 2; ++i) {
-      x[2 * i] = E::lo(w[i]);
-      x[2 * i + 1] = E::hi(w[i]);
-    }
+  for (int i = 0; i < Raw<VEC>::kWords; ++i) {
+    x[2 * i] = E::lo(r.w[i]);
+    if constexpr (VEC > 1) x[2 * i + 1] = E::hi(r.w[i]);
   }
 }
 template <bool F16, int VEC>
@@ -76,98 +84,93 @@ MSLK_AMD_DEVINL int sequence_of(const int32_t* cu, int sequences, int64_t token)
   return lo < sequences && cu[lo] <= token ? lo : -1;
 }
 
+// Where a token goes.
+struct Place {
+  int position, page, slot;
+  int state;   // 0: stored, 1: padding, 2: has no place
+};
+MSLK_AMD_DEVINL Place place_of(const AppendArgs& p, int64_t token) {
+  Place r{0, 0, 0, 1};
+  const int seq = p.cu_seqlens == nullptr ? (token < p.sequences ? (int)token : -1) : sequence_of(p.cu_seqlens, p.sequences, token);
+  if (seq < 0) return r;
+  const int64_t position = (int64_t)p.cache.lens[seq] - (p.cu_seqlens == nullptr ? 1 : p.cu_seqlens[seq + 1] - token);
+  if (position < 0) return r;
+  r.state = 2;
+  if (p.rotary != nullptr && position >= p.rotary_positions) return r;
+  r.position = (int)position;
+  const int index = (int)divide((uint32_t)position, p.cache.page_size);
+  r.slot = r.position - index * (int)p.cache.page_size.d;
+  if (index >= p.cache.table_width) return r;
+  r.page = p.cache.table[seq * p.cache.table_stride + index];
+  if (r.page >= 0 && r.page < p.cache.pages) r.state = 0;
+  return r;
+}
+
 template <bool F16, bool FP8, bool INTERLEAVED, int VEC>
 __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs p, Divider heads, int64_t rows) {
   constexpr int kUnits = kMaxHeadDim / (2 * VEC * kTeam);   // per lane
-  const int64_t row = row_block() * kRowsPerBlock + threadIdx.x / kTeam;
-  if (row >= rows) return;
-  const int lane = threadIdx.x % kTeam;
-  const int64_t token = heads.magic == 0 ? row : row < (int64_t(1) << 31) ? (int64_t)divide((uint32_t)row, heads) : row / heads.d;
-  const int h = (int)(row - token * heads.d);
+  __shared__ Place places[kBlockTokens];
+  const int64_t row0 = row_block() * kBlockRows;
+  if (row0 >= rows) return;
+  const int64_t token0 = row0 < (int64_t(1) << 31) ? (int64_t)divide((uint32_t)row0, heads) : row0 / heads.d;
+  const int lane = threadIdx.x % kTeam, team = threadIdx.x / kTeam;
+  const int lead = (int)(row0 - token0 * heads.d);   // rows of the first token that are in front of the block
+  const int count = (int)min(rows - row0, (int64_t)kBlockRows);
+
+  const int r = lead + min(team, count - 1);   // (teams behind the last row repeat it and store nothing)
+  const int in_block = (int)divide((uint32_t)r, heads), h = r - in_block * (int)heads.d;
+  const int64_t token = token0 + in_block;
   const bool is_q = h < p.Hq, is_v = h >= p.Hq + p.Hkv;
   const int kv_head = is_q ? 0 : is_v ? h - p.Hq - p.Hkv : h - p.Hq;
   const uint16_t* src = is_q   ? p.q.data + token * p.q.token_stride + h * p.q.head_stride
                         : is_v ? p.v.data + token * p.v.token_stride + kv_head * p.v.head_stride
                                : p.k.data + token * p.k.token_stride + kv_head * p.k.head_stride;
-
-  // the token's place
-  int64_t position = -1;
-  const int seq = p.cu_seqlens == nullptr ? (token < p.sequences ? (int)token : -1) : sequence_of(p.cu_seqlens, p.sequences, token);
-  if (seq >= 0) position = (int64_t)p.cache.lens[seq] - (p.cu_seqlens == nullptr ? 1 : p.cu_seqlens[seq + 1] - token);
-  const bool padding = position < 0;
-  bool placed = !padding && (p.rotary == nullptr || position < p.rotary_positions);
-  int64_t page = 0;
-  int slot = 0;
-  if (placed) {
-    const int index = (int)divide((uint32_t)position, p.cache.page_size);
-    slot = (int)position - index * (int)p.cache.page_size.d;
-    placed = index < p.cache.table_width;
-    if (placed) {
-      page = p.cache.table[seq * p.cache.table_stride + index];
-      placed = page >= 0 && page < p.cache.pages;
-    }
-  }
-  if (!placed && !is_q) return;
-
-  const int turned = is_v || p.rotary == nullptr ? 0 : p.rotary_dim;   // rotated channels
-  const int half = turned / 2;
-  const int turning = half / VEC;                                        // units that are rotated
+  const int turned = is_v || p.rotary == nullptr ? 0 : p.rotary_dim, half = turned / 2, turning = half / VEC;   // rotated channels, units
   const int units = turning + (p.D - turned + 2 * VEC - 1) / (2 * VEC);
-  float x[kUnits][2][VEC];
-  int at[kUnits][2];   // first channels of a unit's vectors, D where there is none
+  int at[kUnits][2];   // first channels of a unit's two vectors, D where there is none
+  Raw<VEC> raw[kUnits][2];
 #pragma unroll
   for (int i = 0; i < kUnits; ++i) {
     const int u = lane + i * kTeam;
     at[i][0] = at[i][1] = p.D;
     if (u < units) {
-      if (u >= turning) {
-        at[i][0] = turned + (u - turning) * 2 * VEC;
-        at[i][1] = at[i][0] + VEC;
-      } else if (INTERLEAVED) {
-        at[i][0] = u * 2 * VEC;
-        at[i][1] = at[i][0] + VEC;
-      } else {
-        at[i][0] = u * VEC;
-        at[i][1] = at[i][0] + half;
-      }
+      at[i][0] = u >= turning ? turned + (u - turning) * 2 * VEC : INTERLEAVED ? u * 2 * VEC : u * VEC;
+      at[i][1] = u >= turning || INTERLEAVED ? at[i][0] + VEC : at[i][0] + half;
     }
 #pragma unroll
     for (int j = 0; j < 2; ++j)
-      if (at[i][j] < p.D) load_vec<F16, VEC>(src + at[i][j], x[i][j]);
+      if (at[i][j] < p.D) raw[i][j] = load_raw<VEC>(src + at[i][j]);
   }
-  if (placed && turned != 0) {
-    const float* cosines = p.rotary + position * p.rotary_dim;
+  if ((int)threadIdx.x <= (int)divide((uint32_t)(lead + count - 1), heads)) places[threadIdx.x] = place_of(p, token0 + threadIdx.x);
+  __syncthreads();
+
+  if (team >= count) return;
+  const Place place = places[in_block];
+  const bool placed = place.state == 0;
+  if (!placed && !is_q) return;
+  float x[kUnits][2][VEC];
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    const int u = lane + i * kTeam;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) to_floats<F16, VEC>(raw[i][j], x[i][j]);
+    if (!placed || u >= turning) continue;
+    const float* cosines = p.rotary + (int64_t)place.position * p.rotary_dim + u * VEC;
     const float* sines = cosines + half;
 #pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-      const int u = lane + i * kTeam;
-      if (u >= turning) continue;
-      if constexpr (!INTERLEAVED) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float cs = cosines[u * VEC + e], sn = sines[u * VEC + e], a = x[i][0][e], b = x[i][1][e];
-          x[i][0][e] = __fsub_rn(__fmul_rn(a, cs), __fmul_rn(b, sn));
-          x[i][1][e] = __fadd_rn(__fmul_rn(b, cs), __fmul_rn(a, sn));
-        }
-      } else {
-        float flat[2 * VEC];
-#pragma unroll
-        for (int e = 0; e < 2 * VEC; ++e) flat[e] = x[i][e / VEC][e % VEC];
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float cs = cosines[u * VEC + e], sn = sines[u * VEC + e], a = flat[2 * e], b = flat[2 * e + 1];
-          flat[2 * e] = __fsub_rn(__fmul_rn(a, cs), __fmul_rn(b, sn));
-          flat[2 * e + 1] = __fadd_rn(__fmul_rn(b, cs), __fmul_rn(a, sn));
-        }
-#pragma unroll
-        for (int e = 0; e < 2 * VEC; ++e) x[i][e / VEC][e % VEC] = flat[e];
-      }
+    for (int e = 0; e < VEC; ++e) {
+      // partners: element e of the two vectors, or neighbours in the 2 VEC channels that they make up
+      float& a = INTERLEAVED ? x[i][2 * e / VEC][2 * e % VEC] : x[i][0][e];
+      float& b = INTERLEAVED ? x[i][(2 * e + 1) / VEC][(2 * e + 1) % VEC] : x[i][1][e];
+      const float cs = cosines[e], sn = sines[e], a0 = a, b0 = b;
+      a = __fsub_rn(__fmul_rn(a0, cs), __fmul_rn(b0, sn));
+      b = __fadd_rn(__fmul_rn(b0, cs), __fmul_rn(a0, sn));
     }
   }
 
   if (is_q) {
     uint16_t* dst = p.q_out + (token * p.Hq + h) * p.D;
-    const float other = padding ? 0.f : __builtin_nanf("");
+    const float other = place.state == 1 ? 0.f : __builtin_nanf("");
 #pragma unroll
     for (int i = 0; i < kUnits; ++i)
 #pragma unroll
@@ -181,7 +184,7 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs p, Divider 
     return;
   }
   const int64_t* stride = is_v ? p.cache.v_stride : p.cache.k_stride;
-  const int64_t to = page * stride[0] + slot * stride[1] + kv_head * stride[2];
+  const int64_t to = place.page * stride[0] + place.slot * stride[1] + kv_head * stride[2];
   if constexpr (!FP8) {
     uint16_t* dst = (uint16_t*)(is_v ? p.cache.v : p.cache.k) + to;
 #pragma unroll
@@ -208,15 +211,14 @@ __global__ __launch_bounds__(kThreads) void append_kernel(AppendArgs p, Divider 
         if (at[i][j] < p.D) store_codes<VEC>(dst + at[i][j], x[i][j], inv);
     if (lane == 0) {
       const int64_t* ss = is_v ? p.cache.v_scale_stride : p.cache.k_scale_stride;
-      (is_v ? p.cache.v_scale : p.cache.k_scale)[page * ss[0] + slot * ss[1] + kv_head * ss[2]] = amax / 448.0f;
+      (is_v ? p.cache.v_scale : p.cache.k_scale)[place.page * ss[0] + place.slot * ss[1] + kv_head * ss[2]] = amax / 448.0f;
     }
   }
 }
 
 template <bool F16, bool FP8, bool INTERLEAVED>
 hipError_t pick(const AppendArgs& p, hipStream_t s) {
-  const int64_t rows = p.tokens * (p.Hq + 2 * p.Hkv);
-  const int64_t blocks = (rows + kRowsPerBlock - 1) / kRowsPerBlock;
+  const int64_t rows = p.tokens * (p.Hq + 2 * p.Hkv), blocks = (rows + kBlockRows - 1) / kBlockRows;
   const Divider heads = divider((uint32_t)(p.Hq + 2 * p.Hkv));
   // the widest vectors that fit between the partners of a rotation
   const int fit = p.rotary == nullptr ? 8 : p.rotary_dim / 2;
