@@ -208,6 +208,32 @@ def test_prompt_long():
     near(lse[rows.to(DEV)], want[1], want[3])
 
 
+@pytest.mark.parametrize("hq,hkv", [(2, 1), (8, 8), (48, 16)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_prompt_ragged_batches(hq, hkv, causal):
+    """2 to 65 sequences of any lengths, few and many heads: whichever order the blocks of queries are taken in, each comes once."""
+    g = torch.Generator().manual_seed(hq)
+    for n in (2, 9, 64, 65):
+        lens = (torch.rand(n, generator=g) ** 4 * 400).int().tolist()
+        lens_k = [max(x + int(e) - 90, 0) for x, e in zip(lens, torch.randint(0, 200, (n,), generator=g))]
+        q = heads(g, sum(lens), hq, 64, torch.bfloat16)
+        k, v = heads(g, sum(lens_k), hkv, 64, torch.bfloat16), heads(g, sum(lens_k), hkv, 64, torch.bfloat16)
+        check_prompt(q, k, v, lens, lens_k, causal)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("step", [0.05, 0.11, 0.12, 0.5, -0.11])
+def test_prompt_scores_that_creep_up(d, step):
+    """Each key's score lies `step` powers of two above the last one's: a tile's maximum rises by less and by more than what the
+    weights may grow by before they are taken from another reference."""
+    g = torch.Generator().manual_seed(int(step * 100) + d)
+    n = 333
+    q, k, v = heads(g, n, 2, d, torch.bfloat16), heads(g, n, 1, d, torch.bfloat16) / 64, heads(g, n, 1, d, torch.bfloat16)
+    q[:, :, 0] = 1
+    k[:, :, 0] = (step * math.log(2) * torch.arange(n)[:, None]).bfloat16()
+    check_prompt(q, k, v, [n], scale=1.0)
+
+
 def test_prompt_many_sequences_and_repeat():
     g = torch.Generator().manual_seed(9)
     lens = torch.randint(0, 9, (300,), generator=g).tolist()
