@@ -73,6 +73,7 @@ struct PromptArgs {
   const int32_t *cu_q, *cu_k;            // [sequences + 1]
   int64_t tokens, keys;
   int sequences, Hq, Hkv, D, dtype, causal;
+  Divider group;                         // heads of queries per head of keys
   float scale;
 };
 hipError_t launch_attention_prompt(const PromptArgs& p, hipStream_t s);

@@ -9,14 +9,16 @@
 // keys, so a row's maximum and sum are sums inside a lane and two exchanges between lanes, and exp2 of S^T is, without moving
 // between lanes, the second operand of O^T = V^T P^T: the k slots of that product are dealt to the keys in the order in which the
 // lane holds them, and V is read out of LDS with the transposing loads in the same order.
+#include <algorithm>
+
 #include "attention.h"
 #include "gemm_tile.h"
-#include "rows.h"
 
 namespace mslk_amd {
 namespace {
 
 constexpr int kBlockQ = 128, kTileK = 64, kHalfK = 32;
+constexpr int kGridY = 32768;   // blocks of queries per grid row
 
 // DP: head dimension rounded up to what the operands are padded to.
 template <int DP> struct Shape {
@@ -74,12 +76,12 @@ MSLK_AMD_DEVINL int wave_sum(int v) {   // over the lanes, in every lane
   return __builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16) + __builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48);
 }
 MSLK_AMD_DEVINL int wave_scan(int v, int lane) {   // inclusive sum
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int u = __shfl_up(v, d, 64);
-    if (lane >= d) v += u;
-  }
-  return v;
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // from 1, 2, 4, 8 lanes below, inside 16 lanes
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  const int a = __builtin_amdgcn_readlane(v, 15), b = a + __builtin_amdgcn_readlane(v, 31), c = b + __builtin_amdgcn_readlane(v, 47);
+  return v + (lane < 16 ? 0 : lane < 32 ? a : lane < 48 ? b : c);
 }
 
 // Block `index` of the packed queries: sequence by sequence, its last queries, which see the most keys, first; or, `sorted` (up to 64
@@ -169,6 +171,36 @@ MSLK_AMD_DEVINL bool any_wild(const char* rows, Swizzle swizzle) {
   return __ballot(max(top[0], top[1]) >= (F16 ? 0x7C00 : 0x7F80)) != 0;
 }
 
+// Rows of a head's keys or values from a tile's first one on, as a buffer: what lies beyond the last row is read as zeros.
+struct Rows {
+  uint64_t base;
+  uint32_t pitch, row_bytes;
+  int left;   // rows
+  v4i buffer;
+  MSLK_AMD_DEVINL Rows(const HeadRows& r, int64_t row, int head, int D, int rows)
+      : base(reinterpret_cast<uint64_t>(r.data + row * r.token_stride + (int64_t)head * r.head_stride)), pitch((uint32_t)r.token_stride * 2),
+        row_bytes((uint32_t)D * 2), left(rows) {
+    describe();
+  }
+  MSLK_AMD_DEVINL void describe() {
+    buffer = v4i{(int)(uint32_t)base, (int)(uint32_t)(base >> 32), left <= 0 ? 0 : (int)((uint32_t)(min(left, kTileK) - 1) * pitch + row_bytes), 0x00020000};
+  }
+  MSLK_AMD_DEVINL void next() {
+    base += (uint64_t)kTileK * pitch;
+    left -= kTileK;
+    describe();
+  }
+};
+
+constexpr uint32_t kOutside = 0xFFFFFF00u;   // of any buffer of 64 rows that are less than 2^26 bytes apart
+
+// 64 pieces of 16 bytes into LDS at `to`, `from` bytes into the buffer, lane after lane.  To the compiler it is a value made from
+// `token`, so that it can lie between matrix instructions and LDS reads can be moved past it; the fences in front of it and behind
+// it hold the token.
+MSLK_AMD_DEVINL void copy_piece(v4i buffer, uint32_t from, uint32_t to, int& token) {
+  asm("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : "+s"(token) : "v"(from), "s"(buffer), "s"(to) : "m0");
+}
+
 template <bool F16, int DP>
 __global__ __launch_bounds__(64 * Shape<DP>::kWaves, 2) void prompt_kernel(PromptArgs p, int blocks) {
   using E = Elem<F16>;
@@ -179,17 +211,10 @@ __global__ __launch_bounds__(64 * Shape<DP>::kWaves, 2) void prompt_kernel(Promp
   constexpr int kLoads = kTileBytes / 1024 / kWaves;           // wave-level copies of a tile per wave
   __shared__ __attribute__((aligned(1024))) char lds[4 * kTileBytes];   // keys, keys, values, values
 
-  const int64_t id = row_block();
-  if (id >= (int64_t)blocks * p.Hq) return;
-  int head, index;
-  if (p.Hkv % 8 == 0) {   // workgroup i runs on XCD i % 8: heads that share keys on one XCD
-    const int per = p.Hq / 8, i = (int)(id / 8);
-    head = (int)(id % 8) * per + i % per;
-    index = i / per;
-  } else {
-    head = (int)(id % p.Hq);
-    index = (int)(id / p.Hq);
-  }
+  int head = blockIdx.x;
+  const int index = blockIdx.y + blockIdx.z * kGridY;
+  if (index >= blocks) return;
+  if (p.Hkv % 8 == 0) head = head % 8 * (p.Hq / 8) + head / 8;   // workgroup i runs on XCD i % 8: heads that share keys on one XCD
   Work w;
   if (!find_work(p, index, p.sequences > 1 && p.sequences <= 64 && (int64_t)blocks * p.Hq <= kSortedBlocks, w)) return;
   w.q_row = uniform64(w.q_row);
@@ -203,36 +228,25 @@ __global__ __launch_bounds__(64 * Shape<DP>::kWaves, 2) void prompt_kernel(Promp
   const int col = lane & 15, group = lane >> 4;
   const int chunks = p.D / 8;   // 16-byte chunks of a row
 
-  const int kv_head = __builtin_amdgcn_readfirstlane(head / (p.Hq / p.Hkv));
-  const uint8_t* k_base = uniform_ptr(reinterpret_cast<const uint8_t*>(p.k.data + w.k_row * p.k.token_stride + (int64_t)kv_head * p.k.head_stride));
-  const uint8_t* v_base = uniform_ptr(reinterpret_cast<const uint8_t*>(p.v.data + w.k_row * p.v.token_stride + (int64_t)kv_head * p.v.head_stride));
+  const int kv_head = (int)divide((uint32_t)head, p.group);
   const uint32_t k_pitch = (uint32_t)p.k.token_stride * 2, v_pitch = (uint32_t)p.v.token_stride * 2;
   // Which 16-byte chunk of its row a slot of LDS holds: chosen so that the 16 (8-byte loads: 32) lanes that are served together find
   // their rows in different banks.
   auto k_swizzle = [](int r) { return kSlots == 8 ? (r >> 1) & 7 : r & 15; };
   auto v_swizzle = [](int r) { return kSlots == 8 ? r & 6 : (2 * r) & 14; };
 
-  // Copies of a tile: slot (row r, chunk c) of LDS holds chunk c ^ swizzle(r) of row r.  Rows beyond the last key repeat it, so
-  // that nothing of another sequence is ever multiplied; chunks beyond D repeat the last one (their queries are zero, and the
-  // columns of the output are dropped).
+  // Copies of a tile: slot (row r, chunk c) of LDS holds chunk c ^ swizzle(r) of row r.  Rows beyond the last key and chunks beyond D
+  // lie outside the buffer and come as zeros.
   constexpr int kRowsPerCopy = 64 / kSlots;
   uint32_t k_off[kLoads], v_off[kLoads];   // of this lane's pieces from a tile's first row
-  auto offsets = [&](uint32_t pitch, int valid, uint32_t (&off)[kLoads], auto swizzle) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      int slot = lane;
-      asm volatile("" : "+v"(slot));   // (once or twice per block: its parts are not worth registers)
-      const int r = (wave * kLoads + i) * kRowsPerCopy + slot / kSlots;
-      const int c = (slot % kSlots) ^ swizzle(r);
-      off[i] = (uint32_t)min(r, valid - 1) * pitch + (uint32_t)min(c, chunks - 1) * 16;
-    }
-  };
-  auto copy = [&](const uint8_t* tile, const uint32_t (&off)[kLoads], int buffer) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < kLoads; ++i)
-      dma16(tile, off[i], lds + __builtin_amdgcn_readfirstlane(buffer * kTileBytes + (wave * kLoads + i) * 1024));
-  };
-  const uint64_t k_step = (uint64_t)kTileK * k_pitch, v_step = (uint64_t)kTileK * v_pitch;
+  for (int i = 0; i < kLoads; ++i) {
+    const int r = (wave * kLoads + i) * kRowsPerCopy + lane / kSlots;
+    const int k_chunk = (lane % kSlots) ^ k_swizzle(r), v_chunk = (lane % kSlots) ^ v_swizzle(r);
+    k_off[i] = k_chunk < chunks ? (uint32_t)r * k_pitch + (uint32_t)k_chunk * 16 : kOutside;
+    v_off[i] = v_chunk < chunks ? (uint32_t)r * v_pitch + (uint32_t)v_chunk * 16 : kOutside;
+  }
+  const uint32_t lds_wave = __builtin_amdgcn_readfirstlane((int)(uint32_t)(uintptr_t)(lds_ptr_t)lds + wave * kLoads * 1024);
 
   const int wave_row = kWaveQ * wave;
   const int seen = min(w.keys, w.q0 + w.rows + w.shift);                   // keys that the block's last query sees
@@ -244,10 +258,17 @@ __global__ __launch_bounds__(64 * Shape<DP>::kWaves, 2) void prompt_kernel(Promp
   const int whole = min(min(w.keys, w.q0 + w.shift + 1) / kTileK, tiles);  // tiles that every query of the block sees whole
   const float c = p.scale * kLog2e, slack = 8.f / c;
 
+  Rows k_rows(p.k, w.k_row, kv_head, p.D, min(w.keys, tiles * kTileK)), v_rows(p.v, w.k_row, kv_head, p.D, min(w.keys, tiles * kTileK));
+  int token = 0;
+  auto piece = [&](int i, int parity) {   // copies 0 to kLoads - 1: values of the next tile; from kLoads on: keys of the one after it
+    if (i < kLoads) copy_piece(v_rows.buffer, v_off[i], lds_wave + (2 + (parity ^ 1)) * kTileBytes + i * 1024, token);
+    else copy_piece(k_rows.buffer, k_off[i - kLoads], lds_wave + parity * kTileBytes + (i - kLoads) * 1024, token);
+  };
   if (tiles > 0) {
-    offsets(k_pitch, w.keys, k_off, k_swizzle);
-    offsets(v_pitch, w.keys, v_off, v_swizzle);
-    copy(k_base, k_off, 0);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) piece(kLoads + i, 0);
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) piece(i, 1);
   }
   // queries: lane (col, group) holds channels 32 step + 8 group ... + 7 of query wave_row + 16 b + col; zeros beyond D
   v4i q[kB][kSteps];
@@ -272,24 +293,16 @@ __global__ __launch_bounds__(64 * Shape<DP>::kWaves, 2) void prompt_kernel(Promp
     l[b] = 0.f;
   }
 
-  auto fetch = [&](int t) __attribute__((always_inline)) {   // values of the next tile, keys of the one after it
-    if (t + 1 < tiles) {
-      v_base += v_step;
-      if ((t + 2) * kTileK > w.keys) [[unlikely]] offsets(v_pitch, w.keys - (t + 1) * kTileK, v_off, v_swizzle);
-      copy(v_base, v_off, 2 + ((t + 1) & 1));
-    }
-    if (t + 2 < tiles) {
-      k_base += k_step;
-      if ((t + 3) * kTileK > w.keys) [[unlikely]] offsets(k_pitch, w.keys - (t + 2) * kTileK, k_off, k_swizzle);
-      copy(k_base, k_off, t & 1);
-    }
+  auto next = [&] {
+    v_rows.next();
+    k_rows.next();
   };
   auto fence = [&] {   // this wave's copies are in LDS and its reads are done; so are the other waves'
     __builtin_amdgcn_sched_barrier(0);
-    asm volatile("" ::: "memory");
+    asm volatile("" : "+s"(token) : : "memory");
     __builtin_amdgcn_s_waitcnt(0x0070);   // vmcnt(0) lgkmcnt(0)
     __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
+    asm volatile("" : "+s"(token) : : "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
 
@@ -383,13 +396,10 @@ __global__ __launch_bounds__(64 * Shape<DP>::kWaves, 2) void prompt_kernel(Promp
   };
 
   if (tiles > 0) {
-    copy(v_base, v_off, 2);
-    if (tiles > 1) {
-      k_base += k_step;
-      if (2 * kTileK > w.keys) offsets(k_pitch, w.keys - kTileK, k_off, k_swizzle);
-      copy(k_base, k_off, 1);
-    }
     fence();
+    k_rows.next();
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) piece(kLoads + i, 1);
     scores(0, 0);
     scores(0, 1);
     const int pairs = max((whole - 1) / 2, 0);   // of tiles that are whole, and so is the next
@@ -398,7 +408,9 @@ __global__ __launch_bounds__(64 * Shape<DP>::kWaves, 2) void prompt_kernel(Promp
       for (int y = 0; y < 2; ++y) {
         softmax();
         fence();
-        fetch(2 * i + y);
+        next();
+#pragma unroll
+        for (int j = 0; j < 2 * kLoads; ++j) piece(j, y);
         product(y, 0, same);
         product(y, 1, same);
         scores(y ^ 1, 0);
@@ -424,7 +436,11 @@ __global__ __launch_bounds__(64 * Shape<DP>::kWaves, 2) void prompt_kernel(Promp
         softmax();
       }
       fence();
-      fetch(t);
+      next();
+      if (t + 1 < tiles) {
+#pragma unroll
+        for (int i = 0; i < 2 * kLoads; ++i) piece(i, t & 1);
+      }
       if (t < wave_tiles) {
         const char* vb = lds + (2 + (t & 1)) * kTileBytes;
 #pragma unroll
@@ -469,23 +485,29 @@ __global__ __launch_bounds__(64 * Shape<DP>::kWaves, 2) void prompt_kernel(Promp
   for (int b = 0; b < kB; ++b) {
     const int row = wave_row + 16 * b + col;
     const float total = sum_rows16(l[b]);
-    if (row >= w.rows) continue;
     const float inv = total == 0.f ? 0.f : 1.f / total;
     uint16_t* dst = p.out + ((w.q_row + row) * p.Hq + head) * p.D;
 #pragma unroll
-    for (int d = 0; d < kBlocksD; ++d) {
-      const int ch = 16 * d + 4 * group;
-      if (ch < p.D)
-        *reinterpret_cast<v2i*>(dst + ch) = v2i{(int)E::pack(o[b][d][0] * inv, o[b][d][1] * inv), (int)E::pack(o[b][d][2] * inv, o[b][d][3] * inv)};
+    for (int d = 0; d < kBlocksD; d += 2) {   // neighbours in `group` exchange halves of two blocks of 16 channels: 16 bytes per lane
+      v4i x;
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const auto two = __builtin_amdgcn_permlane16_swap(E::pack(o[b][d][2 * y] * inv, o[b][d][2 * y + 1] * inv),
+                                                          E::pack(o[b][d + 1][2 * y] * inv, o[b][d + 1][2 * y + 1] * inv), false, false);
+        x[y] = (int)two[0];
+        x[2 + y] = (int)two[1];
+      }
+      const int ch = 16 * (d + (group & 1)) + 8 * (group / 2);
+      if (row < w.rows && ch < p.D) *reinterpret_cast<v4i*>(dst + ch) = x;
     }
-    if (group == 0) p.lse[(w.q_row + row) * p.Hq + head] = total == 0.f ? -__builtin_inff() : m[b] * p.scale + log2_fast(total) * kLn2;
+    if (group == 0 && row < w.rows) p.lse[(w.q_row + row) * p.Hq + head] = total == 0.f ? -__builtin_inff() : m[b] * p.scale + log2_fast(total) * kLn2;
   }
 }
 
 template <bool F16, int DP>
 hipError_t launch(const PromptArgs& p, hipStream_t s) {
   const int64_t blocks = p.tokens / kBlockQ + (p.sequences < p.tokens ? p.sequences : p.tokens) + 2;
-  hipLaunchKernelGGL((prompt_kernel<F16, DP>), row_grid(blocks * p.Hq), dim3(64 * Shape<DP>::kWaves), 0, s, p, (int)blocks);
+  hipLaunchKernelGGL((prompt_kernel<F16, DP>), dim3((unsigned)p.Hq, (unsigned)std::min<int64_t>(blocks, kGridY), (unsigned)((blocks + kGridY - 1) / kGridY)), dim3(64 * Shape<DP>::kWaves), 0, s, p, (int)blocks);
   return hipGetLastError();
 }
 

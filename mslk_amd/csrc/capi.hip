@@ -600,6 +600,7 @@ int mslk_amd_attention_prompt(const mslk_amd_heads* q, const mslk_amd_heads* k, 
   p.sequences = (int)sequences;
   p.Hq = (int)Hq; p.Hkv = (int)Hkv; p.D = (int)D; p.dtype = dtype;
   p.causal = causal != 0;
+  p.group = divider((uint32_t)(Hq / Hkv));
   p.scale = scale;
   return check_hip(launch_attention_prompt(p, (hipStream_t)stream), "attention_prompt launch");
 }
