@@ -149,6 +149,7 @@ __global__ __launch_bounds__(64, STEPS <= 4 ? 2 : 1) void decode_kernel(DecodeAr
   using value_t = typename RowTraits<ROWS>::value_t;
   constexpr bool FP8 = ROWS != kRows16Bit;
   constexpr int kDP = 128 * SETS, kElem = FP8 ? 1 : 2;
+  constexpr int kLeast = STEPS == 2 ? 1 : STEPS == 3 ? 65 : STEPS == 4 ? (FP8 ? 65 : 97) : STEPS == 6 ? 129 : 193;   // smallest D
   constexpr int kPer = ROWS == kRowsE4m3 ? 2 : 1;            // steps of a piece of a key: channels 32 kPer x + 8 kPer g + 8 y ... + 7 in step
   static_assert(STEPS % kPer == 0, "pieces cover whole steps");   // kPer x + y of lane (i, g)
   const int key_pieces = p.D / (8 * kPer);
@@ -234,13 +235,18 @@ __global__ __launch_bounds__(64, STEPS <= 4 ? 2 : 1) void decode_kernel(DecodeAr
     float m = -__builtin_inff(), l = 0.f;
     auto compute = [&](const Tile& t, int key0) {
       v4f s[2] = {v4f{}, v4f{}};
+      // A piece of a key.  Channels beyond D: zeros of q would not silence an infinity that was read in their place.
+      auto key_piece = [&](int b, int x) {
+        if (32 * kPer * (x + 1) <= kLeast || 4 * x + g < key_pieces) return t.k[b][x];
+        return key_t{};
+      };
 #pragma unroll
       for (int x = 0; x < STEPS; ++x)
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          if constexpr (ROWS == kRows16Bit) s[b] = E::mfma16(t.k[b][x], q[x], s[b]);
-          else if constexpr (ROWS == kRowsE4m3By8) s[b] = E::mfma16(widen<F16>(t.k[b][x]), q[x], s[b]);
-          else s[b] = E::mfma16(widen<F16>(v2i{t.k[b][x / 2][2 * (x % 2)], t.k[b][x / 2][2 * (x % 2) + 1]}), q[x], s[b]);
+          if constexpr (ROWS == kRows16Bit) s[b] = E::mfma16(key_piece(b, x), q[x], s[b]);
+          else if constexpr (ROWS == kRowsE4m3By8) s[b] = E::mfma16(widen<F16>(key_piece(b, x)), q[x], s[b]);
+          else s[b] = E::mfma16(widen<F16>(v2i{key_piece(b, x / 2)[2 * (x % 2)], key_piece(b, x / 2)[2 * (x % 2) + 1]}), q[x], s[b]);
         }
       float e[8], vs[8], lg = 0.f;
       if constexpr (FP8) lg = fminf(fmaxf(log2_fast(t.scale), -60.f), 60.f);
@@ -258,14 +264,11 @@ __global__ __launch_bounds__(64, STEPS <= 4 ? 2 : 1) void decode_kernel(DecodeAr
         for (int j = 0; j < 8; ++j)
           if (t.bad >> (16 * g + j) & 1) e[j] = __builtin_nanf("");
       }
-      const bool cut = key0 + kTile > key_end;
-      if (cut) {
+      if (key0 + kTile > key_end) {   // n copies of the last key: 1 / n of its weight each (none, and an infinite value would give NaN)
+        const float share = log2_fast((float)(key0 + kTile - key_end + 1));
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          if (key0 + key_of(j, g) >= key_end) {
-            e[j] = -__builtin_inff();
-            vs[j] = 0.f;
-          }
+          if (key0 + key_of(j, g) >= key_end - 1) e[j] -= share;
       }
       float top = m;
       each8([&](auto jj) {

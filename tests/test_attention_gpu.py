@@ -178,6 +178,26 @@ def test_prompt_scores_far_apart():
     check_prompt(q, k, v, [500], scale=1e-4, causal=False)
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d", [64, 72, 80, 200])
+def test_prompt_infinite_keys_and_values(d, causal):
+    """Keys that score minus infinity weigh nothing; an infinite value of the last key makes its channel infinite where it is seen."""
+    g = torch.Generator().manual_seed(d)
+    n = 150
+    q, k, v = (heads(g, n, 2, d, torch.bfloat16) for _ in range(3))
+    q[:, :, -1] = q[:, :, -1].abs() + 1
+    gone = torch.zeros(n, dtype=torch.bool)
+    gone[10:20] = gone[70:140] = True
+    visible = (causal_mask(n, n) if causal else torch.ones(n, n, dtype=torch.bool)) & ~gone
+    out, lse, bound, lse_bound = attention(q, k, v, d ** -0.5, visible)
+    k[gone, :, -1] = -math.inf
+    v[n - 1, 0, 3] = math.inf
+    out[visible[:, n - 1], 0, 3] = math.inf
+    got = mslk_amd.attention_prompt(*(x.to(DEV) for x in (q, k, v)), offsets([n]).to(DEV), causal=causal, return_lse=True)
+    near(got[0], out, bound)
+    near(got[1], lse, lse_bound)
+
+
 def test_prompt_strides_and_alignment():
     g = torch.Generator().manual_seed(7)
     t, hq, hkv, d = 210, 6, 2, 96
@@ -391,6 +411,27 @@ def test_decode_wild_values_touch_their_sequence_only():
     out = mslk_amd.attention_decode(q.to(DEV), *Cache(g, [100, 70], 2, 64, 16, torch.bfloat16, rows=rows).on_gpu()).cpu()
     assert (out[0, 2:, 2] == math.inf).all() and torch.isnan(out[0, :2, 3]).all()
     assert torch.isfinite(out).sum() == out.numel() - 4
+
+
+@pytest.mark.parametrize("d", [64, 72, 80, 136, 200])
+def test_decode_infinite_keys_and_values(d):
+    """Keys that score minus infinity weigh nothing; an infinite value of the last key makes its channel infinite, not NaN."""
+    g = torch.Generator().manual_seed(d)
+    lens = [33, 100, 2500]
+    rows = [[heads(g, n, 2, d, torch.bfloat16) for n in lens] for _ in range(2)]
+    q = heads(g, 3, 4, d, torch.bfloat16)
+    q[:, :, -1] = q[:, :, -1].abs() + 1
+    want = []
+    for b, n in enumerate(lens):
+        gone = (torch.arange(n) >= n // 3) & (torch.arange(n) < n // 3 + 20)
+        want.append(attention(q[b:b + 1], rows[0][b], rows[1][b], d ** -0.5, ~gone[None]))
+        rows[0][b][gone, :, -1] = -math.inf
+        rows[1][b][n - 1, 1, 5] = math.inf
+        want[b][0][0, 2:, 5] = math.inf
+    got = mslk_amd.attention_decode(q.to(DEV), *Cache(g, lens, 2, d, 16, torch.bfloat16, rows=rows).on_gpu(), return_lse=True)
+    for b, (out, lse, bound, lse_bound) in enumerate(want):
+        near(got[0][b:b + 1], out, bound)
+        near(got[1][b:b + 1], lse, lse_bound)
 
 
 def test_decode_long_and_offsets_beyond_32_bits():
