@@ -4,7 +4,7 @@
 // tile of keys s = q k, l' = l 2^(c(m - m')) + sum 2^(c(s - m')), O' = O 2^(c(m - m')) + 2^(c(s - m')) V with c = scale log2(e), and
 // O / l at the end.
 //
-// A workgroup of four waves takes 128 queries of one head, a wave 32 of them; tiles of 64 keys and values are copied into LDS, two of
+// A workgroup takes 128 or 64 queries of one head, a wave 32 or 16 of them; tiles of 64 keys and values are copied into LDS, two of
 // each.  Both products are v_mfma_f32_16x16x32 with the keys first: S^T = K Q^T leaves a lane one query and a quarter of the tile's
 // keys, so a row's maximum and sum are sums inside a lane and two exchanges between lanes, and exp2 of S^T is, without moving
 // between lanes, the second operand of O^T = V^T P^T: the k slots of that product are dealt to the keys in the order in which the
@@ -17,13 +17,13 @@
 namespace mslk_amd {
 namespace {
 
-constexpr int kBlockQ = 128, kTileK = 64, kHalfK = 32;
+constexpr int kTileK = 64, kHalfK = 32;
 constexpr int kGridY = 32768;   // blocks of queries per grid row
 
-// DP: head dimension rounded up to what the operands are padded to.
-template <int DP> struct Shape {
-  static constexpr int kB = DP <= 128 ? 2 : 1;   // blocks of 16 queries per wave
-  static constexpr int kWaveQ = 16 * kB, kWaves = kBlockQ / kWaveQ;
+// DP: head dimension rounded up to what the operands are padded to.  Q: queries of a workgroup.
+template <int DP, int Q> struct Shape {
+  static constexpr int kB = DP <= 128 && Q == 128 ? 2 : 1;   // blocks of 16 queries per wave
+  static constexpr int kWaveQ = 16 * kB, kWaves = Q / kWaveQ;
 };
 
 typedef short v4s __attribute__((ext_vector_type(4)));
@@ -36,10 +36,10 @@ struct Work {
   int q0, rows, keys, shift;
 };
 
-// A sequence of the packed queries and its keys.
-struct Sequence {
+// A sequence of the packed queries and its keys; blocks of Q queries.
+template <int Q> struct Sequence {
   int start, len, k_start, k_len;
-  MSLK_AMD_DEVINL int blocks() const { return (len + kBlockQ - 1) / kBlockQ; }
+  MSLK_AMD_DEVINL int blocks() const { return (len + Q - 1) / Q; }
   // Blocks that visit at least `tiles` tiles of keys: the last ones.
   MSLK_AMD_DEVINL int blocks_of(int tiles, bool causal) const {
     const int n = blocks();
@@ -47,7 +47,7 @@ struct Sequence {
     const uint32_t keys = (uint32_t)(tiles - 1) * kTileK + 1;   // the last query has to see this many
     if (keys > (uint32_t)k_len) return 0;
     const int queries = (int)keys - (k_len - len);
-    return !causal || queries <= 0 ? n : n - (queries - 1) / kBlockQ;
+    return !causal || queries <= 0 ? n : n - (queries - 1) / Q;
   }
 };
 
@@ -55,8 +55,9 @@ MSLK_AMD_DEVINL int clamp_offset(int v, int64_t limit) { return (int)min((int64_
 MSLK_AMD_DEVINL int64_t uniform64(int64_t v) {
   return ((int64_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)v);
 }
-MSLK_AMD_DEVINL Sequence sequence(const PromptArgs& p, int b) {
-  Sequence s{0, 0, 0, 0};
+template <int Q>
+MSLK_AMD_DEVINL Sequence<Q> sequence(const PromptArgs& p, int b) {
+  Sequence<Q> s{0, 0, 0, 0};
   if (b >= p.sequences) return s;
   s.start = clamp_offset(p.cu_q[b], p.tokens);
   s.len = max(clamp_offset(p.cu_q[b + 1], p.tokens) - s.start, 0);
@@ -93,11 +94,12 @@ MSLK_AMD_DEVINL int wave_scan(int v, int lane) {   // inclusive sum
 // 184.4, 4800 317 / 313; 6000 tokens in 13 sequences, not causal, D = 96, 976 workgroups 46.8 / 51.4, 1952 88.4 / 93.6, 3904 165.3 /
 // 160.8; but 4873 tokens in 8 sequences, causal, 1536 workgroups 79.8 / 76.7.
 constexpr int kSortedBlocks = 2048;
+template <int Q>
 MSLK_AMD_DEVINL bool find_work(const PromptArgs& p, int index, bool sorted, Work& w) {
   const int lane = threadIdx.x & 63;
   int before = 0;   // blocks of the sequences looked at so far
   for (int base = 0; base < p.sequences; base += 64) {
-    const Sequence s = sequence(p, base + lane);
+    const Sequence<Q> s = sequence<Q>(p, base + lane);
     const int n = s.blocks();
     int src = -1, block = 0;
     if (sorted) {
@@ -131,8 +133,8 @@ MSLK_AMD_DEVINL bool find_work(const PromptArgs& p, int index, bool sorted, Work
       const int len = __builtin_amdgcn_readlane(s.len, src);
       w.keys = __builtin_amdgcn_readlane(s.k_len, src);
       w.k_row = __builtin_amdgcn_readlane(s.k_start, src);
-      w.q0 = block * kBlockQ;
-      w.rows = min(len - w.q0, kBlockQ);
+      w.q0 = block * Q;
+      w.rows = min(len - w.q0, Q);
       w.q_row = __builtin_amdgcn_readlane(s.start, src) + w.q0;
       w.shift = p.causal ? w.keys - len : w.keys;   // not causal: every query sees everything
       return true;
@@ -140,13 +142,13 @@ MSLK_AMD_DEVINL bool find_work(const PromptArgs& p, int index, bool sorted, Work
   }
   // tokens of no sequence
   const int head = clamp_offset(p.cu_q[0], p.tokens), tail = clamp_offset(p.cu_q[p.sequences], p.tokens);
-  const int head_blocks = (head + kBlockQ - 1) / kBlockQ;
+  const int head_blocks = (head + Q - 1) / Q;
   index -= before;
   const bool front = index < head_blocks;
   if (!front) index -= head_blocks;
-  const int64_t from = (front ? 0 : tail) + (int64_t)index * kBlockQ, to = front ? head : p.tokens;
+  const int64_t from = (front ? 0 : tail) + (int64_t)index * Q, to = front ? head : p.tokens;
   if (from >= to) return false;
-  w = Work{from, 0, 0, (int)min(to - from, (int64_t)kBlockQ), 0, -1};
+  w = Work{from, 0, 0, (int)min(to - from, (int64_t)Q), 0, -1};
   return true;
 }
 
@@ -201,10 +203,11 @@ MSLK_AMD_DEVINL void copy_piece(v4i buffer, uint32_t from, uint32_t to, int& tok
   asm("s_mov_b32 m0, %3\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" : "+s"(token) : "v"(from), "s"(buffer), "s"(to) : "m0");
 }
 
-template <bool F16, int DP>
-__global__ __launch_bounds__(64 * Shape<DP>::kWaves, 2) void prompt_kernel(PromptArgs p, int blocks) {
+template <bool F16, int DP, int Q>
+__global__ __launch_bounds__((64 * Shape<DP, Q>::kWaves), 2) void prompt_kernel(PromptArgs p, int blocks) {
   using E = Elem<F16>;
-  constexpr int kB = Shape<DP>::kB, kWaveQ = Shape<DP>::kWaveQ, kWaves = Shape<DP>::kWaves;
+  using S = Shape<DP, Q>;
+  constexpr int kB = S::kB, kWaveQ = S::kWaveQ, kWaves = S::kWaves;
   constexpr int kSlots = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;   // 16-byte chunks of a row in LDS, a power of two
   constexpr int kRowBytes = kSlots * 16, kTileBytes = kTileK * kRowBytes;
   constexpr int kSteps = DP / 32, kBlocksD = DP / 16;
@@ -216,7 +219,7 @@ __global__ __launch_bounds__(64 * Shape<DP>::kWaves, 2) void prompt_kernel(Promp
   if (index >= blocks) return;
   if (p.Hkv % 8 == 0) head = head % 8 * (p.Hq / 8) + head / 8;   // workgroup i runs on XCD i % 8: heads that share keys on one XCD
   Work w;
-  if (!find_work(p, index, p.sequences > 1 && p.sequences <= 64 && (int64_t)blocks * p.Hq <= kSortedBlocks, w)) return;
+  if (!find_work<Q>(p, index, p.sequences > 1 && p.sequences <= 64 && (int64_t)blocks * p.Hq <= kSortedBlocks, w)) return;
   w.q_row = uniform64(w.q_row);
   w.k_row = uniform64(w.k_row);
   w.q0 = __builtin_amdgcn_readfirstlane(w.q0);
@@ -504,11 +507,24 @@ __global__ __launch_bounds__(64 * Shape<DP>::kWaves, 2) void prompt_kernel(Promp
   }
 }
 
+template <bool F16, int DP, int Q>
+hipError_t launch(const PromptArgs& p, int64_t blocks, hipStream_t s) {
+  hipLaunchKernelGGL((prompt_kernel<F16, DP, Q>), dim3((unsigned)p.Hq, (unsigned)std::min<int64_t>(blocks, kGridY), (unsigned)((blocks + kGridY - 1) / kGridY)),
+                     dim3(64 * Shape<DP, Q>::kWaves), 0, s, p, (int)blocks);
+  return hipGetLastError();
+}
+// Few workgroups of 128 queries (up to two per CU, or one where LDS holds no second) leave the matrix cores waiting for one another's
+// softmax and the last workgroup long: blocks of 64 queries then, in waves of 16, though LDS is read twice as often.  128 against 64, us:
+// D = 128 on 32 heads, causal: 100 tokens (96 workgroups) 8.5 / 6.5, 256 (160) 12.5 / 8.4, 500 (192) 17.2 / 11.7, 1000 (320) 27.0 / 20.1,
+// 1400 (448) 37.7 / 28.7, 2048 (608) 52.4 / 51.0; 20 sequences of 100 on 16 heads (592) 12.4 / 14.1; 6000 tokens in 13 sequences on 16
+// heads (976) 47 / 57.  D = 256, 1000 tokens: 16 heads (160) 36.5 / 31.3, 32 heads (320) 39.0 / 41.1.
+template <int DP> constexpr int kFewBlocks = DP <= 128 ? 512 : 256;
 template <bool F16, int DP>
 hipError_t launch(const PromptArgs& p, hipStream_t s) {
-  const int64_t blocks = p.tokens / kBlockQ + (p.sequences < p.tokens ? p.sequences : p.tokens) + 2;
-  hipLaunchKernelGGL((prompt_kernel<F16, DP>), dim3((unsigned)p.Hq, (unsigned)std::min<int64_t>(blocks, kGridY), (unsigned)((blocks + kGridY - 1) / kGridY)), dim3(64 * Shape<DP>::kWaves), 0, s, p, (int)blocks);
-  return hipGetLastError();
+  const int64_t parts = std::min<int64_t>(p.sequences, p.tokens) + 2;
+  const int64_t blocks = p.tokens / 128 + parts;
+  if (blocks * p.Hq <= kFewBlocks<DP>) return launch<F16, DP, 64>(p, p.tokens / 64 + parts, s);
+  return launch<F16, DP, 128>(p, blocks, s);
 }
 
 template <bool F16>

@@ -228,6 +228,28 @@ def test_prompt_long():
     near(lse[rows.to(DEV)], want[1], want[3])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [40, 64, 80, 96, 128, 160, 192, 256])
+def test_prompt_many_heads(d, dtype):
+    """As many heads as fill the machine: the larger blocks of queries."""
+    g = torch.Generator().manual_seed(d)
+    lens = [257, 1, 77]
+    q, k, v = heads(g, sum(lens), 120, d, dtype), heads(g, sum(lens), 8, d, dtype), heads(g, sum(lens), 8, d, dtype)
+    v[250, 0, 3] = math.nan if dtype == torch.float16 else math.inf      # hidden from all rows of its head but the last of a sequence
+    k[257 + 1 + 60, 1, 5] = math.inf
+    seen = [x.clone() for x in (k, v)]
+    seen[0][257 + 1 + 60:, 1] = 0
+    seen[1][250:257, 0] = 0
+    out, lse = mslk_amd.attention_prompt(q.to(DEV), k.to(DEV), v.to(DEV), offsets(lens).to(DEV), return_lse=True)
+    at = 0
+    for n in lens:
+        want = attention(q[at:at + n], seen[0][at:at + n], seen[1][at:at + n], d ** -0.5, causal_mask(n, n))
+        upto = n - 7 if n == 257 else 60 if n == 77 else n               # rows in front of the wild ones
+        for got, w, bound in ((out, want[0], want[2]), (lse, want[1], want[3])):
+            near(got[at:at + upto], w[:upto], bound[:upto])
+        at += n
+
+
 @pytest.mark.parametrize("hq,hkv", [(2, 1), (8, 8), (48, 16)])
 @pytest.mark.parametrize("causal", [True, False])
 def test_prompt_ragged_batches(hq, hkv, causal):
