@@ -87,9 +87,6 @@ typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
 template <bool F16> struct Elem;
 template <> struct Elem<false> {
-  MSLK_AMD_DEVINL static v16f mfma32(v4i a, v4i b, v16f c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
-  }
   MSLK_AMD_DEVINL static v4f mfma16(v4i a, v4i b, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
   }
@@ -98,9 +95,6 @@ template <> struct Elem<false> {
   MSLK_AMD_DEVINL static float hi(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 };
 template <> struct Elem<true> {
-  MSLK_AMD_DEVINL static v16f mfma32(v4i a, v4i b, v16f c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
-  }
   MSLK_AMD_DEVINL static v4f mfma16(v4i a, v4i b, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c, 0, 0, 0);
   }
@@ -116,11 +110,7 @@ constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f
 MSLK_AMD_DEVINL float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 MSLK_AMD_DEVINL float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
 
-// Value of the lane whose number differs in bit 5 / bit 4.
-MSLK_AMD_DEVINL float other_half(float x) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
-}
+// Over the two halves of the wave.
 MSLK_AMD_DEVINL float max_halves(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
