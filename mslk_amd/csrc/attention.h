@@ -110,6 +110,23 @@ constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f
 MSLK_AMD_DEVINL float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 MSLK_AMD_DEVINL float log2_fast(float x) { return __builtin_amdgcn_logf(x); }
 
+// Over the lanes of a wave.
+MSLK_AMD_DEVINL int wave_sum(int v) {   // in every lane
+  v += __builtin_amdgcn_update_dpp(0, v, 0x128, 0xF, 0xF, false);   // rotated by 8 inside 16 lanes, ...
+  v += __builtin_amdgcn_update_dpp(0, v, 0x124, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x122, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x121, 0xF, 0xF, false);
+  return __builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16) + __builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48);
+}
+MSLK_AMD_DEVINL int wave_scan(int v, int lane) {   // inclusive sum
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // from 1, 2, 4, 8 lanes below, inside 16 lanes
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  const int a = __builtin_amdgcn_readlane(v, 15), b = a + __builtin_amdgcn_readlane(v, 31), c = b + __builtin_amdgcn_readlane(v, 47);
+  return v + (lane < 16 ? 0 : lane < 32 ? a : lane < 48 ? b : c);
+}
+
 // Over the two halves of the wave.
 MSLK_AMD_DEVINL float max_halves(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);

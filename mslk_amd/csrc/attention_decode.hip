@@ -26,6 +26,7 @@ constexpr int kMostParts = 2048, kLongParts = 1024;
 
 struct Line {          // how the work is divided
   int head_blocks;     // per sequence: KV heads x blocks of kHeads query heads
+  Divider by_head_blocks;
   int per_kv;          // blocks of query heads per KV head
   int group;           // query heads per KV head
   int parts;
@@ -39,15 +40,6 @@ MSLK_AMD_DEVINL int length_of(const DecodeArgs& p, int b) {
 }
 MSLK_AMD_DEVINL int tiles_of(int len) { return max(1, (len + kTile - 1) / kTile); }
 
-MSLK_AMD_DEVINL int wave_scan(int v, int lane) {   // inclusive sum over the lanes
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int u = __shfl_up(v, d, 64);
-    if (lane >= d) v += u;
-  }
-  return v;
-}
-
 // Part `w` of the line: tiles [begin, end), the sequence that holds the first of them and the tiles in front of that sequence.  (A line
 // has fewer than 2^31 tiles; 64-bit divisions would take longer than a tile.)
 struct Part {
@@ -59,15 +51,12 @@ MSLK_AMD_DEVINL bool find_part(const DecodeArgs& p, const Line& ln, int w, Part&
   int n = lane < p.sequences ? tiles_of(len) : 0, upto = wave_scan(n, lane);
   uint32_t total = __builtin_amdgcn_readlane(upto, 63);
   for (int base = 64; base < p.sequences; base += 64) {
-    int more = base + lane < p.sequences ? tiles_of(length_of(p, base + lane)) : 0;
-#pragma unroll
-    for (int d = 32; d >= 1; d /= 2) more += __shfl_xor(more, d, 64);
-    total += __builtin_amdgcn_readfirstlane(more);
+    total += wave_sum(base + lane < p.sequences ? tiles_of(length_of(p, base + lane)) : 0);
   }
   total *= ln.head_blocks;
   const uint32_t parts = total <= kMostParts ? total : kLongParts;   // none of them empty
   if ((uint32_t)w >= parts) return false;
-  const uint32_t each = total / parts, more = total - each * parts;   // the first `more` parts hold one tile more
+  const uint32_t each = parts == total ? 1 : total / parts, more = total - each * parts;   // the first `more` parts hold one tile more
   r.begin = w * each + min((uint32_t)w, more);
   r.end = r.begin + each + ((uint32_t)w < more ? 1 : 0);
   r.before = 0;
@@ -402,42 +391,46 @@ __global__ __launch_bounds__(64, STEPS <= 4 ? 2 : 1) void decode_kernel(DecodeAr
 
 // Joins the pieces of a head block where there is more than one.  Workgroup (x, y): `per` heads of head block x, from y * per on.  A team
 // of kDP / 4 lanes, four channels each, sums the pieces of a head, or every n-th of them where there are fewer heads than teams.
+typedef float v2f __attribute__((ext_vector_type(2)));
 constexpr int kJoinThreads = 256;
 template <bool F16, int SETS>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(DecodeArgs p, Line ln, int per) {
   using E = Elem<F16>;
   constexpr int kDP = 128 * SETS, kLanes = kDP / 4, kTeams = kJoinThreads / kLanes, kPiece = kHeads * (kDP + 2);
   __shared__ __attribute__((aligned(16))) float sums[kTeams][kDP];
+  __shared__ v2f weights[kTeams];
   const int lane = threadIdx.x % kLanes, team = threadIdx.x / kLanes;
-  const int seq = blockIdx.x / ln.head_blocks, hb = blockIdx.x - seq * ln.head_blocks;
+  const int seq = (int)divide(blockIdx.x, ln.by_head_blocks), hb = blockIdx.x - seq * ln.head_blocks;
   const int first = p.ends[2 * (int64_t)blockIdx.x], last = p.ends[2 * (int64_t)blockIdx.x + 1];
   if (first == last) return;   // one piece: its wave has written the result
   const int pieces = last / 2 - first / 2 + 1;
-  const int kv_head = hb / ln.per_kv, from = (hb - kv_head * ln.per_kv) * kHeads, heads = min(ln.group - from, kHeads);
+  const int kv_head = ln.per_kv == 1 ? hb : hb / ln.per_kv, from = (hb - kv_head * ln.per_kv) * kHeads, heads = min(ln.group - from, kHeads);
   const int h0 = blockIdx.y * per, hn = min(per, heads - h0);
   if (hn <= 0) return;
   // piece 0 lies in slot `first`, piece i in the first slot of its wave
   const auto piece = [&](int i) { return p.partial + (int64_t)(i == 0 ? first : (first & ~1) + 2 * i) * kPiece; };
-  const int groups = max(kTeams / hn, 1), share = min(hn, kTeams);
-  const int mine = team % share, group = team / share;   // (teams left over repeat the last group's work and store nothing)
+  const int groups = hn == 1 ? kTeams : max(kTeams / hn, 1), share = min(hn, kTeams);
+  const int group = share == 1 ? team : team / share, mine = team - group * share;   // (teams left over repeat the last group's work and store nothing)
   for (int h = h0 + mine; h < h0 + hn; h += share) {
+    // One pass, a reference that follows the maximum: nothing that is loaded waits for anything but `ends`.
     float top = -__builtin_inff(), total = 0.f;
-    for (int i = lane; i < pieces; i += kLanes) top = fmaxf(top, piece(i)[kHeads * kDP + h]);
-#pragma unroll
-    for (int d = kLanes / 2; d >= 1; d /= 2) top = fmaxf(top, __shfl_xor(top, d, 64));
-    const float base = top == -__builtin_inff() ? 0.f : top;
-    for (int i = lane; i < pieces; i += kLanes) total += exp2_fast(piece(i)[kHeads * kDP + h] - base) * piece(i)[kHeads * kDP + kHeads + h];
-#pragma unroll
-    for (int d = kLanes / 2; d >= 1; d /= 2) total += __shfl_xor(total, d, 64);
     v4f acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
+    const auto add = [&](float m, float l, v4f o) {
+      const float next = fmaxf(top, m), base = next == -__builtin_inff() ? 0.f : next;
+      const float a = exp2_fast(top - base), b = exp2_fast(m - base);
+      total = total * a + l * b;
+      acc = acc * a + o * b;
+      top = next;
+    };
+#pragma unroll 4
     for (int i = group; i < pieces; i += groups)
-      acc += exp2_fast(piece(i)[kHeads * kDP + h] - base) * *reinterpret_cast<const v4f*>(piece(i) + h * kDP + 4 * lane);
+      add(piece(i)[kHeads * kDP + h], piece(i)[kHeads * kDP + kHeads + h], *reinterpret_cast<const v4f*>(piece(i) + h * kDP + 4 * lane));
     if (groups > 1) {   // (then every head has its teams at once)
       *reinterpret_cast<v4f*>(&sums[team][4 * lane]) = acc;
+      if (lane == 0) weights[team] = v2f{top, total};
       __syncthreads();
       if (group == 0)
-        for (int i = 1; i < groups; ++i) acc += *reinterpret_cast<const v4f*>(&sums[i * share + mine][4 * lane]);
+        for (int i = 1; i < groups; ++i) add(weights[i * share + mine][0], weights[i * share + mine][1], *reinterpret_cast<const v4f*>(&sums[i * share + mine][4 * lane]));
     }
     if (group == 0) {
       const int64_t row = (int64_t)seq * p.Hq + kv_head * ln.group + from + h;
@@ -454,6 +447,7 @@ Line line_of(int64_t sequences, int64_t Hq, int64_t Hkv, int64_t longest) {
   r.group = (int)(Hq / Hkv);
   r.per_kv = (r.group + kHeads - 1) / kHeads;
   r.head_blocks = (int)Hkv * r.per_kv;
+  r.by_head_blocks = divider((uint32_t)r.head_blocks);
   const int64_t tiles = longest / kTile + 1;   // (longest + 1 keys, see length_of())
   const int64_t all = sequences * r.head_blocks * tiles;
   r.parts = (int)(all < kMostParts ? all : kMostParts);   // at most; what there is of them the lengths decide

@@ -69,22 +69,6 @@ MSLK_AMD_DEVINL Sequence<Q> sequence(const PromptArgs& p, int b) {
   }
   return s;
 }
-MSLK_AMD_DEVINL int wave_sum(int v) {   // over the lanes, in every lane
-  v += __builtin_amdgcn_update_dpp(0, v, 0x128, 0xF, 0xF, false);   // rotated by 8 inside 16 lanes, ...
-  v += __builtin_amdgcn_update_dpp(0, v, 0x124, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x122, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x121, 0xF, 0xF, false);
-  return __builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16) + __builtin_amdgcn_readlane(v, 32) + __builtin_amdgcn_readlane(v, 48);
-}
-MSLK_AMD_DEVINL int wave_scan(int v, int lane) {   // inclusive sum
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // from 1, 2, 4, 8 lanes below, inside 16 lanes
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-  const int a = __builtin_amdgcn_readlane(v, 15), b = a + __builtin_amdgcn_readlane(v, 31), c = b + __builtin_amdgcn_readlane(v, 47);
-  return v + (lane < 16 ? 0 : lane < 32 ? a : lane < 48 ? b : c);
-}
-
 // Block `index` of the packed queries: sequence by sequence, its last queries, which see the most keys, first; or, `sorted` (up to 64
 // sequences), in the order of how many tiles of keys they visit, most first.  Behind them the tokens in front of and behind all
 // sequences, which see nothing.
