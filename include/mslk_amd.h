@@ -309,7 +309,7 @@ int mslk_amd_f8f8bf16_rowwise_batched(const void* xq, const void* wq, const floa
  *
  * Rows of heads: element (token, head, channel) lies at data[token * token_stride + head * head_stride + channel], strides in
  * elements.  Query head h reads KV head h / (Hq / Hkv).  D is a multiple of 8, at most 256; rows begin on 16-byte boundaries
- * (base pointers and strides multiples of 8 elements).  `dtype` is MSLK_AMD_DTYPE_BF16 or _F16; sums, softmax and rotation run
+ * (base pointers and strides multiples of 8 elements; token strides below 2^25).  `dtype` is MSLK_AMD_DTYPE_BF16 or _F16; sums, softmax and rotation run
  * in fp32.
  */
 typedef struct {
@@ -321,7 +321,8 @@ typedef struct {
  * A paged cache.  Key t of sequence b lies in slot t % page_size of page page_table[b * table_stride + t / page_size]; its row of
  * head h begins at k + page * k_stride[0] + slot * k_stride[1] + h * k_stride[2] (elements), that of its value and, where the
  * cache holds e4m3 codes, their fp32 scales alike.  Entries of the page table that no key needs are not used; a key whose entry
- * is not in [0, pages), or lies beyond table_width, makes the attention of its sequence NaN.
+ * is not in [0, pages), or lies beyond table_width, makes the attention of its sequence NaN.  Strides are not negative; those of
+ * keys and values stay below 2^35 elements (eight times 2^32), those of scales below 2^32.
  */
 typedef struct {
   void *k, *v;
@@ -353,6 +354,7 @@ int mslk_amd_append_kv(const mslk_amd_heads* q, const mslk_amd_heads* k, const m
 /*
  * out[b, h] = sum_t softmax_t(scale q[b, h] . k[t]) v[t] over the kv_lens[b] keys of sequence b (q: one token per sequence), and
  * lse[b, h] = log sum_t exp(scale q . k[t]).  No keys: zeros and -inf.  scale > 0.
+ * The tiles of 32 keys of all sequences and KV heads (counting what the page table could hold) have to be fewer than 2^31.
  *   out [sequences, Hq, D], lse [sequences, Hq], contiguous; workspace: mslk_amd_attention_decode_workspace_bytes() of it, 16-byte aligned.
  */
 size_t mslk_amd_attention_decode_workspace_bytes(int64_t sequences, int64_t Hq, int64_t Hkv, int64_t D, int64_t table_width, int64_t page_size);

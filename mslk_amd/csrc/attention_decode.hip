@@ -13,6 +13,12 @@
 // and wave i of W, each a workgroup of its own, takes the i-th of W equal parts of the line.  Where a part begins or ends inside a
 // (sequence, head block), what was summed there is written out in 32 bits, together with where the pieces of the block begin and
 // end, and a second launch joins them in their order.
+//
+// Bound: the memory.  64 heads of 128 on 8: one sequence of 131071 keys (537 MB) 97.3 us, 5.5 TB/s; 32 sequences of up to 8192 keys
+// (515 MB) 95.8 us, 5.4 TB/s; 128 sequences in e4m3 (1269 MB) 241 us, 5.3 TB/s, and 221 us where a pool keeps its scales by head (one
+// row of 4 bytes per key and head lies among those of the other heads, whose waves fetch the same lines).  A copy moves 5.1 TB/s
+// on the same card, a plain read 6.2.  Short caches are bound by what waits for one another: the lengths, the page numbers, the rows,
+// the second launch: 700 keys on 8 KV heads take 5.1 + 4.6 us in the two kernels, 8.6 us a call in a graph.
 #include "attention.h"
 #include "rows.h"
 
@@ -22,6 +28,10 @@ namespace mslk_amd {
 namespace {
 
 constexpr int kTile = 32, kHeads = 16;
+// A line of at most kMostParts tiles is cut into parts of one tile, a longer one into kLongParts parts.  Two waves fit a SIMD (kMostParts of
+// them the GPU), but in a long line one keeps the memory busy and there is half as much to join: 1024 against 2048 parts, us: one
+// sequence of 131071 keys 99 / 105, 128 sequences in e4m3 247 / 257.  Short lines have no tile to load while another is computed:
+// 256 sequences of 4 keys (2048 tiles) 11.5 in parts of one, 14.0 in 1024 parts.
 constexpr int kMostParts = 2048, kLongParts = 1024;
 
 struct Line {          // how the work is divided
@@ -43,7 +53,7 @@ MSLK_AMD_DEVINL int tiles_of(int len) { return max(1, (len + kTile - 1) / kTile)
 // Part `w` of the line: tiles [begin, end), the sequence that holds the first of them and the tiles in front of that sequence.  (A line
 // has fewer than 2^31 tiles; 64-bit divisions would take longer than a tile.)
 struct Part {
-  int begin, end, before, seq, len;
+  int index, begin, end, before, seq, len;
 };
 MSLK_AMD_DEVINL bool find_part(const DecodeArgs& p, const Line& ln, int w, Part& r) {
   const int lane = threadIdx.x;
@@ -56,6 +66,12 @@ MSLK_AMD_DEVINL bool find_part(const DecodeArgs& p, const Line& ln, int w, Part&
   total *= ln.head_blocks;
   const uint32_t parts = total <= kMostParts ? total : kLongParts;   // none of them empty
   if ((uint32_t)w >= parts) return false;
+  // Workgroup i runs on XCD i % 8.  Neighbours in the line go to one XCD where they share lines: the scales of the heads of a key
+  // (128 sequences in e4m3, 64 heads on 8: 246 -> 241 us; 8 sequences, 16 heads of 64: 21.8 -> 20.6), the pieces that one join reads
+  // and the page table (700 keys: 9.2 -> 8.6).  Long lines of 16-bit rows, which share nothing, are better spread: 64 sequences of 1024
+  // keys 53.3, by neighbours 54.6; heads of 256 72.2 / 76.9.
+  if (p.fp8 || parts == total) w = (w % 8) * (parts / 8) + min((uint32_t)w % 8, parts % 8) + w / 8;
+  r.index = w;
   const uint32_t each = parts == total ? 1 : total / parts, more = total - each * parts;   // the first `more` parts hold one tile more
   r.begin = w * each + min((uint32_t)w, more);
   r.end = r.begin + each + ((uint32_t)w < more ? 1 : 0);
@@ -123,7 +139,8 @@ template <> struct RowTraits<kRowsE4m3By8> {
   typedef v2i key_t, value_t;
 };
 // A load of values covers whole rows, whose lines no other load asks for: non-temporal.  A load of keys takes 64 bytes of each of its
-// rows and the next one the rest of the line, which has to be there still.
+// rows and the next one the rest of the line, which has to be there still (in e4m3 247 us with plain loads of keys, 346 with
+// non-temporal ones of half the width).
 template <typename T>
 MSLK_AMD_DEVINL T stream(const char* at) { return __builtin_nontemporal_load(reinterpret_cast<const T*>(at)); }
 
@@ -342,7 +359,7 @@ __global__ __launch_bounds__(64, STEPS <= 4 ? 2 : 1) void decode_kernel(DecodeAr
 
     l = sum_rows16(l);
     const bool whole = n == tiles;
-    const int slot = 2 * (int)blockIdx.x + (at == part.begin ? 0 : 1);
+    const int slot = 2 * part.index + (at == part.begin ? 0 : 1);
     if (ln.joined && lane == 0) {
       int* ends = p.ends + 2 * (seq * (int64_t)ln.head_blocks + hb);
       if (tile0 == 0) ends[0] = slot;
@@ -389,7 +406,9 @@ __global__ __launch_bounds__(64, STEPS <= 4 ? 2 : 1) void decode_kernel(DecodeAr
   }
 }
 
-// Joins the pieces of a head block where there is more than one.  Workgroup (x, y): `per` heads of head block x, from y * per on.  A team
+// Joins the pieces of a head block where there is more than one: 4 to 6 us, most of it the launch and the two loads that wait for one
+// another.  (A workgroup of eight waves per head block, joined in LDS in one launch, took 12.3 us for 700 keys and 55 for 4 sequences
+// of 4096, against 9.2 and 19.6: too few waves load.)  Workgroup (x, y): `per` heads of head block x, from y * per on.  A team
 // of kDP / 4 lanes, four channels each, sums the pieces of a head, or every n-th of them where there are fewer heads than teams.
 typedef float v2f __attribute__((ext_vector_type(2)));
 constexpr int kJoinThreads = 256;
