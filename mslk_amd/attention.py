@@ -7,7 +7,8 @@ They have no counterpart in the reference's FP8 path: they are what a program pu
 
 A cache is two tensors [pages, page_size, kv_heads, channels], in the type of the queries or in float8_e4m3fn with one fp32 scale
 per row (`k_scale`, `v_scale` [pages, page_size, kv_heads]).  Strides are free as long as channels are contiguous, so a
-pool [pages, kv_heads, page_size, channels] is passed as `pool.transpose(1, 2)`.  `page_table` [sequences, width] (int32) names the
+pool [pages, kv_heads, page_size, channels] is passed as `pool.transpose(1, 2)`; scales kept by head like that, [pages, kv_heads,
+page_size], are read with fewer bytes, because a head's lie side by side.  `page_table` [sequences, width] (int32) names the
 pages of each sequence in order, `kv_lens` [sequences] (int32) says how many keys it has; both are read on the GPU only, so a
 captured graph follows them.  Nothing here is differentiable.
 """
