@@ -205,7 +205,7 @@ __global__ __launch_bounds__((64 * Shape<DP, Q>::kWaves), 2) void prompt_kernel(
   using E = Elem<F16>;
   using S = Shape<DP, Q>;
   constexpr int kB = S::kB, kWaveQ = S::kWaveQ, kWaves = S::kWaves;
-  constexpr int kSlots = DP <= 64 ? 8 : DP <= 128 ? 16 : 32;   // 16-byte chunks of a row in LDS, a power of two
+  constexpr int kSlots = DP / 8;   // 16-byte chunks of a row in LDS
   constexpr int kRowBytes = kSlots * 16, kTileBytes = kTileK * kRowBytes;
   constexpr int kSteps = DP / 32, kBlocksD = DP / 16;
   constexpr int kLoads = kTileBytes / 1024 / kWaves;           // wave-level copies of a tile per wave
@@ -231,18 +231,17 @@ __global__ __launch_bounds__((64 * Shape<DP, Q>::kWaves), 2) void prompt_kernel(
   const int kv_head = (int)divide((uint32_t)head, p.group);
   const uint32_t k_pitch = (uint32_t)p.k.token_stride * 2, v_pitch = (uint32_t)p.v.token_stride * 2;
   // Which 16-byte chunk of its row a slot of LDS holds: chosen so that the 16 (8-byte loads: 32) lanes that are served together find
-  // their rows in different banks.
-  auto k_swizzle = [](int r) { return kSlots == 8 ? (r >> 1) & 7 : r & 15; };
-  auto v_swizzle = [](int r) { return kSlots == 8 ? r & 6 : (2 * r) & 14; };
+  // their rows in different banks (64 of 4 bytes: rows of 16 or 32 chunks begin in the same one, of 8 or 24 in two in turn, of 12 in four).
+  auto k_swizzle = [](int r) { return kSlots % 16 == 8 ? (r >> 1) & 7 : kSlots == 12 ? (r >> 2) & 3 : r & 15; };
+  auto v_swizzle = [](int r) { return kSlots % 16 == 8 ? r & 6 : kSlots == 12 ? (r >> 1) & 2 : (2 * r) & 14; };
 
   // Copies of a tile: slot (row r, chunk c) of LDS holds chunk c ^ swizzle(r) of row r.  Rows beyond the last key and chunks beyond D
   // lie outside the buffer and come as zeros.
-  constexpr int kRowsPerCopy = 64 / kSlots;
   uint32_t k_off[kLoads], v_off[kLoads];   // of this lane's pieces from a tile's first row
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
-    const int r = (wave * kLoads + i) * kRowsPerCopy + lane / kSlots;
-    const int k_chunk = (lane % kSlots) ^ k_swizzle(r), v_chunk = (lane % kSlots) ^ v_swizzle(r);
+    const int slot = (wave * kLoads + i) * 64 + lane, r = slot / kSlots;
+    const int k_chunk = (slot % kSlots) ^ k_swizzle(r), v_chunk = (slot % kSlots) ^ v_swizzle(r);
     k_off[i] = k_chunk < chunks ? (uint32_t)r * k_pitch + (uint32_t)k_chunk * 16 : kOutside;
     v_off[i] = v_chunk < chunks ? (uint32_t)r * v_pitch + (uint32_t)v_chunk * 16 : kOutside;
   }
