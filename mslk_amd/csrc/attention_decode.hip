@@ -12,7 +12,7 @@
 // Keys are divided evenly whatever the lengths: every (sequence, head block) has its tiles of 32 keys, all tiles stand in one line,
 // and wave i of W, each a workgroup of its own, takes the i-th of W equal parts of the line.  Where a part begins or ends inside a
 // (sequence, head block), what was summed there is written out in 32 bits, together with where the pieces of the block begin and
-// end, and a second launch joins them in their order.
+// end, and a second launch joins them in their order.  (Short caches are not cut: a wave each for their head blocks.)
 //
 // Bound: the memory.  64 heads of 128 on 8: one sequence of 131071 keys (537 MB) 97.3 us, 5.5 TB/s; 32 sequences of up to 8192 keys
 // (515 MB) 95.8 us, 5.4 TB/s; 128 sequences in e4m3 (1269 MB) 241 us, 5.3 TB/s, and 221 us where a pool keeps its scales by head (one
@@ -33,6 +33,13 @@ constexpr int kTile = 32, kHeads = 16;
 // sequence of 131071 keys 99 / 105, 128 sequences in e4m3 247 / 257.  Short lines have no tile to load while another is computed:
 // 256 sequences of 4 keys (2048 tiles) 11.5 in parts of one, 14.0 in 1024 parts.
 constexpr int kMostParts = 2048, kLongParts = 1024;
+
+// Where the page tables hold few keys, or not many more than there are head blocks, a wave takes a whole head block instead, and there
+// is nothing to join.  In parts against whole, us, 32 heads on 8: 100 keys, 1 sequence 8.3 / 7.2, 64 sequences 13.6 / 8.5; 250 keys, 1
+// sequence 8.3 / 10.1, 16 10.6 / 10.4, 64 18.0 / 13.8; 500 keys, 16 sequences 15.1 / 16.7, 32 17.9 / 17.0, 128 45.0 / 39.8; 1000 keys, 16
+// sequences 18.8 / 28.6, 64 41.4 / 41.5, 128 79.0 / 78.2, and of 1 to 1000 keys 76.0 / 60.2 (a part there holds pieces of several
+// blocks, each with its own start).  Longer ones, 64 of 1 to 4000 keys: 94.7 / 126.8, the longest block long after the others.
+constexpr int kWholeKeys = 128, kMostWholeKeys = 1024;
 
 struct Line {          // how the work is divided
   int head_blocks;     // per sequence: KV heads x blocks of kHeads query heads
@@ -56,6 +63,15 @@ struct Part {
   int index, begin, end, before, seq, len;
 };
 MSLK_AMD_DEVINL bool find_part(const DecodeArgs& p, const Line& ln, int w, Part& r) {
+  if (!ln.joined) {   // a head block each
+    r.seq = (int)divide((uint32_t)w, ln.by_head_blocks);
+    r.len = __builtin_amdgcn_readfirstlane(length_of(p, r.seq));
+    r.index = 0;
+    r.before = 0;
+    r.begin = (w - r.seq * ln.head_blocks) * tiles_of(r.len);
+    r.end = r.begin + tiles_of(r.len);
+    return true;
+  }
   const int lane = threadIdx.x;
   int len = lane < p.sequences ? length_of(p, lane) : 0;
   int n = lane < p.sequences ? tiles_of(len) : 0, upto = wave_scan(n, lane);
@@ -468,9 +484,9 @@ Line line_of(int64_t sequences, int64_t Hq, int64_t Hkv, int64_t longest) {
   r.head_blocks = (int)Hkv * r.per_kv;
   r.by_head_blocks = divider((uint32_t)r.head_blocks);
   const int64_t tiles = longest / kTile + 1;   // (longest + 1 keys, see length_of())
-  const int64_t all = sequences * r.head_blocks * tiles;
-  r.parts = (int)(all < kMostParts ? all : kMostParts);   // at most; what there is of them the lengths decide
-  r.joined = tiles > 1;
+  const int64_t blocks = sequences * r.head_blocks, all = blocks * tiles;
+  r.joined = longest > kWholeKeys && (longest > kMostWholeKeys || blocks < longest / 2);
+  r.parts = (int)(!r.joined ? blocks : all < kMostParts ? all : kMostParts);   // at most; what there is of them the lengths decide
   return r;
 }
 int padded(int64_t D) { return D <= 128 ? 128 : 256; }

@@ -353,6 +353,23 @@ def test_decode_lengths(lens, fp8):
     check_decode(heads(g, len(lens), 4, 64, torch.bfloat16), Cache(g, lens, 2, 64, 16, torch.bfloat16, fp8))
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("d", [64, 128, 200])
+@pytest.mark.parametrize("lens", [[0], [1], [0, 0, 3], [31, 32, 33], [127, 128, 129], [255, 0, 257, 1], [1] * 130, [1000, 1, 700], [65] * 70 + [0] * 70])
+def test_decode_lengths_in_wide_tables(lens, d, fp8):
+    """Tables with room for many more keys: how the work is divided goes by what they could hold."""
+    g = torch.Generator().manual_seed(sum(lens) + d)
+    check_decode(heads(g, len(lens), 6, d, torch.bfloat16), Cache(g, lens, 2, d, 16, torch.bfloat16, fp8, extra=100))
+
+
+@pytest.mark.parametrize("sequences,hkv,longest", [(3, 1, 120), (3, 1, 200), (40, 4, 200), (200, 1, 500), (300, 2, 1000), (140, 8, 1030)])
+def test_decode_batches_of_short_caches(sequences, hkv, longest):
+    g = torch.Generator().manual_seed(longest)
+    lens = torch.randint(0, longest, (sequences,), generator=g).tolist()
+    lens[0] = longest
+    check_decode(heads(g, sequences, 2 * hkv, 64, torch.float16), Cache(g, lens, hkv, 64, 8, torch.float16, extra=0))
+
+
 @pytest.mark.parametrize("hq,hkv", [(1, 1), (3, 1), (15, 1), (16, 1), (17, 1), (40, 1), (5, 5), (64, 8), (34, 2), (48, 16)])
 def test_decode_head_layouts(hq, hkv):
     g = torch.Generator().manual_seed(hq)
