@@ -232,7 +232,8 @@ __global__ __launch_bounds__((64 * Shape<DP, Q>::kWaves), 2) void prompt_kernel(
   const uint32_t k_pitch = (uint32_t)p.k.token_stride * 2, v_pitch = (uint32_t)p.v.token_stride * 2;
   // Which 16-byte chunk of its row a slot of LDS holds: chosen so that the 16 (8-byte loads: 32) lanes that are served together find
   // their rows in different banks (64 of 4 bytes: rows of 16 or 32 chunks begin in the same one, of 8 or 24 in two in turn, of 12 in four).
-  auto k_swizzle = [](int r) { return kSlots % 16 == 8 ? (r >> 1) & 7 : kSlots == 12 ? (r >> 2) & 3 : r & 15; };
+  // Of a 16-byte load these are rows 0 to 3 and 12 to 15 of one `group` and 4 to 11 of its neighbour.
+  auto k_swizzle = [](int r) { return kSlots % 16 == 8 ? (r >> 1) & 7 : kSlots == 12 ? ((r >> 1) & 2) ^ 3 * ((r >> 3) & 1) : r & 15; };
   auto v_swizzle = [](int r) { return kSlots % 16 == 8 ? r & 6 : kSlots == 12 ? (r >> 1) & 2 : (2 * r) & 14; };
 
   // Copies of a tile: slot (row r, chunk c) of LDS holds chunk c ^ swizzle(r) of row r.  Rows beyond the last key and chunks beyond D
