@@ -202,16 +202,17 @@ __global__ __launch_bounds__(64, STEPS <= 4 ? 2 : 1) void decode_kernel(DecodeAr
     const float* vs_base = p.cache.v_scale + kv_head * p.cache.v_scale_stride[2];
 
     // Pages of the keys whose rows or scales a lane fetches: keys i and 16 + i, and key (i % 8, g).  Keys beyond the end repeat the
-    // last one.
+    // last one; a sequence without keys, whose first look-up stands in front of the test for that, asks for the place of key 0.
+    const int last_key = max(key_end - 1, 0);
     struct Place { int page[3], slot[3]; };
     auto places = [&](int key0) {
       Place r;
 #pragma unroll
       for (int x = 0; x < 3; ++x) {
-        const int key = min(key0 + (x == 0 ? i : x == 1 ? 16 + i : key_of(i & 7, g)), key_end - 1);
+        const int key = min(key0 + (x == 0 ? i : x == 1 ? 16 + i : key_of(i & 7, g)), last_key);
         const int index = (int)divide((uint32_t)key, p.cache.page_size);
         r.slot[x] = key - index * (int)p.cache.page_size.d;
-        r.page[x] = index < p.cache.table_width ? table[index] : -1;
+        r.page[x] = (uint32_t)index < (uint32_t)p.cache.table_width ? table[index] : -1;
       }
       return r;
     };

@@ -385,6 +385,23 @@ def test_decode_page_sizes(page):
     check_decode(heads(g, 4, 4, 64, torch.float16), Cache(g, lens, 2, 64, page, torch.float16, fp8=True))
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("extra", [2, 5000])
+@pytest.mark.parametrize("lens", [[0], [0, 40, 0, 33, 0], [0] * 3, [7, 0]])
+def test_decode_empty_sequences_with_pages_of_one_key(lens, extra, fp8):
+    """A sequence without keys reads nothing of its table, whose entry of a key -1 would lie in front of it: the first table row,
+    rows in between and one for all sequences, few keys of room (a head block per wave) and much of it (equal parts)."""
+    g = torch.Generator().manual_seed(sum(lens))
+    cache = Cache(g, lens, 2, 64, 1, torch.bfloat16, fp8, extra=extra)
+    q = heads(g, len(lens), 4, 64, torch.bfloat16)
+    check_decode(q, cache)
+    if not any(lens):
+        k, v, table, kv_lens, ks, vs = cache.on_gpu()
+        for t in (table[:1].expand(len(lens), -1), torch.zeros(len(lens), 0, dtype=torch.int32, device=DEV)):
+            out, lse = mslk_amd.attention_decode(q.to(DEV), k, v, t, kv_lens, ks, vs, return_lse=True)
+            assert (out == 0).all() and (lse == -math.inf).all()
+
+
 def test_decode_scores_far_apart_and_scales_far_apart():
     g = torch.Generator().manual_seed(11)
     lens = [700, 90]
