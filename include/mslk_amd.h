@@ -353,7 +353,7 @@ int mslk_amd_append_kv(const mslk_amd_heads* q, const mslk_amd_heads* k, const m
 
 /*
  * out[b, h] = sum_t softmax_t(scale q[b, h] . k[t]) v[t] over the kv_lens[b] keys of sequence b (q: one token per sequence), and
- * lse[b, h] = log sum_t exp(scale q . k[t]).  No keys: zeros and -inf.  scale > 0.
+ * lse[b, h] = log sum_t exp(scale q . k[t]).  No keys: zeros and -inf.  0 < scale <= 2e38.
  * The tiles of 32 keys of all sequences and KV heads (counting what the page table could hold) have to be fewer than 2^31.
  *   out [sequences, Hq, D], lse [sequences, Hq], contiguous; workspace: mslk_amd_attention_decode_workspace_bytes() of it, 16-byte aligned.
  */

@@ -76,7 +76,7 @@ def attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tens
     """Attention of q [sequences, Hq, D], one token per sequence, over the first `kv_lens` keys of each sequence's pages.
 
     Returns out [sequences, Hq, D] and, with `return_lse`, log sum exp of the scaled scores [sequences, Hq] (fp32).  `scale` is
-    1 / sqrt(D) unless given.  A sequence without keys gives zeros and -inf; one whose keys lack a page gives NaN."""
+    1 / sqrt(D) unless given (positive, at most 2e38).  A sequence without keys gives zeros and -inf; one whose keys lack a page gives NaN."""
     _check_gpu("attention_decode", q)
     out, lse = torch.ops.mslk.attention_decode(q, k_cache, v_cache, page_table, kv_lens, k_scale, v_scale, scale)
     return (out, lse) if return_lse else out

@@ -256,7 +256,7 @@ __global__ __launch_bounds__((64 * Shape<DP, Q>::kWaves), 2) void prompt_kernel(
   const int wave_seen = wave_row >= w.rows ? 0 : max(min(w.keys, wave_first + kWaveQ), 0);
   const int wave_tiles = (wave_seen + kTileK - 1) / kTileK;
   const int whole = min(min(w.keys, w.q0 + w.shift + 1) / kTileK, tiles);  // tiles that every query of the block sees whole
-  const float c = p.scale * kLog2e, slack = 8.f / c;
+  const float c = p.scale * kLog2e;
 
   Rows k_rows(p.k, w.k_row, kv_head, p.D, min(w.keys, tiles * kTileK)), v_rows(p.v, w.k_row, kv_head, p.D, min(w.keys, tiles * kTileK));
   int token = 0;
@@ -355,7 +355,7 @@ __global__ __launch_bounds__((64 * Shape<DP, Q>::kWaves), 2) void prompt_kernel(
       for (int r = 1; r < 16; ++r) top = fmaxf(top, s[b][r / 4][r % 4]);
       top = max_rows16(top);
       // the reference follows the maximum when it is left behind by more than 8 powers of two: the weights stay below 2^8
-      const float m_new = top > m[b] + slack ? top : m[b];
+      const float m_new = (top - m[b]) * c > 8.f ? top : m[b];   // (infinite as long as there is no reference, whatever c is)
       const float base = m_new == -__builtin_inff() ? 0.f : m_new * c;
       shrink[b] = exp2_fast(__builtin_fmaf(m[b], c, -base));
       m[b] = m_new;

@@ -120,7 +120,9 @@ int check_cache(const char* op, const mslk_amd_paged_cache* c, int dtype, int64_
   out.lens = c->kv_lens;
   return 0;
 }
-bool good_scale(float scale) { return scale > 0.f && scale <= 3.0e38f; }
+int check_scale(const char* op, float scale) {   // (the kernels multiply by scale log2(e), which has to be finite too)
+  return scale > 0.f && scale <= 2e38f ? 0 : fail("%s: scale must be positive and at most 2e38", op);
+}
 
 }  // namespace
 
@@ -550,7 +552,7 @@ int mslk_amd_attention_decode(const mslk_amd_heads* q, int dtype, int64_t sequen
   DecodeArgs p{};
   if (int rc = check_heads(op, dtype, sequences, Hq, Hkv, D)) return rc;
   if (int rc = check_cache(op, cache, dtype, sequences, p.cache)) return rc;
-  if (!good_scale(scale)) return fail("%s: scale must be positive and finite", op);
+  if (int rc = check_scale(op, scale)) return rc;
   if (sequences == 0) return 0;
   if (int rc = check_rows(op, "q", q, p.q)) return rc;
   if (!out || !lse || !aligned(out, 16)) return fail("%s: out and lse must not be null and out be 16-byte aligned", op);
@@ -582,7 +584,7 @@ int mslk_amd_attention_prompt(const mslk_amd_heads* q, const mslk_amd_heads* k, 
   if (keys < 0 || keys >= kMaxTokens) return fail("%s: token counts must be in [0, 2^30) (got %lld)", op, (long long)keys);
   if (sequences < 0 || sequences >= kMaxTokens) return fail("%s: sequences out of range (got %lld)", op, (long long)sequences);
   if (cu_seqlens_k == nullptr && keys != tokens) return fail("%s: without cu_seqlens_k there are as many keys as queries (%lld, %lld)", op, (long long)keys, (long long)tokens);
-  if (!good_scale(scale)) return fail("%s: scale must be positive and finite", op);
+  if (int rc = check_scale(op, scale)) return rc;
   if (tokens == 0) return 0;
   if (!cu_seqlens) return fail("%s: null pointer (cu_seqlens)", op);
   if (int rc = check_rows(op, "q", q, p.q)) return rc;

@@ -600,7 +600,7 @@ int64_t sequences_of(const char* op, const char* name, const Tensor& cu) {
 }
 float scale_of(const char* op, std::optional<double> scale, int64_t D) {
   const double s = scale.value_or(1.0 / std::sqrt((double)D));
-  TORCH_CHECK((float)s > 0.f && std::isfinite((float)s), op, ": scale must be positive and finite, got ", s);
+  TORCH_CHECK((float)s > 0.f && (float)s <= 2e38f, op, ": scale must be positive and at most 2e38, got ", s);
   return (float)s;
 }
 

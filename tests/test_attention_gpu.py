@@ -178,6 +178,39 @@ def test_prompt_scores_far_apart():
     check_prompt(q, k, v, [500], scale=1e-4, causal=False)
 
 
+@pytest.mark.parametrize("scale", [1e-44, 1e-38, 1.5e-38, 1e-30, 1e30, 2e38])
+def test_scales_at_the_ends_of_their_range(scale):
+    """Tiny: every key weighs the same, in however many tiles.  Huge: scores of 0 and of minus the scale, so that the first
+    kind alone counts; lse = log of their number."""
+    g = torch.Generator().manual_seed(10)
+    n, d = 330, 64
+    q, k, v = torch.zeros(n, 2, d).bfloat16(), torch.zeros(n, 2, d).bfloat16(), heads(g, n, 2, d, torch.bfloat16)
+    q[:, :, 0] = 1
+    counts = torch.arange(n) % 3 == 0
+    k[~counts, :, 0] = -1
+    weighs = counts if scale > 1 else torch.ones(n, dtype=torch.bool)
+    out, lse, bound, lse_bound = attention(q, torch.zeros_like(k), v, 1.0, causal_mask(n, n) & weighs)
+    got = mslk_amd.attention_prompt(*(x.to(DEV) for x in (q, k, v)), offsets([n]).to(DEV), scale=scale, return_lse=True)
+    near(got[0], out, bound)
+    near(got[1], lse, lse_bound)
+    for length in (n, 5):
+        cache = Cache(g, [length], 2, d, 16, torch.bfloat16, extra=100, rows=[[k[:length]], [v[:length]]])
+        got = mslk_amd.attention_decode(q[:1].to(DEV), *cache.on_gpu(), scale=scale, return_lse=True)
+        near(got[0], out[length - 1:length], bound[length - 1:length])
+        near(got[1], lse[length - 1:length], lse_bound[length - 1:length])
+
+
+def test_scales_beyond_their_range_are_refused():
+    q = torch.zeros(4, 2, 64, dtype=torch.bfloat16, device=DEV)
+    pool, table, lens = torch.zeros(1, 16, 2, 64, dtype=torch.bfloat16, device=DEV), torch.zeros(4, 1, dtype=torch.int32, device=DEV), torch.ones(
+        4, dtype=torch.int32, device=DEV)
+    for scale in (2.5e38, 3e38, 1e39, 1e-46):   # scale log2(e) infinite, the scale itself, the scale zero
+        with pytest.raises(RuntimeError, match="positive"):
+            mslk_amd.attention_prompt(q, q, q, offsets([4]).to(DEV), scale=scale)
+        with pytest.raises(RuntimeError, match="positive"):
+            mslk_amd.attention_decode(q, pool, pool, table, lens, scale=scale)
+
+
 @pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("d", [64, 72, 80, 200])
 def test_prompt_infinite_keys_and_values(d, causal):
