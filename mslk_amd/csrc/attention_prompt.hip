@@ -1,8 +1,9 @@
 // Attention of packed prompts:  O = softmax(scale Q K^T + mask) V  per sequence and head, heads of queries sharing keys.
 //
-// One pass over the keys per block of queries with a reference m near the running maximum and the running sum l of a softmax: for a
-// tile of keys s = q k, l' = l 2^(c(m - m')) + sum 2^(c(s - m')), O' = O 2^(c(m - m')) + 2^(c(s - m')) V with c = scale log2(e), and
-// O / l at the end.
+// One pass over the keys per block of queries with a reference m near the running maximum and the running sum l of a softmax in base
+// 2: for a tile of keys s = q k, l' = l 2^(m - m') + sum 2^(c s - m'), O' = O 2^(m - m') + 2^(c s - m') V with c = scale log2(e), and
+// O / l at the end.  m is the rounded product of c and a score, and everything is taken from that one number: where it stays, the
+// sums are scaled by exactly 1, however large the scores are.
 //
 // A workgroup takes 128 or 64 queries of one head, a wave 32 or 16 of them; tiles of 64 keys and values are copied into LDS, two of
 // each.  Both products are v_mfma_f32_16x16x32 with the keys first: S^T = K Q^T leaves a lane one query and a quarter of the tile's
@@ -354,10 +355,11 @@ __global__ __launch_bounds__((64 * Shape<DP, Q>::kWaves), 2) void prompt_kernel(
 #pragma unroll
       for (int r = 1; r < 16; ++r) top = fmaxf(top, s[b][r / 4][r % 4]);
       top = max_rows16(top);
+      top *= c;
       // the reference follows the maximum when it is left behind by more than 8 powers of two: the weights stay below 2^8
-      const float m_new = (top - m[b]) * c > 8.f ? top : m[b];   // (infinite as long as there is no reference, whatever c is)
-      const float base = m_new == -__builtin_inff() ? 0.f : m_new * c;
-      shrink[b] = exp2_fast(__builtin_fmaf(m[b], c, -base));
+      const float m_new = top > m[b] + 8.f ? top : m[b];
+      const float base = m_new == -__builtin_inff() ? 0.f : m_new;
+      shrink[b] = exp2_fast(m[b] - base);
       m[b] = m_new;
       float sum = 0.f;
 #pragma unroll
@@ -500,7 +502,7 @@ __global__ __launch_bounds__((64 * Shape<DP, Q>::kWaves), 2) void prompt_kernel(
       const int ch = 16 * (d + (group & 1)) + 8 * (group / 2);
       if (row < w.rows && ch < p.D) *reinterpret_cast<v4i*>(dst + ch) = x;
     }
-    if (group == 0 && row < w.rows) p.lse[(w.q_row + row) * p.Hq + head] = total == 0.f ? -__builtin_inff() : m[b] * p.scale + log2_fast(total) * kLn2;
+    if (group == 0 && row < w.rows) p.lse[(w.q_row + row) * p.Hq + head] = total == 0.f ? -__builtin_inff() : (m[b] + log2_fast(total)) * kLn2;
   }
 }
 

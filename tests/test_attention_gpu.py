@@ -309,6 +309,27 @@ def test_prompt_scores_that_creep_up(d, step):
     check_prompt(q, k, v, [n], scale=1.0)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("tokens,hq", [(16, 4), (300, 104)])
+def test_prompt_equal_scores_weigh_the_same_in_every_tile(tokens, hq, d, dtype):
+    """Scores that are all the same, however large: the reference stays, so the sums of the first tile may not fade until the last.
+    Values of 1 in the first half of the keys and -1 in the second add up to zero, exactly: a weight of 11 bits times up to 2^13 keys
+    fits 24.  lse: the rounding of scale log2(e) and of two products, 2^-21 of it, and 256 sums of a row in 32 bits, 2^-14."""
+    n = 16384
+    scores = torch.tensor([50.0, 700.0, -300.0, 37.0])
+    q, k, v = torch.zeros(tokens, hq, d, dtype=dtype), torch.zeros(n, 4, d, dtype=dtype), torch.ones(n, 4, d, dtype=dtype)
+    q[:, :, 0] = 1
+    k[:, :, 0] = scores.to(dtype)
+    v[n // 2:] = -1
+    cu, cu_k = offsets([tokens]).to(DEV), offsets([n]).to(DEV)
+    for scale in (1.0, 0.7):
+        out, lse = mslk_amd.attention_prompt(*(x.to(DEV) for x in (q, k, v)), cu, cu_k, causal=False, scale=scale, return_lse=True)
+        assert out.float().abs().max() <= 2.0 ** -20
+        want = (scores.double() * torch.tensor(scale).double() + math.log(n)).repeat_interleave(hq // 4).expand(tokens, -1)
+        near(lse, want, 2.0 ** -21 * want.abs() + 2.0 ** -14)
+
+
 def test_prompt_many_sequences_and_repeat():
     g = torch.Generator().manual_seed(9)
     lens = torch.randint(0, 9, (300,), generator=g).tolist()
