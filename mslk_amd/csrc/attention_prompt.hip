@@ -348,7 +348,7 @@ __global__ __launch_bounds__((64 * Shape<DP, Q>::kWaves), 2) void prompt_kernel(
   };
   auto same = [](int x) { return x; };
   auto softmax = [&] {
-    float shrink[kB];
+    float shrink[kB], base[kB], largest = 0.f;
 #pragma unroll
     for (int b = 0; b < kB; ++b) {
       float top = s[b][0][0];
@@ -358,15 +358,34 @@ __global__ __launch_bounds__((64 * Shape<DP, Q>::kWaves), 2) void prompt_kernel(
       top *= c;
       // the reference follows the maximum when it is left behind by more than 8 powers of two: the weights stay below 2^8
       const float m_new = top > m[b] + 8.f ? top : m[b];
-      const float base = m_new == -__builtin_inff() ? 0.f : m_new;
-      shrink[b] = exp2_fast(m[b] - base);
+      base[b] = m_new == -__builtin_inff() ? 0.f : m_new;
+      shrink[b] = exp2_fast(m[b] - base[b]);
       m[b] = m_new;
+      largest = fmaxf(largest, __builtin_fabsf(base[b]));
+    }
+    float by = c;
+    if (__ballot(largest > 0x1p24f) != 0) {
+      // The product in a weight's fused multiply-add is not rounded, that in the reference is: here by more than a power of two, and
+      // at the same score too, which may leave the range of 16 bits.  Both rounded instead.
+      by = 1.f;
+#pragma unroll
+      for (int b = 0; b < kB; ++b) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float x = s[b][r / 4][r % 4] * c;
+          s[b][r / 4][r % 4] = x - base[b];
+        }
+        base[b] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < kB; ++b) {
       float sum = 0.f;
 #pragma unroll
       for (int g = 0; g < 4; ++g)
 #pragma unroll
         for (int r = 0; r < 4; r += 2) {
-          const float x = exp2_fast(__builtin_fmaf(s[b][g][r], c, -base)), y = exp2_fast(__builtin_fmaf(s[b][g][r + 1], c, -base));
+          const float x = exp2_fast(__builtin_fmaf(s[b][g][r], by, -base[b])), y = exp2_fast(__builtin_fmaf(s[b][g][r + 1], by, -base[b]));
           sum += x + y;
           pk[b][g / 2][2 * (g % 2) + r / 2] = (int)E::pack(x, y);   // the weights' one rounding; l sums them unrounded
         }

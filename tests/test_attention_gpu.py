@@ -311,6 +311,34 @@ def test_prompt_scores_that_creep_up(d, step):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("hq", [4, 104])
+def test_scores_whose_rounding_is_many_powers_of_two(hq, d, dtype):
+    """Scores of 10^6 to 10^37: one key in each half of the sequence scores twice what the others do, so the output is its value
+    (up to the weight's one rounding) and lse its score, with the rounding of scale log2(e) and of two products."""
+    g = torch.Generator().manual_seed(34)
+    n = 300
+    q, k, v = torch.zeros(n, hq, d, dtype=dtype), torch.zeros(n, 4, d, dtype=dtype), heads(g, n, 4, d, dtype)
+    q[:, :, 0] = 1031
+    for scale in [float(x) for x in 10 ** (1 + 4 * torch.rand(6, generator=g))] + ([1e13, 1e30] if dtype == torch.bfloat16 else []):
+        for sign in (1, -1):
+            k[:, :, 0] = sign * (1000 + 8 * torch.rand(n, 1, generator=g)) * (1 if sign > 0 else 3)
+            k[40, :, 0] = sign * 2003
+            k[211, :, 0] = sign * (4007 if sign > 0 else 1001)
+            winner = torch.where(torch.arange(n) >= 211, 211, 40)
+            out, lse = mslk_amd.attention_prompt(*(x.to(DEV) for x in (q, k, v)), offsets([n]).to(DEV), scale=scale, return_lse=True)
+            score = (q.double()[:, :, :1] * k.double()[winner][:, :, :1].repeat_interleave(hq // 4, 1))[..., 0] * scale
+            value = v.double()[winner].repeat_interleave(hq // 4, 1)
+            seen = slice(40, n)
+            near(out[seen], value[seen], (2 * ROUND[dtype] * value.abs())[seen], f"{scale}")
+            near(lse[seen], score[seen], 2.0 ** -21 * score[seen].abs(), f"lse, {scale}")
+            cache = Cache(g, [n], 4, d, 16, dtype, rows=[[k], [v]])
+            got = mslk_amd.attention_decode(q[:1].to(DEV), *cache.on_gpu(), scale=scale, return_lse=True)
+            near(got[0], value[n - 1:], 2 * ROUND[dtype] * value[n - 1:].abs())
+            near(got[1], score[n - 1:], 2.0 ** -21 * score[n - 1:].abs())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128, 256])
 @pytest.mark.parametrize("tokens,hq", [(16, 4), (300, 104)])
 def test_prompt_equal_scores_weigh_the_same_in_every_tile(tokens, hq, d, dtype):
     """Scores that are all the same, however large: the reference stays, so the sums of the first tile may not fade until the last.
