@@ -366,7 +366,7 @@ int mslk_amd_attention_decode(const mslk_amd_heads* q, int dtype, int64_t sequen
  * The same for whole prompts packed one after the other: queries cu_seqlens[b] ... cu_seqlens[b + 1] - 1 of `tokens` over keys
  * cu_seqlens_k[b] ... of `keys` (NULL: cu_seqlens).  causal != 0: the last query of a sequence sees its last key, the one before
  * it all but that, and so on; queries in front of the first key, and tokens of no sequence, see nothing.
- *   out [tokens, Hq, D], lse [tokens, Hq], contiguous.  tokens, keys < 2^30.
+ *   out [tokens, Hq, D], lse [tokens, Hq], contiguous.  tokens, keys < 2^30.  Token strides of k and v (of more than one key) are at least D.
  */
 int mslk_amd_attention_prompt(const mslk_amd_heads* q, const mslk_amd_heads* k, const mslk_amd_heads* v, int dtype, int64_t tokens,
                               int64_t keys, int64_t Hq, int64_t Hkv, int64_t D, const int32_t* cu_seqlens,

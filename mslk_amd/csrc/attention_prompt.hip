@@ -171,7 +171,8 @@ MSLK_AMD_DEVINL bool any_wild(const char* rows, Swizzle swizzle) {
   return __ballot(max(top[0], top[1]) >= (F16 ? 0x7C00 : 0x7F80)) != 0;
 }
 
-// Rows of a head's keys or values from a tile's first one on, as a buffer: what lies beyond the last row is read as zeros.
+// Rows of a head's keys or values from a tile's first one on, as a buffer: what lies beyond the last row is read as zeros (a row's pitch
+// is at least its length).
 struct Rows {
   uint64_t base;
   uint32_t pitch, row_bytes;

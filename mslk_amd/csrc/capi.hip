@@ -591,6 +591,9 @@ int mslk_amd_attention_prompt(const mslk_amd_heads* q, const mslk_amd_heads* k, 
   if (keys > 0) {
     if (int rc = check_rows(op, "k", k, p.k)) return rc;
     if (int rc = check_rows(op, "v", v, p.v)) return rc;
+    // (the kernel tells rows behind the last key by their offset; the stride of a single key has no meaning)
+    if (keys == 1) p.k.token_stride = p.v.token_stride = D;
+    if (p.k.token_stride < D || p.v.token_stride < D) return fail("%s: rows of k and v must not overlap (token strides of at least the head dimension)", op);
   }
   if (!out || !lse || !aligned(out, 16)) return fail("%s: out and lse must not be null and out be 16-byte aligned", op);
   p.out = (uint16_t*)out;

@@ -562,15 +562,16 @@ Tensor grouped_mm_op(const Tensor& XQ, const Tensor& WQ, const Tensor& x_scale, 
 // ---------------------------------------------------------------------------------------------------------------------
 // attention
 // ---------------------------------------------------------------------------------------------------------------------
-// [tokens, heads, channels] with rows that the kernels can read as they are (itself if it is that, a copy otherwise).
+// [tokens, heads, channels] with rows that the kernels can read as they are (itself if it is that, a copy otherwise); `apart`: rows of
+// one head may not overlap.
 struct HeadsArg {
   c10::MaybeOwned<Tensor> keep;
   mslk_amd_heads view{};
 };
-HeadsArg heads_of(const Tensor& t) {
+HeadsArg heads_of(const Tensor& t, bool apart = false) {
   HeadsArg h;
   // (the stride of a dimension of size 0 or 1 has no meaning)
-  const bool fits = aligned16(t) && (t.size(2) <= 1 || t.stride(2) == 1) && (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) < (1 << 25))) &&
+  const bool fits = aligned16(t) && (t.size(2) <= 1 || t.stride(2) == 1) && (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) < (1 << 25) && (!apart || t.stride(0) >= t.size(2)))) &&
                     (t.size(1) <= 1 || t.stride(1) % 8 == 0);
   h.keep = fits ? c10::MaybeOwned<Tensor>::borrowed(t) : c10::MaybeOwned<Tensor>::owned(t.clone(at::MemoryFormat::Contiguous));
   const Tensor& u = *h.keep;
@@ -731,7 +732,7 @@ std::tuple<Tensor, Tensor> attention_prompt(const Tensor& q, const Tensor& k, co
   Tensor out = empty_on(q.sizes(), q.scalar_type(), q), lse = empty_on({T, Hq}, at::kFloat, q);
   if (T == 0) return {out, lse};
   const c10::DeviceGuard guard(q.device());
-  const HeadsArg hq = heads_of(q), hk = heads_of(k), hv = heads_of(v);
+  const HeadsArg hq = heads_of(q), hk = heads_of(k, true), hv = heads_of(v, true);
   check_rc(api.mslk_amd_attention_prompt(&hq.view, &hk.view, &hv.view, float_code(q.scalar_type()), T, S, Hq, Hkv, D, cu, cu_k, sequences, causal, s,
                                          out.mutable_data_ptr(), lse.mutable_data_ptr<float>(), stream_of(q)));
   return {out, lse};

@@ -249,6 +249,46 @@ def test_prompt_strides_and_alignment():
     assert torch.equal(one, mslk_amd.attention_prompt(q, k[:, :1], v[:, :1], cu))
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("d", [64, 72, 128, 200])
+@pytest.mark.parametrize("t", [1, 40, 70])
+def test_prompt_keys_and_values_that_share_memory(t, d, causal):
+    """One key for more queries than a wave holds; a key and a value repeated for all tokens; rows that overlap.  An infinite value
+    makes its channel infinite where it is seen, not NaN."""
+    g = torch.Generator().manual_seed(t + d)
+    n = 200
+    q, row = heads(g, n, 4, d, torch.bfloat16), heads(g, 1, 2, d, torch.bfloat16)
+    row[0, 1, 3] = math.inf
+    flat = torch.randn(2, 8 * t + d, generator=g).bfloat16()
+    flat[1, 8 * (t - 1) + 9] = math.inf
+    sliding = [flat.to(DEV).as_strided((t, 2, d), (8, 8 * t + d, 1)), flat.as_strided((t, 2, d), (8, 8 * t + d, 1))]
+    for on_gpu, rows in ((row.to(DEV).expand(t, -1, -1), row.expand(t, -1, -1)), sliding):
+        seen = (causal_mask(n, t) if causal else torch.ones(n, t, dtype=torch.bool))
+        # scores of finite keys; values: the finite ones, and infinite where such a value is seen
+        key = torch.where(rows.isinf(), 0, rows)
+        out, lse, bound, lse_bound = attention(q, key, key, d ** -0.5, seen)
+        wild = torch.einsum("nt,thd->nhd", seen.float(), rows.isinf().float()).repeat_interleave(2, 1) > 0
+        out[wild] = math.inf
+        got = mslk_amd.attention_prompt(q.to(DEV), key.to(DEV) if rows is sliding[1] else torch.where(row.isinf(), 0, row).to(DEV).expand(t, -1, -1),
+                                        on_gpu, offsets([n]).to(DEV), offsets([t]).to(DEV), causal=causal, return_lse=True)
+        near(got[0], out, bound)
+        near(got[1], lse, lse_bound)
+
+
+def test_prompt_refuses_overlapping_rows_through_the_c_interface():
+    import ctypes
+    from mslk_amd import _lib
+    x, out = torch.zeros(4, 2, 64, dtype=torch.bfloat16, device=DEV), torch.zeros(4, 2, 64, dtype=torch.bfloat16, device=DEV)
+    lse, cu = torch.zeros(4, 2, device=DEV), offsets([4]).to(DEV)
+    rows = lambda stride: ctypes.byref(_lib.Heads(x.data_ptr(), stride, 64))   # noqa: E731
+    def call(k_stride, v_stride):
+        return _lib.lib().mslk_amd_attention_prompt(rows(128), rows(k_stride), rows(v_stride), 0, 4, 4, 2, 2, 64, cu.data_ptr(), None, 1, 1, 1.0,
+                                                    out.data_ptr(), lse.data_ptr(), torch.cuda.current_stream().cuda_stream)
+    assert call(0, 128) != 0 and call(128, 56) != 0
+    assert call(128, 128) == 0 and call(64, 64) == 0
+    torch.cuda.synchronize()
+
+
 def test_prompt_long():
     """16 thousand keys: against the definition on the GPU in 64 bits, a few of the rows."""
     g = torch.Generator().manual_seed(8)
