@@ -354,7 +354,8 @@ int mslk_amd_append_kv(const mslk_amd_heads* q, const mslk_amd_heads* k, const m
 /*
  * out[b, h] = sum_t softmax_t(scale q[b, h] . k[t]) v[t] over the kv_lens[b] keys of sequence b (q: one token per sequence), and
  * lse[b, h] = log sum_t exp(scale q . k[t]).  No keys: zeros and -inf.  0 < scale <= 2e38.
- * The tiles of 32 keys of all sequences and KV heads (counting what the page table could hold) have to be fewer than 2^31.
+ * The page table has room for at most 2^30 keys per sequence (table_width * page_size), and the tiles of 32 keys of all sequences and
+ * KV heads, counting what it could hold, have to be fewer than 2^31.
  *   out [sequences, Hq, D], lse [sequences, Hq], contiguous; workspace: mslk_amd_attention_decode_workspace_bytes() of it, 16-byte aligned.
  */
 size_t mslk_amd_attention_decode_workspace_bytes(int64_t sequences, int64_t Hq, int64_t Hkv, int64_t D, int64_t table_width, int64_t page_size);

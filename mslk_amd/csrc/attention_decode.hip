@@ -50,10 +50,9 @@ struct Line {          // how the work is divided
   int joined;          // whether a head block may be cut
 };
 
-// A length that the page table cannot hold counts as one key more than it holds: that key has no page.
+// A length that the page table cannot hold counts as one key more than it holds: that key has no page.  (Room for at most 2^30 keys.)
 MSLK_AMD_DEVINL int length_of(const DecodeArgs& p, int b) {
-  const int64_t most = (int64_t)p.cache.table_width * p.cache.page_size.d + 1;
-  return (int)min((int64_t)max(p.cache.lens[b], 0), min(most, (int64_t)1 << 30));
+  return min(max(p.cache.lens[b], 0), p.cache.table_width * (int)p.cache.page_size.d + 1);
 }
 MSLK_AMD_DEVINL int tiles_of(int len) { return max(1, (len + kTile - 1) / kTile); }
 
@@ -524,21 +523,16 @@ hipError_t pick_rows(const DecodeArgs& p, const Line& ln, hipStream_t s) {
 
 size_t partial_bytes(const Line& ln, int64_t D) { return (size_t)2 * ln.parts * kHeads * (padded(D) + 2) * sizeof(float); }
 
-int64_t longest_of(int64_t table_width, int64_t page_size) {
-  const int64_t n = table_width * page_size;
-  return n < (int64_t(1) << 30) ? n : int64_t(1) << 30;
-}
-
 }  // namespace
 
 size_t decode_workspace_bytes(int64_t sequences, int64_t Hq, int64_t Hkv, int64_t D, int64_t longest) {
-  const Line ln = line_of(sequences, Hq, Hkv, longest_of(longest, 1));
+  const Line ln = line_of(sequences, Hq, Hkv, longest);
   return ln.joined ? partial_bytes(ln, D) + (size_t)2 * sequences * ln.head_blocks * sizeof(int) : 0;
 }
 
 hipError_t launch_attention_decode(const DecodeArgs& args, hipStream_t s) {
   DecodeArgs p = args;
-  const Line ln = line_of(p.sequences, p.Hq, p.Hkv, longest_of(p.cache.table_width, p.cache.page_size.d));
+  const Line ln = line_of(p.sequences, p.Hq, p.Hkv, (int64_t)p.cache.table_width * p.cache.page_size.d);
   p.ends = (int*)((char*)p.partial + partial_bytes(ln, p.D));
   return p.dtype == 1 ? pick_rows<true>(p, ln, s) : pick_rows<false>(p, ln, s);
 }

@@ -540,7 +540,7 @@ int mslk_amd_append_kv(const mslk_amd_heads* q, const mslk_amd_heads* k, const m
 
 size_t mslk_amd_attention_decode_workspace_bytes(int64_t sequences, int64_t Hq, int64_t Hkv, int64_t D, int64_t table_width, int64_t page_size) {
   if (sequences <= 0 || sequences > 65535 || Hq <= 0 || Hkv <= 0 || Hq > 65535 || Hq % Hkv != 0 || D <= 0 || D > kMaxHeadDim || table_width < 0 ||
-      table_width >= kMaxTokens || page_size <= 0 || page_size >= kMaxTokens)
+      table_width >= kMaxTokens || page_size <= 0 || page_size >= kMaxTokens || table_width * page_size > kMaxTokens)
     return 0;
   return decode_workspace_bytes(sequences, Hq, Hkv, D, table_width * page_size);
 }
@@ -556,6 +556,9 @@ int mslk_amd_attention_decode(const mslk_amd_heads* q, int dtype, int64_t sequen
   if (sequences == 0) return 0;
   if (int rc = check_rows(op, "q", q, p.q)) return rc;
   if (!out || !lse || !aligned(out, 16)) return fail("%s: out and lse must not be null and out be 16-byte aligned", op);
+  if (cache->table_width * cache->page_size > kMaxTokens)   // (a key's number and a sequence's tiles are counted in 32 bits)
+    return fail("%s: the page table must have room for at most 2^30 keys per sequence (%lld pages of %lld)", op, (long long)cache->table_width,
+                (long long)cache->page_size);
   const int64_t blocks = sequences * Hkv * ((Hq / Hkv + 15) / 16);
   if (blocks * (cache->table_width * cache->page_size / 32 + 1) >= (int64_t(1) << 31))
     return fail("%s: the page tables have room for too many keys (at most 2^31 tiles of 32, over sequences and KV heads)", op);

@@ -612,6 +612,19 @@ def test_decode_infinite_keys_and_values(d):
         near(got[1][b:b + 1], lse, lse_bound)
 
 
+def test_decode_with_room_for_2_to_the_30_keys():
+    """The most that a page table may have room for; a length beyond it gives NaN as any that the table cannot hold."""
+    g = torch.Generator().manual_seed(17)
+    cache = Cache(g, [700, 90], 1, 64, 1024, torch.bfloat16)
+    q = heads(g, 2, 2, 64, torch.bfloat16)
+    k, v, table, lens, _, _ = cache.on_gpu()
+    wide = torch.full((2, 1 << 20), -1, dtype=torch.int32, device=DEV)
+    wide[:, :table.shape[1]] = table
+    check_decode(q, cache, got=mslk_amd.attention_decode(q.to(DEV), k, v, wide, lens, return_lse=True))
+    with pytest.raises(RuntimeError, match="2.30 keys"):
+        mslk_amd.attention_decode(q.to(DEV), k, v, torch.zeros(1, (1 << 20) + 1, dtype=torch.int32, device=DEV).expand(2, -1), lens)
+
+
 def test_decode_long_and_offsets_beyond_32_bits():
     """A pool of more than 2^32 bytes whose used pages lie at both ends."""
     g = torch.Generator().manual_seed(16)
