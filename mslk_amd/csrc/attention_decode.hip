@@ -63,6 +63,7 @@ struct Part {
 };
 MSLK_AMD_DEVINL bool find_part(const DecodeArgs& p, const Line& ln, int w, Part& r) {
   if (!ln.joined) {   // a head block each
+    if (w >= ln.parts) return false;
     r.seq = (int)divide((uint32_t)w, ln.by_head_blocks);
     r.len = __builtin_amdgcn_readfirstlane(length_of(p, r.seq));
     r.index = 0;
@@ -182,7 +183,7 @@ __global__ __launch_bounds__(64, STEPS <= 4 ? 2 : 1) void decode_kernel(DecodeAr
   const float c = p.scale * kLog2e;
 
   Part part;
-  if (!find_part(p, ln, blockIdx.x, part)) return;
+  if (!find_part(p, ln, (int)row_block(), part)) return;
   int at = part.begin;
   int seq = part.seq, len = part.len;
 
@@ -424,7 +425,7 @@ __global__ __launch_bounds__(64, STEPS <= 4 ? 2 : 1) void decode_kernel(DecodeAr
 
 // Joins the pieces of a head block where there is more than one: 4 to 6 us, most of it the launch and the two loads that wait for one
 // another.  (A workgroup of eight waves per head block, joined in LDS in one launch, took 12.3 us for 700 keys and 55 for 4 sequences
-// of 4096, against 9.2 and 19.6: too few waves load.)  Workgroup (x, y): `per` heads of head block x, from y * per on.  A team
+// of 4096, against 9.2 and 19.6: too few waves load.)  Workgroup (x, y, z): `per` heads of head block z kRowGridX + x, from y * per on.  A team
 // of kDP / 4 lanes, four channels each, sums the pieces of a head, or every n-th of them where there are fewer heads than teams.
 typedef float v2f __attribute__((ext_vector_type(2)));
 constexpr int kJoinThreads = 256;
@@ -435,8 +436,10 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(DecodeArgs p, Line l
   __shared__ __attribute__((aligned(16))) float sums[kTeams][kDP];
   __shared__ v2f weights[kTeams];
   const int lane = threadIdx.x % kLanes, team = threadIdx.x / kLanes;
-  const int seq = (int)divide(blockIdx.x, ln.by_head_blocks), hb = blockIdx.x - seq * ln.head_blocks;
-  const int first = p.ends[2 * (int64_t)blockIdx.x], last = p.ends[2 * (int64_t)blockIdx.x + 1];
+  const uint32_t block = blockIdx.z * (uint32_t)kRowGridX + blockIdx.x;
+  const int seq = (int)divide(block, ln.by_head_blocks), hb = block - seq * ln.head_blocks;
+  if (seq >= p.sequences) return;
+  const int first = p.ends[2 * (int64_t)block], last = p.ends[2 * (int64_t)block + 1];
   if (first == last) return;   // one piece: its wave has written the result
   const int pieces = last / 2 - first / 2 + 1;
   const int kv_head = ln.per_kv == 1 ? hb : hb / ln.per_kv, from = (hb - kv_head * ln.per_kv) * kHeads, heads = min(ln.group - from, kHeads);
@@ -493,14 +496,15 @@ int padded(int64_t D) { return D <= 128 ? 128 : 256; }
 
 template <bool F16, Rows ROWS, int STEPS, int SETS>
 hipError_t launch(const DecodeArgs& p, const Line& ln, hipStream_t s) {
-  hipLaunchKernelGGL((decode_kernel<F16, ROWS, STEPS, SETS>), dim3(ln.parts), dim3(64), 0, s, p, ln);
+  hipLaunchKernelGGL((decode_kernel<F16, ROWS, STEPS, SETS>), row_grid(ln.parts), dim3(64), 0, s, p, ln);
   if (hipError_t e = hipGetLastError(); e != hipSuccess || !ln.joined) return e;
   // heads of a workgroup: as many as leave two workgroups per CU
   const int64_t blocks = (int64_t)p.sequences * ln.head_blocks;
   const int most = ln.group < kHeads ? ln.group : kHeads;
   int per = most;
   while (per > 1 && blocks * ((most + per - 1) / per) < 512) per = (per + 1) / 2;
-  hipLaunchKernelGGL((join_kernel<F16, SETS>), dim3((unsigned)blocks, (most + per - 1) / per), dim3(kJoinThreads), 0, s, p, ln, per);
+  const dim3 lines = row_grid(blocks);
+  hipLaunchKernelGGL((join_kernel<F16, SETS>), dim3(lines.x, (most + per - 1) / per, lines.y), dim3(kJoinThreads), 0, s, p, ln, per);
   return hipGetLastError();
 }
 

@@ -625,6 +625,31 @@ def test_decode_with_room_for_2_to_the_30_keys():
         mslk_amd.attention_decode(q.to(DEV), k, v, torch.zeros(1, (1 << 20) + 1, dtype=torch.int32, device=DEV).expand(2, -1), lens)
 
 
+@pytest.mark.parametrize("hkv,room", [(1032, 4), (264, 1040)])
+def test_decode_with_more_workgroups_than_one_line_of_a_grid(hkv, room):
+    """65535 sequences of many heads: more than 2^32 work-items, a head block per wave (little room) and in the join (much of it),
+    against the same call on parts of the sequences.  Values of one sign and about one size, so that the bound of a call is (2 u + 2^-16) |out|
+    (scores of 8 channels: their errors lie below 2^-18), and of two calls twice that."""
+    g = torch.Generator(DEV).manual_seed(18)
+    b, d, page = 65535, 8, 4
+    k, v = torch.randn(300, page, hkv, d, generator=g, device=DEV).bfloat16(), (torch.rand(300, page, hkv, d, generator=g, device=DEV) + 0.5).bfloat16()
+    q = torch.randn(b, hkv, d, generator=g, device=DEV, dtype=torch.bfloat16)
+    table = torch.randint(0, 300, (b, room // page), generator=g, device=DEV, dtype=torch.int32)
+    lens = torch.randint(0, 4, (b,), generator=g, device=DEV, dtype=torch.int32)
+    lens[::256] = room
+    out, lse = mslk_amd.attention_decode(q, k, v, table, lens, return_lse=True)
+    for at in range(0, b, 8192):
+        part = slice(at, min(at + 8192, b))
+        want, want_lse = mslk_amd.attention_decode(q[part], k, v, table[part], lens[part], return_lse=True)
+        empty = lens[part] == 0
+        assert (out[part][empty] == 0).all() and (lse[part][empty] == -math.inf).all()
+        got, want = out[part][~empty].float(), want[~empty].float()
+        assert ((got - want).abs() <= 2 * (2.0 ** -7 + 2.0 ** -16) * want).all()
+        assert ((lse[part] - want_lse)[~empty].abs() <= 2.0 ** -17 * (1 + want_lse[~empty].abs())).all()
+    del q, out, lse
+    torch.cuda.empty_cache()
+
+
 def test_decode_long_and_offsets_beyond_32_bits():
     """A pool of more than 2^32 bytes whose used pages lie at both ends."""
     g = torch.Generator().manual_seed(16)
