@@ -23,6 +23,9 @@ _library = torch.library.Library("mslk", "FRAGMENT")
 
 def _fake_append_kv(q, k, v, k_cache, v_cache, page_table, kv_lens, cu_seqlens=None, rotary=None, interleaved=False, k_scale=None,
                     v_scale=None):
+    for t in (k_cache, v_cache, k_scale, v_scale):   # written, as far as autograd is concerned
+        if t is not None and not t.is_inference():
+            torch.autograd.graph.increment_version(t)
     return torch.empty(q.shape, dtype=q.dtype, device=q.device)
 
 

@@ -652,6 +652,11 @@ mslk_amd_paged_cache cache_of(const char* op, const Tensor& q, const Tensor& k_c
   return c;
 }
 
+// What autograd goes by to see that a tensor it has saved was written.  (Tensors made in inference mode have no version.)
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 Tensor append_kv(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& k_cache, const Tensor& v_cache, const Tensor& page_table,
                  const Tensor& kv_lens, const OptTensor& cu_seqlens, const OptTensor& rotary, bool interleaved, const OptTensor& k_scale,
                  const OptTensor& v_scale) {
@@ -687,6 +692,9 @@ Tensor append_kv(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor
   const HeadsArg hq = heads_of(q), hk = heads_of(k), hv = heads_of(v);
   check_rc(api.mslk_amd_append_kv(&hq.view, &hk.view, &hv.view, float_code(q.scalar_type()), T, Hq, Hkv, D, &cache, cu, sequences, turn, positions,
                                   rotary_dim, interleaved, out.mutable_data_ptr(), stream_of(q)));
+  for (const Tensor* t : {&k_cache, &v_cache}) written(*t);
+  if (cache.dtype == MSLK_AMD_DTYPE_E4M3FN)
+    for (const OptTensor* t : {&k_scale, &v_scale}) written(**t);
   return out;
 }
 

@@ -959,6 +959,46 @@ def test_nothing_joins_a_graph_of_gradients():
     assert not out.requires_grad
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+def test_appending_is_seen_as_a_write(fp8):
+    """A tensor that was saved for a gradient and then written is refused by the backward pass; tensors made in inference mode, which
+    have no version, are written all the same; a compiled step leaves the caches as the eager one does."""
+    g = torch.Generator().manual_seed(35)
+    rows = heads(g, 2, 8, 64, torch.bfloat16).to(DEV)
+    q, k, v = rows[:, :4], rows[:, 4:6], rows[:, 6:]
+    table, lens = torch.tensor([[0, 1], [2, 3]], dtype=torch.int32, device=DEV), torch.tensor([3, 20], dtype=torch.int32, device=DEV)
+
+    def caches():
+        pools = [torch.zeros(4, 16, 2, 64, device=DEV).to(F8 if fp8 else torch.bfloat16) for _ in range(2)]
+        return pools, {"k_scale": torch.zeros(4, 16, 2, device=DEV), "v_scale": torch.zeros(4, 16, 2, device=DEV)} if fp8 else {}
+
+    pools, scales = caches()
+    weight = torch.ones(4, 16, 2, 64 if not fp8 else 1, device=DEV, requires_grad=True)
+    saved = scales["v_scale"][..., None] if fp8 else pools[1]
+    loss = (weight * saved).sum()
+    mslk_amd.append_kv(q, k, v, *pools, table, lens, **scales)
+    assert all(t._version > 0 for t in (*pools, *scales.values()))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+    with torch.inference_mode():
+        others, other_scales = caches()
+    mslk_amd.append_kv(q, k, v, *others, table, lens, **other_scales)
+    with torch.inference_mode():
+        mslk_amd.append_kv(q, k, v, *others, table, lens, **other_scales)
+        assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip((*pools, *scales.values()), (*others, *other_scales.values())))
+
+    def step(q, k, v, pools, scales):
+        turned = mslk_amd.append_kv(q, k, v, *pools, table, lens, **scales)
+        return mslk_amd.attention_decode(turned, *pools, table, lens, *scales.values())
+
+    want = step(q, k, v, pools, scales)
+    again, again_scales = caches()
+    got = torch.compile(step, backend="aot_eager", fullgraph=True)(q, k, v, again, again_scales)
+    assert torch.equal(got, want)
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip((*pools, *scales.values()), (*again, *again_scales.values())))
+
+
 def test_operators_have_shape_functions():
     q, k = torch.randn(4, 4, 64, device=DEV).bfloat16(), torch.randn(4, 2, 64, device=DEV).bfloat16()
     cu = offsets([4]).to(DEV)
