@@ -650,6 +650,55 @@ def test_decode_with_more_workgroups_than_one_line_of_a_grid(hkv, room):
     torch.cuda.empty_cache()
 
 
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d,lens,extra", [(64, [300, 40], 2), (128, [5000, 1], 2), (80, [90, 33], 0), (256, [700, 64], 100)])
+def test_decode_weights_are_not_rounded_to_16_bits(d, lens, extra, dtype, fp8):
+    """The output is off by its own rounding and by its share of the weights' error: 2^-15 where they are two numbers of 8 bits, 2^-20 where
+    they are two of 11, and the scores' error in fp32.  (One number each, 2^-8 and 2^-11, shows where values cancel out.)"""
+    g = torch.Generator().manual_seed(d)
+    cache = Cache(g, lens, 2, d, 16, dtype, fp8, extra=extra)
+    q = heads(g, 2, 8, d, dtype)
+    got = mslk_amd.attention_decode(q.to(DEV), *cache.on_gpu(), return_lse=True)
+    for b, n in enumerate(lens):
+        everything = torch.ones(1, n, dtype=torch.bool)
+        out, _, _, two_delta = attention(q[b:b + 1], cache.k[b], cache.v[b], d ** -0.5, everything)
+        size = attention(q[b:b + 1], cache.k[b], cache.v[b].abs(), d ** -0.5, everything)[0]   # sum of weight times |value|
+        weights = 2.0 ** -15 if dtype == torch.bfloat16 else 2.0 ** -20
+        near(got[0][b:b + 1], out, ROUND[dtype] * out.abs() + (weights + two_delta[..., None]) * size + 2.0 ** -25, f"sequence {b} of {n}")
+
+
+@pytest.mark.parametrize("fp8", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_decode_infinite_values_of_small_weights(dtype, fp8):
+    """A value of infinity makes its channel infinite for every weight down to 2^-20 of the largest, not NaN, and the others stay."""
+    g = torch.Generator().manual_seed(36)
+    n, d = 120, 64
+    k, v = torch.zeros(n, 1, d, dtype=dtype), heads(g, n, 1, d, dtype)
+    k[:, 0, 0] = -(torch.arange(n) / 6.0).to(dtype)          # weights of 2^(-i / 6)
+    q = torch.zeros(n, 1, d, dtype=dtype)
+    q[:, 0, 0] = 1
+    cache = Cache(g, [n], 1, d, 16, dtype, fp8, extra=0, rows=[[k], [v]])   # (few keys of room: not cut, one reference)
+    kc, vc, table, lens, ks, vs = cache.on_gpu()
+    want = mslk_amd.attention_decode(q[:1].to(DEV), kc, vc, table, lens, ks, vs, scale=math.log(2.0))
+    for i in range(n):
+        pools = vc.clone()
+        at = (int(cache.table[0, i // 16]), i % 16, 0, 7)
+        scales = vs
+        if fp8:                                              # e4m3 has no infinity: a row of an infinite scale, its codes not zero
+            pools.view(torch.uint8)[at[:3]] = 0x38
+            scales = vs.clone()
+            scales[at[:3]] = math.inf
+        else:
+            pools[at] = math.inf
+        out = mslk_amd.attention_decode(q[:1].to(DEV), kc, pools, table, lens, ks, scales, scale=math.log(2.0))
+        if fp8:
+            assert (out == math.inf).all(), i
+        else:
+            assert out[0, 0, 7] == math.inf, i
+            assert torch.equal(out[..., torch.arange(d) != 7], want[..., torch.arange(d) != 7]), i
+
+
 def test_decode_long_and_offsets_beyond_32_bits():
     """A pool of more than 2^32 bytes whose used pages lie at both ends."""
     g = torch.Generator().manual_seed(16)
