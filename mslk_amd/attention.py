@@ -11,6 +11,10 @@ pool [pages, kv_heads, page_size, channels] is passed as `pool.transpose(1, 2)`;
 page_size], are read with fewer bytes, because a head's lie side by side.  `page_table` [sequences, width] (int32) names the
 pages of each sequence in order, `kv_lens` [sequences] (int32) says how many keys it has; both are read on the GPU only, so a
 captured graph follows them.  Nothing here is differentiable.
+
+Scores, softmax statistics and sums are fp32.  `attention_decode` keeps 16 bits or more of each softmax weight, so that its output is off
+by its one rounding; `attention_prompt` rounds the weights to the type of the queries, which adds about as much again (relative to 64
+bits 0.002 instead of 0.0016 in bf16, 0.00028 instead of 0.0002 in fp16).
 """
 from __future__ import annotations
 

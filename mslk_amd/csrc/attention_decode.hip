@@ -16,11 +16,13 @@
 // (sequence, head block), what was summed there is written out in 32 bits, together with where the pieces of the block begin and
 // end, and a second launch joins them in their order.  (Short caches are not cut: a wave each for their head blocks.)
 //
-// Bound: the memory.  64 heads of 128 on 8: one sequence of 131071 keys (537 MB) 97.3 us, 5.5 TB/s; 32 sequences of up to 8192 keys
-// (515 MB) 95.8 us, 5.4 TB/s; 128 sequences in e4m3 (1269 MB) 241 us, 5.3 TB/s, and 221 us where a pool keeps its scales by head (one
+// Bound: the memory.  64 heads of 128 on 8: one sequence of 131071 keys (537 MB) 92.5 us, 5.8 TB/s; 32 sequences of up to 8192 keys
+// (515 MB) 94.3 us, 5.5 TB/s; 128 sequences in e4m3 (1269 MB) 234 us, 5.4 TB/s, and 6 % less where a pool keeps its scales by head (one
 // row of 4 bytes per key and head lies among those of the other heads, whose waves fetch the same lines).  A copy moves 5.1 TB/s
 // on the same card, a plain read 6.2.  Short caches are bound by what waits for one another: the lengths, the page numbers, the rows,
-// the second launch: 700 keys on 8 KV heads take 5.1 + 4.6 us in the two kernels, 8.6 us a call in a graph.
+// the second launch: 700 keys on 8 KV heads take 5.1 + 3.0 us in the two kernels, 8.1 to 8.5 us a call in a graph.  With heads of 64 half of
+// a load of values, of the second product and of a piece is padding, and a tile holds half the bytes: 8 sequences of up to 3001 keys
+// (60 MB) 23 us, 2.6 TB/s.
 #include "attention.h"
 #include "rows.h"
 
@@ -30,17 +32,19 @@ namespace mslk_amd {
 namespace {
 
 constexpr int kTile = 32, kHeads = 16;
-// A line of at most kMostParts tiles is cut into parts of one tile, a longer one into kLongParts parts.  Two waves fit a SIMD (kMostParts of
-// them the GPU), but in a long line one keeps the memory busy and there is half as much to join: 1024 against 2048 parts, us: one
-// sequence of 131071 keys 99 / 105, 128 sequences in e4m3 247 / 257.  Short lines have no tile to load while another is computed:
-// 256 sequences of 4 keys (2048 tiles) 11.5 in parts of one, 14.0 in 1024 parts.
+// A line of at most kMostParts tiles is cut into parts of one tile, a longer one into kLongParts parts.  Two waves fit a SIMD up to D = 128
+// (kMostParts of them the GPU), but in a long line one keeps the memory busy and there is half as much to join: 1024 against 2048 parts,
+// us, heads of 128: one sequence of 131071 keys 94.3 / 99.4, 4 of 4096 19.4 / 20.8, 128 in e4m3 243 / 252; heads of 256, 16 on 4, 32 sequences of
+// up to 4096 keys 62.6 / 67.5, in e4m3 38.1 / 44.7; heads of 64 in e4m3 50.8 / 52.4.  Heads of 64 in 16 bits, whose tiles hold half the
+// bytes, are better off the other way: 8 sequences of up to 3001 keys 24.1 / 21.2, 32 of up to 8192 63.9 / 61.8.  Short lines have no
+// tile to load while another is computed: 256 sequences of 4 keys (2048 tiles) took 11.5 in parts of one, 14.0 in 1024 parts.
 constexpr int kMostParts = 2048, kLongParts = 1024;
 
 // Where the page tables hold few keys, or not many more than there are head blocks, a wave takes a whole head block instead, and there
-// is nothing to join.  In parts against whole, us, 32 heads on 8: 100 keys, 1 sequence 8.3 / 7.2, 64 sequences 13.6 / 8.5; 250 keys, 1
-// sequence 8.3 / 10.1, 16 10.6 / 10.4, 64 18.0 / 13.8; 500 keys, 16 sequences 15.1 / 16.7, 32 17.9 / 17.0, 128 45.0 / 39.8; 1000 keys, 16
-// sequences 18.8 / 28.6, 64 41.4 / 41.5, 128 79.0 / 78.2, and of 1 to 1000 keys 76.0 / 60.2 (a part there holds pieces of several
-// blocks, each with its own start).  Longer ones, 64 of 1 to 4000 keys: 94.7 / 126.8, the longest block long after the others.
+// is nothing to join.  In parts against whole, us, 32 heads on 8: 100 keys, 1 sequence 7.4 / 6.8, 64 sequences 14.9 / 9.3; 250 keys, 1
+// sequence 7.5 / 10.2, 16 10.9 / 10.8, 64 18.3 / 14.9; 500 keys, 16 sequences 16.7 / 18.9, 32 18.6 / 19.1, 128 52.2 / 49.2; 1000 keys, 16
+// sequences 19.1 / 32.4, 64 53.0 / 48.9, 128 94.5 / 92.1, and of 1 to 1000 keys 77.7 / 60.7 (a part there holds pieces of several
+// blocks, each with its own start).  Longer ones, 64 of 1 to 4000 keys: 95.4 / 132.9, the longest block long after the others.
 constexpr int kWholeKeys = 128, kMostWholeKeys = 1024;
 
 struct Line {          // how the work is divided
@@ -85,9 +89,9 @@ MSLK_AMD_DEVINL bool find_part(const DecodeArgs& p, const Line& ln, int w, Part&
   const uint32_t parts = total <= kMostParts ? total : kLongParts;   // none of them empty
   if ((uint32_t)w >= parts) return false;
   // Workgroup i runs on XCD i % 8.  Neighbours in the line go to one XCD where they share lines: the scales of the heads of a key
-  // (128 sequences in e4m3, 64 heads on 8: 246 -> 241 us; 8 sequences, 16 heads of 64: 21.8 -> 20.6), the pieces that one join reads
-  // and the page table (700 keys: 9.2 -> 8.6).  Long lines of 16-bit rows, which share nothing, are better spread: 64 sequences of 1024
-  // keys 53.3, by neighbours 54.6; heads of 256 72.2 / 76.9.
+  // (128 sequences in e4m3, 64 heads on 8: 245.5 -> 242.8 us), the pieces that one join reads and the page table (700 keys: 8.7 -> 8.1).
+  // Long lines of 16-bit rows, which share nothing, are better spread: 64 sequences of 1024 keys 54.4, by neighbours 55.4; 32 of up to
+  // 4096 keys, 16 heads of 256 on 4, 62.5 / 63.1; though 8 of up to 3001 keys, 16 heads of 64, 24.1 / 23.8.
   if (p.fp8 || parts == total) w = (w % 8) * (parts / 8) + min((uint32_t)w % 8, parts % 8) + w / 8;
   r.index = w;
   const uint32_t each = parts == total ? 1 : total / parts, more = total - each * parts;   // the first `more` parts hold one tile more
@@ -444,7 +448,7 @@ __global__ __launch_bounds__(64, STEPS <= 4 ? 2 : 1) void decode_kernel(DecodeAr
   }
 }
 
-// Joins the pieces of a head block where there is more than one: 4 to 6 us, most of it the launch and the two loads that wait for one
+// Joins the pieces of a head block where there is more than one: 3 to 6 us, most of it the launch and the two loads that wait for one
 // another.  (A workgroup of eight waves per head block, joined in LDS in one launch, took 12.3 us for 700 keys and 55 for 4 sequences
 // of 4096, against 9.2 and 19.6: too few waves load.)  Workgroup (x, y, z): `per` heads of head block z kRowGridX + x, from y * per on.  A team
 // of kDP / 4 lanes, four channels each, sums the pieces of a head, or every n-th of them where there are fewer heads than teams.

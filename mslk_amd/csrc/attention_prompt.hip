@@ -14,12 +14,17 @@
 // The reference m follows the maximum when it is left behind by more than 8 powers of two, so that the sums are seldom scaled; weights
 // are below 2^8 and rounded once to 16 bits, l sums them unrounded.
 //
-// Bound: long prompts by the power of the matrix cores: 16384 tokens, 32 heads of 128 on 8, causal, 2020 us, 1090 TFLOP/s of what the mask
-// leaves; with operands of zeros the same kernel runs at a higher clock and a quarter faster, and without any softmax it would gain 11 %.
-// (The 32x32x16 form of both products: 2182 us; it draws more for the same operations.)  Ragged batches (8192 tokens in nine
-// sequences, 64 heads: 473 us, 840 TFLOP/s) lose the rest to masked halves of tiles and to starting workgroups, 4 us each; few
-// and short prompts are bound by a tile's chain of copies, products and softmax, 1.3 us for a workgroup alone on its CU (3100 cycles,
-// 1000 of them matrix instructions): 100 tokens 6.9 us, 1000 tokens 20 us.
+// The weights' rounding is the one thing here that a computation in 32 bits does not have: it adds 2^-9 in bf16 (2^-12 in fp16) to an
+// output that is rounded by as much itself, 0.0019 to 0.0023 from 64 bits instead of 0.0016.  Two numbers per weight, as in
+// attention_decode.hip, would be half as many matrix instructions again in a kernel that these bind.
+//
+// Bound (profiles/attention_rules.txt): long prompts by the power of the matrix cores: 16384 tokens, 32 heads of 128 on 8, causal, 1780 to
+// 1960 us by the card, 1120 to 1240 TFLOP/s of what the mask leaves; busy 0.63 of the time at 1.72 GHz, and with operands of zeros just as
+// busy at 2.23 GHz and 26 % faster; without any softmax it would gain 18 %.  (The 32x32x16 form of both products was 8 % slower.)  Ragged
+// batches (8192 tokens in nine sequences, 64 heads: 427 to 459 us) lose the rest to products behind the mask, 13 % of all, and to the
+// tiles that the mask cuts, 17 %, whose copies, products and softmax do not overlap; so do heads of 96 without a mask (46 us, matrix
+// cores busy 0.31 at full clock: two workgroups per CU are too few to hide one another's softmax).  Few and short prompts are bound by a
+// tile's chain of copies, products and softmax, 0.7 us for a workgroup of 64 queries alone: 100 tokens 6.0 us, 1000 tokens 21.
 #include <algorithm>
 
 #include "attention.h"
@@ -33,9 +38,10 @@ constexpr int kGridY = 32768;   // blocks of queries per grid row
 
 // DP: head dimension rounded up to what the operands are padded to.  Q: queries of a workgroup.
 template <int DP, int Q> struct Shape {
-  // Blocks of 16 queries per wave.  Two halve the reads of LDS per matrix instruction (16384 tokens: 2005 us, with eight waves of one
-  // block 2327).  Beyond D = 128 two do not fit 256 registers, and one wave per SIMD has nothing to run beside its softmax: 8192 tokens, 16
-  // heads of 256, 940 us with four waves of two, 550 with eight of one.
+  // Blocks of 16 queries per wave.  Two halve the reads of LDS per matrix instruction (16384 tokens, D = 128: 1955 us, with eight waves of
+  // one block 2375; 8192 tokens, D = 64: 323 / 342).  Beyond D = 128 two do not fit 256 registers, and one wave per SIMD has nothing to run
+  // beside its softmax: 8192 tokens, 16 heads of 256, 579 us with eight waves of one block; four waves of two had taken 940 where that
+  // form took 550.
   static constexpr int kB = DP <= 128 && Q == 128 ? 2 : 1;
   static constexpr int kWaveQ = 16 * kB, kWaves = Q / kWaveQ;
 };
@@ -88,9 +94,9 @@ MSLK_AMD_DEVINL Sequence<Q> sequence(const PromptArgs& p, int b) {
 // sequences, which see nothing.
 //
 // Few workgroups are sorted, so that the last ones to start are short; of many, those that run together rather share keys in the
-// L2.  Sorted against not, us: 8192 tokens in 9 sequences, causal, D = 128, 600 workgroups 67.0 / 68.2, 1200 94.0 / 104, 2400 181.7 /
-// 184.4, 4800 317 / 313; 6000 tokens in 13 sequences, not causal, D = 96, 976 workgroups 46.8 / 51.4, 1952 88.4 / 93.6, 3904 165.3 /
-// 160.8; but 4873 tokens in 8 sequences, causal, 1536 workgroups 79.8 / 76.7.
+// L2.  Sorted against not, us: 8192 tokens in 9 sequences, causal, D = 128, 600 workgroups 51.3 / 51.8, 1200 69.4 / 71.1, 2400 163.5 /
+// 162.3, 4800 258 / 253; 6000 tokens in 13 sequences, not causal, D = 96, 976 workgroups 47.5 / 48.6, 1952 84.3 / 85.9, 3904 152.6 /
+// 152.2; 4873 tokens in 8 sequences, causal, 1536 workgroups 59.4 / 64.0.
 constexpr int kSortedBlocks = 2048;
 template <int Q>
 MSLK_AMD_DEVINL bool find_work(const PromptArgs& p, int index, bool sorted, Work& w) {
@@ -216,7 +222,10 @@ __global__ __launch_bounds__((64 * Shape<DP, Q>::kWaves), 2) void prompt_kernel(
   int head = blockIdx.x;
   const int index = blockIdx.y + blockIdx.z * kGridY;
   if (index >= blocks) return;
-  if (p.Hkv % 8 == 0) head = head % 8 * (p.Hq / 8) + head / 8;   // workgroup i runs on XCD i % 8: heads that share keys on one XCD
+  // Workgroup i runs on XCD i % 8: heads that share keys on one XCD, where the KV heads can be dealt out evenly.  With against without, us: 64
+  // heads on 8, 8192 tokens in nine sequences 457 / 480, 4096 tokens 281 / 286; 16 heads of 96 on 16 46.8 / 48.4; 32 heads on 8, 16384 tokens
+  // 1963 / 1964.
+  if (p.Hkv % 8 == 0) head = head % 8 * (p.Hq / 8) + head / 8;
   Work w;
   if (!find_work<Q>(p, index, p.sequences > 1 && p.sequences <= 64 && (int64_t)blocks * p.Hq <= kSortedBlocks, w)) return;
   w.q_row = uniform64(w.q_row);
@@ -534,9 +543,10 @@ hipError_t launch(const PromptArgs& p, int64_t blocks, hipStream_t s) {
 }
 // Few workgroups of 128 queries (up to two per CU, or one where LDS holds no second) leave the matrix cores waiting for one another's
 // softmax and the last workgroup long: blocks of 64 queries then, in waves of 16, though LDS is read twice as often.  128 against 64, us:
-// D = 128 on 32 heads, causal: 100 tokens (96 workgroups) 8.5 / 6.5, 256 (160) 12.5 / 8.4, 500 (192) 17.2 / 11.7, 1000 (320) 27.0 / 20.1,
-// 1400 (448) 37.7 / 28.7, 2048 (608) 52.4 / 51.0; 20 sequences of 100 on 16 heads (592) 12.4 / 14.1; 6000 tokens in 13 sequences on 16
-// heads (976) 47 / 57.  D = 256, 1000 tokens: 16 heads (160) 36.5 / 31.3, 32 heads (320) 39.0 / 41.1.
+// D = 128 on 32 heads, causal: 100 tokens (96 workgroups) 8.0 / 6.0, 256 (160) 11.5 / 8.0, 500 (192) 16.4 / 11.2, 1000 (320) 26.8 / 20.5,
+// 1400 (448) 35.3 / 29.0, 2048 (608) 52.4 / 53.0; 20 sequences of 100 tokens on 16 heads (592) 14.9 / 14.8; 6000 tokens in 13 sequences on
+// 16 heads of 96 (976) 50.4 / 55.0.  D = 64 on 32 heads: 1000 tokens 18.3 / 12.8, 2048 33.3 / 31.6.  D = 256, 1000 tokens: 16 heads (160)
+// 36.6 / 29.6, 32 heads (320) 39.4 / 39.3.
 template <int DP> constexpr int kFewBlocks = DP <= 128 ? 512 : 256;
 template <bool F16, int DP>
 hipError_t launch(const PromptArgs& p, hipStream_t s) {
