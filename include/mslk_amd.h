@@ -375,6 +375,40 @@ int mslk_amd_attention_prompt(const mslk_amd_heads* q, const mslk_amd_heads* k, 
                               void* stream);
 
 /*
+ * Microscaled 4-bit floating point (MXFP4, the OCP microscaling format): a row of K values (K a multiple of 32) is K / 32 blocks
+ * of 32 e2m1 codes, two to a byte with the earlier value in the low half, and a scale byte s per block that stands for
+ * 2^(s - 127), 255 for NaN.  Codes [rows, K / 2] and scales [rows, K / 32], row-major contiguous.
+ *
+ * Quantizer: of a block with the largest magnitude a, s = max(floor(log2 a) + 125, 0) and code = e2m1(v 2^(127 - s)), rounded to
+ * nearest even, magnitudes above 6 to 6.  A block with a NaN or an infinity: scale 255, codes 0.  No counterpart in the reference's
+ * FP8 path, like the rest of this section.
+ *   a [rows, K] elements of a_dtype (bf16, fp16, fp32), row stride a_row_stride elements; codes 4-byte aligned.  K < 2^31.
+ */
+int mslk_amd_quantize_mxfp4(const void* a, int a_dtype, int64_t rows, int64_t K, int64_t a_row_stride, void* codes, void* scales,
+                            void* stream);
+
+/* What codes and scales stand for, as bf16, fp16 or fp32 [rows, K]; codes 4-byte aligned, out 16-byte aligned. */
+int mslk_amd_dequantize_mxfp4(const void* codes, const void* scales, int64_t rows, int64_t K, void* out, int out_dtype, void* stream);
+
+/*
+ * y[m, n] = sum_k X[m, k] W[n, k] + bias[n], fp32 sums rounded once to y_dtype (bf16, fp16).
+ * gated != 0: W has 2 N rows, a gate's N rows and then N more, and y = silu(X Wg^T) * (X Wu^T) (no bias); N K < 2^32.
+ *   xq [M, K / 2], wq [N or 2 N, K / 2] codes, 16-byte aligned; x_scale, w_scale their scales; y [M, N].  K < 2^24.
+ *   workspace: mslk_amd_mxfp4_mm_workspace_bytes() of it, 16-byte aligned; `aligned` != 0 says that both scale pointers are 16-byte
+ *   aligned.  Nothing in it is kept from one call to the next.
+ * grouped: row g of the stacked weights wq [G, N or 2 N, K / 2], w_scale [G, N or 2 N, K / 32] belongs to the next m_sizes[g] rows of X
+ *   (int64, device memory).  Rows beyond the sum of the sizes are left untouched; sizes below 0 count as 0.
+ */
+size_t mslk_amd_mxfp4_mm_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated, int aligned);
+int mslk_amd_mxfp4_mm(const void* xq, const void* wq, const void* x_scale, const void* w_scale, const void* bias, int bias_dtype,
+                      int gated, void* y, int y_dtype, int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes,
+                      void* stream);
+size_t mslk_amd_mxfp4_grouped_mm_workspace_bytes(int G, int64_t total_M, int64_t N, int64_t K, int gated, int aligned);
+int mslk_amd_mxfp4_grouped_mm(const void* xq, const void* wq, const void* x_scale, const void* w_scale, const int64_t* m_sizes_dev,
+                              int G, int gated, void* y, int y_dtype, int64_t total_M, int64_t N, int64_t K, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/*
  * Self-test helper: converts n fp32 values to e4m3fn with the same device routine the quantizer
  * uses (hardware v_cvt_pk_fp8_f32 plus the NaN fix-up for |v| > 464).  Used by the parity tests to
  * sweep the conversion against the oracle; no counterpart in the reference.

@@ -80,6 +80,14 @@ SIGNATURES = {
                                           c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
     "mslk_amd_attention_prompt": (c_int, [POINTER(Heads), POINTER(Heads), POINTER(Heads), c_int, c_int64, c_int64, c_int64, c_int64,
                                           c_int64, c_void_p, c_void_p, c_int64, c_int, c_float, c_void_p, c_void_p, c_void_p]),
+    "mslk_amd_quantize_mxfp4": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "mslk_amd_dequantize_mxfp4": (c_int, [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int, c_void_p]),
+    "mslk_amd_mxfp4_mm_workspace_bytes": (c_size_t, [c_int64, c_int64, c_int64, c_int, c_int]),
+    "mslk_amd_mxfp4_mm": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_int64, c_int64,
+                                  c_int64, c_void_p, c_size_t, c_void_p]),
+    "mslk_amd_mxfp4_grouped_mm_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64, c_int, c_int]),
+    "mslk_amd_mxfp4_grouped_mm": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_int64,
+                                          c_int64, c_int64, c_void_p, c_size_t, c_void_p]),
     "mslk_amd_debug_cast_e4m3fn": (c_int, [c_void_p, c_int64, c_void_p, c_void_p]),
     "mslk_amd_debug_dispatch_name": (c_char_p, [c_int64, c_int64, c_int64, c_int, c_int, c_int, c_int]),
     "mslk_amd_debug_grouped_dispatch_name": (c_char_p, [c_int, c_int, c_int64, c_int64, c_int64]),

@@ -9,6 +9,7 @@
 #include "../../include/mslk_amd.h"
 #include "attention.h"
 #include "kernels.h"
+#include "mx.h"
 
 namespace {
 
@@ -122,6 +123,26 @@ int check_cache(const char* op, const mslk_amd_paged_cache* c, int dtype, int64_
 }
 int check_scale(const char* op, float scale) {   // (the kernels multiply by scale log2(e), which has to be finite too)
   return scale > 0.f && scale <= 2e38f ? 0 : fail("%s: scale must be positive and at most 2e38", op);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// MXFP4: checks shared by its products
+// ---------------------------------------------------------------------------------------------------------------------
+int check_mx(const char* op, const void* xq, const void* wq, const void* x_scale, const void* w_scale, const void* y, int y_dtype, int64_t M, int64_t N,
+             int64_t K, int gated, int G, const void* workspace, size_t workspace_bytes, size_t wanted) {
+  if (M < 0 || N < 0 || K < 0 || G < 0) return fail("%s: negative dimension", op);
+  if (K % 32 != 0) return fail("%s: K must be a multiple of 32 (got %lld)", op, (long long)K);
+  if (M > kIntMax || N > kIntMax || K >= (int64_t(1) << 24)) return fail("%s: dimension out of range (M, N < 2^31, K < 2^24)", op);
+  if (gated && (N + 256) * K >= (int64_t(1) << 33)) return fail("%s: gated weights of N = %lld, K = %lld are too large (N K < 2^32)", op, (long long)N, (long long)K);
+  if (y_dtype != MSLK_AMD_DTYPE_BF16 && y_dtype != MSLK_AMD_DTYPE_F16) return fail("%s: bf16 or fp16 output expected (dtype code %d)", op, y_dtype);
+  if (M == 0 || N == 0) return 0;
+  if (!y) return fail("%s: null output", op);
+  if (!aligned(y, 2)) return fail("%s: the output must be 2-byte aligned", op);
+  if (K > 0 && (!xq || !wq || !x_scale || !w_scale)) return fail("%s: null pointer", op);
+  if (!aligned(xq, 16) || !aligned(wq, 16)) return fail("%s: codes must be 16-byte aligned", op);
+  if (wanted > 0 && (!workspace || workspace_bytes < wanted || !aligned(workspace, 16)))
+    return fail("%s: a 16-byte aligned workspace of %zu bytes is wanted", op, wanted);
+  return 0;
 }
 
 }  // namespace
@@ -611,6 +632,73 @@ int mslk_amd_attention_prompt(const mslk_amd_heads* q, const mslk_amd_heads* k, 
   p.group = divider((uint32_t)(Hq / Hkv));
   p.scale = scale;
   return check_hip(launch_attention_prompt(p, (hipStream_t)stream), "attention_prompt launch");
+}
+
+int mslk_amd_quantize_mxfp4(const void* a, int a_dtype, int64_t rows, int64_t K, int64_t a_row_stride, void* codes, void* scales, void* stream) {
+  const char* op = "quantize_mxfp4";
+  if (a_dtype < 0 || a_dtype > 2) return fail("%s: unsupported input dtype code %d", op, a_dtype);
+  if (rows < 0 || K < 0 || K > kIntMax) return fail("%s: dimension out of range", op);
+  if (K % 32 != 0) return fail("%s: K must be a multiple of 32 (got %lld)", op, (long long)K);
+  if (a_row_stride < 0) return fail("%s: negative row stride", op);
+  if (rows == 0 || K == 0) return 0;
+  if (!a || !codes || !scales) return fail("%s: null pointer", op);
+  if (!aligned(codes, 4) || !aligned(a, a_dtype == MSLK_AMD_DTYPE_F32 ? 4 : 2)) return fail("%s: misaligned pointer", op);
+  return check_hip(launch_quantize_mxfp4(a, a_dtype, rows, K, a_row_stride, codes, scales, (hipStream_t)stream), "quantize_mxfp4 launch");
+}
+
+int mslk_amd_dequantize_mxfp4(const void* codes, const void* scales, int64_t rows, int64_t K, void* out, int out_dtype, void* stream) {
+  const char* op = "dequantize_mxfp4";
+  if (out_dtype < 0 || out_dtype > 2) return fail("%s: unsupported output dtype code %d", op, out_dtype);
+  if (rows < 0 || K < 0 || K > kIntMax) return fail("%s: dimension out of range", op);
+  if (K % 32 != 0) return fail("%s: K must be a multiple of 32 (got %lld)", op, (long long)K);
+  if (rows == 0 || K == 0) return 0;
+  if (!codes || !scales || !out) return fail("%s: null pointer", op);
+  if (!aligned(codes, 4) || !aligned(out, 16)) return fail("%s: misaligned pointer", op);
+  return check_hip(launch_dequantize_mxfp4(codes, scales, rows, K, out, out_dtype, (hipStream_t)stream), "dequantize_mxfp4 launch");
+}
+
+size_t mslk_amd_mxfp4_mm_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated, int aligned) {
+  if (M > kIntMax || N > kIntMax || K >= (int64_t(1) << 24)) return 0;
+  return mx_workspace_bytes(M, N, K, gated, 1, false, aligned != 0);
+}
+
+int mslk_amd_mxfp4_mm(const void* xq, const void* wq, const void* x_scale, const void* w_scale, const void* bias, int bias_dtype, int gated,
+                      void* y, int y_dtype, int64_t M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* op = gated ? "mxfp4_gated_mm" : "mxfp4_mm";
+  const bool scales_aligned = aligned(x_scale, 16) && aligned(w_scale, 16);
+  if (int rc = check_mx(op, xq, wq, x_scale, w_scale, y, y_dtype, M, N, K, gated, 1, workspace, workspace_bytes,
+                        mslk_amd_mxfp4_mm_workspace_bytes(M, N, K, gated, scales_aligned)))
+    return rc;
+  if (bias_dtype < 0 || bias_dtype > 2) return fail("%s: bad bias dtype code %d", op, bias_dtype);
+  if ((bias_dtype != 0) != (bias != nullptr)) return fail("%s: bias pointer and bias dtype disagree", op);
+  if (gated && bias) return fail("%s: a gated product takes no bias", op);
+  if (M == 0 || N == 0) return 0;
+  MxProblem p{};
+  p.xq = (const uint8_t*)xq; p.wq = (const uint8_t*)wq; p.xs = (const uint8_t*)x_scale; p.ws = (const uint8_t*)w_scale;
+  p.bias = bias; p.bias_dtype = bias_dtype; p.y = (uint16_t*)y; p.out_f16 = y_dtype == MSLK_AMD_DTYPE_F16;
+  p.M = (int)M; p.N = (int)N; p.K = (int)K; p.gated = gated != 0;
+  return check_hip(launch_mx_mm(p, workspace, scales_aligned, (hipStream_t)stream), op);
+}
+
+size_t mslk_amd_mxfp4_grouped_mm_workspace_bytes(int G, int64_t total_M, int64_t N, int64_t K, int gated, int aligned) {
+  if (total_M > kIntMax || N > kIntMax || K >= (int64_t(1) << 24) || G <= 0) return 0;
+  return mx_workspace_bytes(total_M, N, K, gated, G, true, aligned != 0);
+}
+
+int mslk_amd_mxfp4_grouped_mm(const void* xq, const void* wq, const void* x_scale, const void* w_scale, const int64_t* m_sizes_dev, int G, int gated,
+                              void* y, int y_dtype, int64_t total_M, int64_t N, int64_t K, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* op = "mxfp4_grouped_mm";
+  const bool scales_aligned = aligned(x_scale, 16) && aligned(w_scale, 16);
+  if (int rc = check_mx(op, xq, wq, x_scale, w_scale, y, y_dtype, total_M, N, K, gated, G, workspace, workspace_bytes,
+                        mslk_amd_mxfp4_grouped_mm_workspace_bytes(G, total_M, N, K, gated, scales_aligned)))
+    return rc;
+  if (total_M == 0 || N == 0 || G == 0) return 0;
+  if (!m_sizes_dev) return fail("%s: null pointer", op);
+  MxProblem p{};
+  p.xq = (const uint8_t*)xq; p.wq = (const uint8_t*)wq; p.xs = (const uint8_t*)x_scale; p.ws = (const uint8_t*)w_scale;
+  p.y = (uint16_t*)y; p.out_f16 = y_dtype == MSLK_AMD_DTYPE_F16;
+  p.M = (int)total_M; p.N = (int)N; p.K = (int)K; p.gated = gated != 0; p.G = G; p.m_sizes = m_sizes_dev;
+  return check_hip(launch_mx_mm(p, workspace, scales_aligned, (hipStream_t)stream), op);
 }
 
 int mslk_amd_debug_cast_e4m3fn(const float* in, int64_t n, void* out, void* stream) {

@@ -57,7 +57,13 @@ constexpr auto kF8 = at::kFloat8_e4m3fn;
   X(mslk_amd_append_kv)                                                                                                \
   X(mslk_amd_attention_decode_workspace_bytes)                                                                         \
   X(mslk_amd_attention_decode)                                                                                         \
-  X(mslk_amd_attention_prompt)
+  X(mslk_amd_attention_prompt)                                                                                         \
+  X(mslk_amd_quantize_mxfp4)                                                                                           \
+  X(mslk_amd_dequantize_mxfp4)                                                                                         \
+  X(mslk_amd_mxfp4_mm_workspace_bytes)                                                                                 \
+  X(mslk_amd_mxfp4_mm)                                                                                                 \
+  X(mslk_amd_mxfp4_grouped_mm_workspace_bytes)                                                                         \
+  X(mslk_amd_mxfp4_grouped_mm)
 
 struct Api {
 #define X(name) decltype(&::name) name = nullptr;
@@ -746,6 +752,123 @@ std::tuple<Tensor, Tensor> attention_prompt(const Tensor& q, const Tensor& k, co
   return {out, lse};
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// MXFP4 (mslk_amd/mxfp4.py)
+// ---------------------------------------------------------------------------------------------------------------------
+std::tuple<Tensor, Tensor> quantize_mxfp4(const Tensor& a) {
+  const char* op = "quantize_mxfp4";
+  const int code = float_code(a.scalar_type());
+  TORCH_CHECK(code >= 0, op, ": unsupported input dtype ", a.scalar_type(), " (bf16, fp16, fp32 are supported)");
+  TORCH_CHECK(a.is_cuda(), op, ": input must be a GPU tensor");
+  TORCH_CHECK(a.dim() >= 1 && a.size(-1) % 32 == 0, op, ": the last dimension must be a multiple of 32, got ", a.sizes());
+  const int64_t K = a.size(-1), rows = rows_of(a);
+  // The kernel takes one row stride; anything else (transposed views, broadcast columns) is packed first.
+  const bool strided_rows = a.dim() == 2 && a.stride(-1) == 1;
+  const auto a2 = strided_rows ? c10::MaybeOwned<Tensor>::borrowed(a) : contiguous(a);
+  Tensor codes = empty_on(leading(a, K / 2), at::kByte, a), scales = empty_on(leading(a, K / 32), at::kByte, a);
+  if (rows == 0 || K == 0) return {codes, scales};
+  const c10::DeviceGuard guard(a.device());
+  check_rc(api.mslk_amd_quantize_mxfp4(a2->const_data_ptr(), code, rows, K, strided_rows ? a.stride(0) : K, codes.mutable_data_ptr(),
+                                       scales.mutable_data_ptr(), stream_of(a)));
+  return {codes, scales};
+}
+
+// Codes and scales as bytes or as the torch types of the same bits.
+bool holds_codes(const Tensor& t) { return t.scalar_type() == at::kByte || t.scalar_type() == at::kFloat4_e2m1fn_x2; }
+bool holds_scales(const Tensor& t) { return t.scalar_type() == at::kByte || t.scalar_type() == at::kFloat8_e8m0fnu; }
+
+void check_mx_pair(const char* op, const char* name, const Tensor& codes, const Tensor& scales, const Tensor& like) {
+  TORCH_CHECK(holds_codes(codes), op, ": ", name, " must hold codes as uint8 or float4_e2m1fn_x2, got ", codes.scalar_type());
+  TORCH_CHECK(holds_scales(scales), op, ": the scales of ", name, " must be uint8 or float8_e8m0fnu, got ", scales.scalar_type());
+  TORCH_CHECK(codes.is_cuda() && codes.is_contiguous(), op, ": ", name, " must be a contiguous GPU tensor");
+  TORCH_CHECK(codes.device() == like.device() && scales.device() == like.device(), op, ": all operands must be on the same device");
+  TORCH_CHECK(codes.dim() >= 1 && codes.size(-1) % 16 == 0, op, ": ", name, " must hold whole blocks of 32 codes (16 bytes), got ", codes.sizes());
+  TORCH_CHECK(scales.dim() == codes.dim() && scales.sizes().slice(0, scales.dim() - 1) == codes.sizes().slice(0, codes.dim() - 1) &&
+                  scales.size(-1) * 16 == codes.size(-1),
+              op, ": ", name, " of ", codes.sizes(), " goes with one scale per 16 bytes of each row, got ", scales.sizes());
+}
+
+Tensor dequantize_mxfp4(const Tensor& codes, const Tensor& scales, std::optional<at::ScalarType> out_dtype) {
+  const char* op = "dequantize_mxfp4";
+  check_mx_pair(op, "codes", codes, scales, codes);
+  const at::ScalarType dtype = out_dtype.value_or(at::kBFloat16);
+  const int code = float_code(dtype);
+  TORCH_CHECK(code >= 0, op, ": out_dtype must be bfloat16, float16 or float32, got ", dtype);
+  const int64_t K = codes.size(-1) * 2, rows = rows_of(codes);
+  Tensor out = empty_on(leading(codes, K), dtype, codes);
+  if (rows == 0 || K == 0) return out;
+  const c10::DeviceGuard guard(codes.device());
+  const Tensor c = reinterpret_cast<uintptr_t>(codes.const_data_ptr()) % 4 == 0 ? codes : codes.clone();
+  const auto s = contiguous(scales);
+  check_rc(api.mslk_amd_dequantize_mxfp4(c.const_data_ptr(), s->const_data_ptr(), rows, K, out.mutable_data_ptr(), code, stream_of(codes)));
+  return out;
+}
+
+int mx_output(const char* op, std::optional<at::ScalarType> out_dtype) {
+  const at::ScalarType dtype = out_dtype.value_or(at::kBFloat16);
+  TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kHalf, op, ": out_dtype must be bfloat16 or float16, got ", dtype);
+  return float_code(dtype);
+}
+at::ScalarType type_of(int code) { return code == MSLK_AMD_DTYPE_F16 ? at::kHalf : at::kBFloat16; }
+Tensor fetchable(const Tensor& codes) { return aligned16(codes) ? codes : codes.clone(); }   // (a view that begins inside 16 bytes)
+
+Tensor mx_product(const char* op, const Tensor& XQ, const Tensor& WQ, const Tensor& x_scale, const Tensor& w_scale, const OptTensor& bias,
+                  std::optional<at::ScalarType> out_dtype, bool gated) {
+  check_mx_pair(op, "XQ", XQ, x_scale, XQ);
+  check_mx_pair(op, "WQ", WQ, w_scale, XQ);
+  TORCH_CHECK(WQ.dim() == 2, op, ": WQ must be 2-D, got ", WQ.sizes());
+  TORCH_CHECK(XQ.size(-1) == WQ.size(1), op, ": XQ and WQ must share K, got ", 2 * XQ.size(-1), " vs ", 2 * WQ.size(1));
+  TORCH_CHECK(!gated || WQ.size(0) % 2 == 0, op, ": WQ must hold as many gate rows as others, got ", WQ.size(0), " rows");
+  const int code = mx_output(op, out_dtype);
+  const int64_t M = rows_of(XQ), K = 2 * XQ.size(-1), N = WQ.size(0) / (gated ? 2 : 1);
+  const Bias b = bias_of(bias, N, XQ);
+  Tensor Y = empty_on(leading(XQ, N), type_of(code), XQ);
+  if (M == 0 || N == 0) return Y;
+  const c10::DeviceGuard guard(XQ.device());
+  const Tensor x = fetchable(XQ), w = fetchable(WQ);
+  const auto xs = contiguous(x_scale), ws = contiguous(w_scale);
+  const size_t bytes = api.mslk_amd_mxfp4_mm_workspace_bytes(M, N, K, gated, aligned16(*xs) && aligned16(*ws));
+  Tensor workspace;
+  if (bytes > 0) workspace = empty_on({(int64_t)bytes}, at::kByte, XQ);
+  check_rc(api.mslk_amd_mxfp4_mm(x.const_data_ptr(), w.const_data_ptr(), xs->const_data_ptr(), ws->const_data_ptr(), b.ptr, b.code, gated,
+                                 Y.mutable_data_ptr(), code, M, N, K, bytes > 0 ? workspace.mutable_data_ptr() : nullptr, bytes, stream_of(XQ)));
+  return Y;
+}
+
+Tensor mxfp4_mm(const Tensor& XQ, const Tensor& WQ, const Tensor& x_scale, const Tensor& w_scale, const OptTensor& bias,
+                std::optional<at::ScalarType> out_dtype) {
+  return mx_product("mxfp4_mm", XQ, WQ, x_scale, w_scale, bias, out_dtype, false);
+}
+Tensor mxfp4_gated_mm(const Tensor& XQ, const Tensor& WQ, const Tensor& x_scale, const Tensor& w_scale, std::optional<at::ScalarType> out_dtype) {
+  return mx_product("mxfp4_gated_mm", XQ, WQ, x_scale, w_scale, std::nullopt, out_dtype, true);
+}
+
+Tensor mxfp4_grouped_mm(const Tensor& XQ, const Tensor& WQ, const Tensor& x_scale, const Tensor& w_scale, const Tensor& M_sizes, bool gated,
+                        std::optional<at::ScalarType> out_dtype) {
+  const char* op = "mxfp4_grouped_mm";
+  check_mx_pair(op, "XQ", XQ, x_scale, XQ);
+  check_mx_pair(op, "WQ", WQ, w_scale, XQ);
+  TORCH_CHECK(XQ.dim() == 2 && WQ.dim() == 3, op, ": XQ must be 2-D [total_M, K / 2] and WQ 3-D [G, N, K / 2]");
+  TORCH_CHECK(XQ.size(1) == WQ.size(2), op, ": XQ and WQ must share K, got ", 2 * XQ.size(1), " vs ", 2 * WQ.size(2));
+  TORCH_CHECK(!gated || WQ.size(1) % 2 == 0, op, ": WQ must hold as many gate rows as others, got ", WQ.size(1), " rows");
+  TORCH_CHECK(M_sizes.scalar_type() == at::kLong && M_sizes.device() == XQ.device() && M_sizes.dim() == 1, op, ": M_sizes must be a 1-D int64 tensor on the device of XQ");
+  const int64_t G = WQ.size(0), M = XQ.size(0), K = 2 * XQ.size(1), N = WQ.size(1) / (gated ? 2 : 1);
+  TORCH_CHECK(M_sizes.size(0) == G && G <= INT32_MAX, op, ": M_sizes must have one entry per group (", G, "), got ", M_sizes.size(0));
+  const int code = mx_output(op, out_dtype);
+  Tensor Y = empty_on({M, N}, type_of(code), XQ);
+  if (M == 0 || N == 0 || G == 0) return Y;
+  const c10::DeviceGuard guard(XQ.device());
+  const Tensor x = fetchable(XQ), w = fetchable(WQ);
+  const auto xs = contiguous(x_scale), ws = contiguous(w_scale), sizes = contiguous(M_sizes);
+  const size_t bytes = api.mslk_amd_mxfp4_grouped_mm_workspace_bytes((int)G, M, N, K, gated, aligned16(*xs) && aligned16(*ws));
+  Tensor workspace;
+  if (bytes > 0) workspace = empty_on({(int64_t)bytes}, at::kByte, XQ);
+  check_rc(api.mslk_amd_mxfp4_grouped_mm(x.const_data_ptr(), w.const_data_ptr(), xs->const_data_ptr(), ws->const_data_ptr(), sizes->const_data_ptr<int64_t>(),
+                                         (int)G, gated, Y.mutable_data_ptr(), code, M, N, K, bytes > 0 ? workspace.mutable_data_ptr() : nullptr, bytes,
+                                         stream_of(XQ)));
+  return Y;
+}
+
 // Registered as boxed functions, one operator at a time and when the package asks for it.  A library loaded earlier may have
 // defined an operator (the package then only replaces its GPU kernel): a kernel registered with its C++ type is refused where
 // that library's own kernels take, say, Tensor by value instead of by reference, and an exception in a static initializer
@@ -782,6 +905,11 @@ const Kernel kernels[] = {
     kernel<append_kv>("mslk", "append_kv"),
     kernel<attention_decode>("mslk", "attention_decode"),
     kernel<attention_prompt>("mslk", "attention_prompt"),
+    kernel<quantize_mxfp4>("mslk", "quantize_mxfp4"),
+    kernel<dequantize_mxfp4>("mslk", "dequantize_mxfp4"),
+    kernel<mxfp4_mm>("mslk", "mxfp4_mm"),
+    kernel<mxfp4_gated_mm>("mslk", "mxfp4_gated_mm"),
+    kernel<mxfp4_grouped_mm>("mslk", "mxfp4_grouped_mm"),
 };
 
 }  // namespace
