@@ -674,7 +674,7 @@ int mslk_amd_mxfp4_mm(const void* xq, const void* wq, const void* x_scale, const
   if (gated && bias) return fail("%s: a gated product takes no bias", op);
   if (M == 0 || N == 0) return 0;
   MxProblem p{};
-  p.xq = (const uint8_t*)xq; p.wq = (const uint8_t*)wq; p.xs = (const uint8_t*)x_scale; p.ws = (const uint8_t*)w_scale;
+  p.xq = (const uint8_t*)xq; p.wq = (const uint8_t*)wq; p.xs.data = (const uint8_t*)x_scale; p.ws.data = (const uint8_t*)w_scale;
   p.bias = bias; p.bias_dtype = bias_dtype; p.y = (uint16_t*)y; p.out_f16 = y_dtype == MSLK_AMD_DTYPE_F16;
   p.M = (int)M; p.N = (int)N; p.K = (int)K; p.gated = gated != 0;
   return check_hip(launch_mx_mm(p, workspace, scales_aligned, (hipStream_t)stream), op);
@@ -695,7 +695,7 @@ int mslk_amd_mxfp4_grouped_mm(const void* xq, const void* wq, const void* x_scal
   if (total_M == 0 || N == 0 || G == 0) return 0;
   if (!m_sizes_dev) return fail("%s: null pointer", op);
   MxProblem p{};
-  p.xq = (const uint8_t*)xq; p.wq = (const uint8_t*)wq; p.xs = (const uint8_t*)x_scale; p.ws = (const uint8_t*)w_scale;
+  p.xq = (const uint8_t*)xq; p.wq = (const uint8_t*)wq; p.xs.data = (const uint8_t*)x_scale; p.ws.data = (const uint8_t*)w_scale;
   p.y = (uint16_t*)y; p.out_f16 = y_dtype == MSLK_AMD_DTYPE_F16;
   p.M = (int)total_M; p.N = (int)N; p.K = (int)K; p.gated = gated != 0; p.G = G; p.m_sizes = m_sizes_dev;
   return check_hip(launch_mx_mm(p, workspace, scales_aligned, (hipStream_t)stream), op);

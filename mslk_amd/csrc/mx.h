@@ -18,25 +18,33 @@ hipError_t launch_quantize_mxfp4(const void* a, int dtype, int64_t rows, int64_t
 // out [rows, K] of the same dtype codes, everything contiguous.
 hipError_t launch_dequantize_mxfp4(const void* codes, const void* scales, int64_t rows, int64_t K, void* out, int dtype, hipStream_t s);
 
+// Where scales lie: those of row r, blocks 16 p ... 16 p + 15 are the 16 bytes at data + (r / 64) * block + (r % 64) * row + p * pair_stride,
+// all multiples of 16.  A tensor's own: row = K / 32, block = 64 row, pair_stride = 16.  Arranged: [rows / 64][pairs][64][16], blocks beyond K 0.
+struct MxScales {
+  const uint8_t* data;
+  int64_t block;
+  int row, pair_stride;
+};
+
 // Y[m, n] = sum_k X[m, k] W[n, k] + bias[n]; gated: W has 2 N rows, gate rows first, and Y = silu(X Wg^T) * (X Wu^T).
 // Groups (m_sizes != nullptr): W [G, rows of W, K]; the rows of X are those of group 0, of group 1, ...
 struct MxProblem {
   const uint8_t *xq, *wq;          // codes, rows of K / 2 bytes
-  const uint8_t *xs, *ws;          // scales, rows of scale_pitch bytes
+  MxScales xs, ws;
   const void* bias;
   uint16_t* y;
   float* part;                     // sums of K slices [slices][M][N], nullptr without
   const int64_t* m_sizes;
   int M, N, K;                     // N: columns of Y
-  int x_pitch, w_pitch;            // bytes between the rows of xs, ws: multiples of 16
   int G;
   int bias_dtype;                  // 0 none, 1 fp32, 2 bf16
   int out_f16;
   int gated;
   int slices;
 };
-// Bytes of workspace that launch_mx_mm() wants for this problem (only sizes are looked at, and whether the scales are aligned).
+// Bytes of workspace that launch_mx_mm() wants for this problem (scales_aligned: both tensors of scales begin on 16 bytes).
 size_t mx_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated, int G, bool grouped, bool scales_aligned);
+// p.xs.data and p.ws.data: the tensors; the rest of p.xs and p.ws is filled in.
 hipError_t launch_mx_mm(MxProblem p, void* workspace, bool scales_aligned, hipStream_t s);
 
 }  // namespace mslk_amd

@@ -2,22 +2,25 @@
 //
 // One workgroup (a WM x WN grid of wavefronts) makes a BM x BN tile of sums.
 //
-// Steps.  K is consumed 256 values (128 bytes of a row) at a time, copied global -> LDS by the 128-bit DMA load (gemm_tile.h) into a
-// ring of NS stages.  Eight 16-byte chunks make a row of 128 bytes in LDS, one chunk being one block of 32 values; they are permuted
-// by swz_x() / swz_w() so that the lanes which are served together touch different banks, and since the DMA cannot scatter inside a
-// wave the permutation is applied to the global side.
-// Scales.  A row's scales of two steps are 16 bytes.  They travel by the same DMA, every second step, into a ring of their own, 16
-// bytes per row.  (Loaded into registers instead, the compiler's wait for them would be one for the DMA loads too, which it does
-// not know of; and a lane's load would touch a line per row.)
+// Steps.  K is consumed 256 values (128 bytes of a row) at a time, copied global -> LDS by the 128-bit DMA load (gemm_tile.h).  Eight
+// 16-byte chunks make a row of 128 bytes in LDS, one chunk being one block of 32 values; they are permuted by chunk ^ swz(row), so that
+// the lanes which are served together touch different banks, and since the DMA cannot scatter inside a wave the permutation is applied to
+// the global side.
+// Scales.  A row's scales of two steps, a pair, are 16 bytes.  They travel by the same DMA into a ring of their own, 16 bytes per row.
+// (Loaded into registers instead, the compiler's wait for them would be one for the DMA loads too, which it does not know of.)  As
+// they lie in the tensor, each row's 16 bytes are a line for the L1 and the L2 to look up, and a pair of a 256 x 256 tile 512 lines next to
+// 1024 of codes: 0.28 of 1.94 us per step.  So large products have them arranged first, 64 rows to a KiB (MxScales).
+// K's end.  Of a last step of fewer than eight blocks the missing chunks are filled with chunk 0, and their scales are 0, 2^-127, in rows
+// that the caller has padded: products of two such blocks are below 2^-243 and vanish in fp32.
 // Products.  v_mfma_scale_f32_32x32x64_f8f6f4, W first: lane (i = l & 31, h = l >> 5) gives row i's chunk 4 h + j to product j of a
 // step, and the four bytes of its scales of the step are those of chunks 4 h ... 4 h + 3: the instruction picks byte j.  Any order of
 // K would do that both operands share; this one needs neither shifts nor shuffles of scales.  Out of registers and on quantized normal
 // numbers these run at 6.66 PFLOP/s, 16x16x128 at 5.96 (on zeros 9.89 and 6.63: the limit on numbers is power).
-// Rows of W in a fragment.  A lane receives, of 32 rows of the fragment, rows 8 q + 4 h + r (q, r = 0 ... 3).  Fragment 2 T + t of a
-// wave reads LDS rows 64 T + 16 q + 8 h + 4 t + r, so that the two fragments of a pair give a lane eight neighbouring rows: 16 bytes
-// of a row of Y, stored as they are.
-// GATED: a tile has BN / 2 columns; its LDS rows with t = 0 are filled from the gate's rows of W, those with t = 1 from the rows N
-// further, so a lane holds both factors of its columns.
+// Rows.  LDS row f 32 W + w 32 + i of an operand is row i of fragment f of wave row (column) w, W of them.  Of 32 rows of W a lane receives
+// rows 8 q + 4 h + r (q, r = 0 ... 3); fragment 2 T + t takes columns 64 T + 16 q + 8 h + 4 t + r of the wave's, so that a pair of fragments
+// gives a lane eight neighbouring columns: 16 bytes of a row of Y, stored as they are.
+// GATED: a tile has BN / 2 columns; fragments with t = 0 are rows of the gate, those with t = 1 the rows N further, of columns
+// 32 T + 16 h + 4 q + r, so a lane holds both factors of its columns.
 #pragma once
 #include <type_traits>
 
@@ -27,7 +30,6 @@
 namespace mslk_amd {
 
 constexpr int kMxStep = 128;          // bytes of a row per step
-constexpr int kMxStepValues = 256;
 
 // NS stages: NS - 1 steps are in flight while one is multiplied.
 template <int BM_, int BN_, int WM_, int WN_, int NS_>
@@ -40,6 +42,7 @@ struct MxShape {
   // scales of two steps: DMA loads per wave (the rows of X, then of W, 64 rows a load; the last ones may have none)
   static constexpr int LS = ((BM + BN) / 64 + NW - 1) / NW;
   static constexpr int S_BYTES = LS * NW * 1024;
+  static_assert(LS <= 2, "copy_scales()");
   // A pair's place is taken again by the pair S_STAGES further, NS - 1 steps before that begins and after the last step of this one.
   static constexpr int S_STAGES = (NS + 2) / 2;
   static constexpr int LDS_BYTES = NS * (X_BYTES + W_BYTES) + S_STAGES * S_BYTES;
@@ -47,18 +50,31 @@ struct MxShape {
   static_assert(LDS_BYTES <= 160 * 1024, "LDS of a CU");
 };
 
+// Scales of a tile: row r of it is row `first` + r behind `base`, which is the first of 64.
+struct MxTileScales {
+  const uint8_t* base;
+  uint32_t block, row, first;   // bytes of 64 rows, of one
+  int pair_stride;
+  MSLK_AMD_DEVINL MxTileScales() = default;
+  MSLK_AMD_DEVINL MxTileScales(const MxScales& s, int64_t first_row)
+      : base(s.data + (first_row >> 6) * s.block), block((uint32_t)s.block), row(s.row), first((uint32_t)first_row & 63), pair_stride(s.pair_stride) {}
+  MSLK_AMD_DEVINL uint32_t offset(int r) const {   // of the 16 bytes for steps 0 and 1
+    const uint32_t at = first + (uint32_t)r;
+    return (at >> 6) * block + (at & 63) * row;
+  }
+};
+
 // What a tile reads: first rows of its operands, valid rows (>= 1), steps [0, steps) of which the last has `last_chunks` blocks.
 struct MxOperands {
-  const uint8_t *x, *w, *xs, *ws;
+  const uint8_t *x, *w;
+  MxTileScales xs, ws;
   int rows_x, rows_w;       // rows_w: of the gate's rows, if gated
   uint32_t ld;              // bytes between rows of x and of w
-  int x_pitch, w_pitch;     // between rows of scales
-  uint32_t up, up_scale;    // gated: bytes from a gate's row of codes / scales to its partner
+  uint32_t up, up_rows;     // gated: bytes (rows) from a gate's row to its partner
   int steps, last_chunks;
 };
 
-MSLK_AMD_DEVINL int swz_x(int row) { return (row >> 1) & 7; }
-MSLK_AMD_DEVINL int swz_w(int row) { return ((row >> 1) & 1) | (((row >> 3) & 3) << 1); }
+MSLK_AMD_DEVINL int mx_swz(int row) { return (row >> 1) & 7; }
 
 MSLK_AMD_DEVINL v8i mx_operand(v4i a) { return v8i{a[0], a[1], a[2], a[3], 0, 0, 0, 0}; }
 
@@ -66,48 +82,52 @@ template <typename TS, bool GATED>
 struct MxTile {
   uint32_t x_off[TS::LX], w_off[TS::LW];   // of this lane's chunk of a load, step 0
   uint32_t s_off[TS::LS];                  // of this lane's 16 bytes of scales, relative to xs or ws
-  bool s_is_w[TS::LS];                     // which of the two (the same in every lane of a wave)
   MxOperands o;
 
   MSLK_AMD_DEVINL static int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
-  // Row of W (of the tile's) that LDS row r holds, and whether it is one of the second half.
+  // Row of the tile that LDS row r of X holds.
+  MSLK_AMD_DEVINL static int x_row(int r) { return ((r >> 5) % TS::WM) * (TS::BM / TS::WM) + r / (32 * TS::WM) * 32 + (r & 31); }
+  // Row of W (of the tile's) that LDS row r of W holds, and whether it is one of the second half.
   MSLK_AMD_DEVINL static int w_row(int r, bool& up) {
-    up = false;
-    if constexpr (!GATED) return r;
-    up = (r >> 2) & 1;
-    // within a wave's 64 rows: q, h, r as above; column 16 h + 4 q + r, so that a lane's columns of a pair are neighbours
-    return (r >> 6) * 32 + ((r >> 3) & 1) * 16 + ((r >> 4) & 3) * 4 + (r & 3);
+    const int wn = (r >> 5) % TS::WN, tn = r / (32 * TS::WN), i = r & 31;
+    up = GATED && (tn & 1) != 0;
+    if constexpr (GATED) return wn * (TS::BN / TS::WN / 2) + (tn >> 1) * 32 + ((i >> 2) & 1) * 16 + (i >> 3) * 4 + (i & 3);
+    else return wn * (TS::BN / TS::WN) + (tn >> 1) * 64 + (tn & 1) * 4 + (i >> 2) * 8 + (i & 3);
   }
+  // First of the 8 LDS rows that load q of this wave fills.
+  MSLK_AMD_DEVINL static int x_load_row(int q) { return (wave_id() * TS::LX + q) * 8; }
+  MSLK_AMD_DEVINL static int w_load_row(int q) { return (wave_id() * TS::LW + q) * 8; }
 
   MSLK_AMD_DEVINL void init(const MxOperands& operands) {
     o = operands;
     o.x = uniform_ptr(o.x);
     o.w = uniform_ptr(o.w);
-    o.xs = uniform_ptr(o.xs);
-    o.ws = uniform_ptr(o.ws);
+    o.xs.base = uniform_ptr(o.xs.base);
+    o.ws.base = uniform_ptr(o.ws.base);
     const int lane = threadIdx.x & 63, wave = wave_id();
 #pragma unroll
-    for (int i = 0; i < TS::LX; ++i) {   // rows beyond the valid ones read the last valid one again: their sums are not stored
-      const int r = (wave * TS::LX + i) * 8 + (lane >> 3);
-      x_off[i] = (uint32_t)min(r, o.rows_x - 1) * o.ld + (((lane & 7) ^ swz_x(r)) << 4);
+    for (int q = 0; q < TS::LX; ++q) {   // rows beyond the valid ones read the last valid one again: their sums are not stored
+      const int r = x_load_row(q) + (lane >> 3);
+      x_off[q] = (uint32_t)min(x_row(r), o.rows_x - 1) * o.ld + (((lane & 7) ^ mx_swz(r)) << 4);
     }
 #pragma unroll
-    for (int i = 0; i < TS::LW; ++i) {
-      const int r = (wave * TS::LW + i) * 8 + (lane >> 3);
+    for (int q = 0; q < TS::LW; ++q) {
+      const int r = w_load_row(q) + (lane >> 3);
       bool up;
       const int row = min(w_row(r, up), o.rows_w - 1);
-      w_off[i] = (uint32_t)row * o.ld + (up ? o.up : 0u) + (((lane & 7) ^ swz_w(r)) << 4);
+      w_off[q] = (uint32_t)row * o.ld + (up ? o.up : 0u) + (((lane & 7) ^ mx_swz(r)) << 4);
     }
 #pragma unroll
-    for (int i = 0; i < TS::LS; ++i) {
-      const int first = (wave * TS::LS + i) * 64;   // in the list of rows of X, then of W
-      const int r = min(first + lane, TS::BM + TS::BN - 1);
-      // (with BM = 32 the first load has rows of both: s_is_w is then that of the lane)
-      s_is_w[i] = r >= TS::BM;
-      bool up;
-      const int row = s_is_w[i] ? min(w_row(r - TS::BM, up), o.rows_w - 1) : min(r, o.rows_x - 1);
-      s_off[i] = s_is_w[i] ? (uint32_t)row * (uint32_t)o.w_pitch + (up ? o.up_scale : 0u) : (uint32_t)row * (uint32_t)o.x_pitch;
+    for (int i = 0; i < TS::LS; ++i) {   // the list of LDS rows of X, then of W
+      const int r = min((wave * TS::LS + i) * 64 + lane, TS::BM + TS::BN - 1);
+      bool up = false;
+      if (r >= TS::BM) {
+        const int row = min(w_row(r - TS::BM, up), o.rows_w - 1);
+        s_off[i] = o.ws.offset(row + (up ? (int)o.up_rows : 0));
+      } else {
+        s_off[i] = o.xs.offset(min(x_row(r), o.rows_x - 1));
+      }
     }
   }
 
@@ -115,42 +135,25 @@ struct MxTile {
   MSLK_AMD_DEVINL static char* w_stage(char* lds, int i) { return lds + TS::NS * TS::X_BYTES + i * TS::W_BYTES; }
   MSLK_AMD_DEVINL static char* s_stage(char* lds, int i) { return lds + TS::NS * (TS::X_BYTES + TS::W_BYTES) + i * TS::S_BYTES; }
 
-  // The loads of step kt into stage `at`; of the scales, too, where a pair of steps begins.
-  MSLK_AMD_DEVINL void issue(char* lds, int kt, int at) {
-    const int lane = threadIdx.x & 63, wave = wave_id();
-    if ((kt & 1) == 0) {
-      char* dst = s_stage(lds, (kt >> 1) % TS::S_STAGES);
-#pragma unroll
-      for (int i = 0; i < TS::LS; ++i) {
-        if constexpr (TS::BM % 64 == 0) {
-          dma16((__builtin_amdgcn_readfirstlane((int)s_is_w[i]) ? o.ws : o.xs) + (kt >> 1) * 16, s_off[i], dst + (wave * TS::LS + i) * 1024);
-        } else {   // one base for lanes of both: the 64-bit difference does not fit the offset, so two loads share the instruction slot
-          if (s_is_w[i]) dma16(o.ws + (kt >> 1) * 16, s_off[i], dst + (wave * TS::LS + i) * 1024);
-          else dma16(o.xs + (kt >> 1) * 16, s_off[i], dst + (wave * TS::LS + i) * 1024);
-        }
-      }
-    }
-    const uint8_t *x = o.x + (int64_t)kt * kMxStep, *w = o.w + (int64_t)kt * kMxStep;
-    char *xd = x_stage(lds, at) + wave * TS::LX * 1024, *wd = w_stage(lds, at) + wave * TS::LW * 1024;
-    const bool whole = kt + 1 < o.steps || o.last_chunks == 8;
-    if (whole) {
-#pragma unroll
-      for (int i = 0; i < TS::LX; ++i) dma16(x, x_off[i], xd + i * 1024);
-#pragma unroll
-      for (int i = 0; i < TS::LW; ++i) dma16(w, w_off[i], wd + i * 1024);
-    } else {   // the last blocks of the rows: chunks behind them become zeros.  (Each load has lanes with chunk 0, so each is issued.)
-#pragma unroll
-      for (int i = 0; i < TS::LX; ++i) {
-        const int r = (wave * TS::LX + i) * 8 + (lane >> 3);
-        if (((lane & 7) ^ swz_x(r)) < o.last_chunks) dma16(x, x_off[i], xd + i * 1024);
-        else *reinterpret_cast<uint4*>(xd + i * 1024 + lane * 16) = make_uint4(0, 0, 0, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < TS::LW; ++i) {
-        const int r = (wave * TS::LW + i) * 8 + (lane >> 3);
-        if (((lane & 7) ^ swz_w(r)) < o.last_chunks) dma16(w, w_off[i], wd + i * 1024);
-        else *reinterpret_cast<uint4*>(wd + i * 1024 + lane * 16) = make_uint4(0, 0, 0, 0);
-      }
+  // What is added to the offsets of a step's loads: 0, but in a last step of fewer blocks lanes of missing chunks go back to chunk 0.
+  // Loads of even and of odd number differ: swz() of their rows does, in bit 2.
+  struct Adjust { uint32_t even, odd; };
+  MSLK_AMD_DEVINL Adjust adjust(int kt) const {
+    const int lane = threadIdx.x & 63, c = (lane & 7) ^ (lane >> 4);
+    const int chunks = kt + 1 < o.steps ? 8 : o.last_chunks;
+    return Adjust{c < chunks ? 0u : (uint32_t)(-16 * c), (c ^ 4) < chunks ? 0u : (uint32_t)(-16 * (c ^ 4))};
+  }
+  // Load i of the scales of steps 2 pair and 2 pair + 1 into the place of `pair`; behind the last pair, the last one's again.
+  MSLK_AMD_DEVINL void copy_scales(char* lds, int pair, int i) {
+    const int64_t from = (int64_t)min(pair, (o.steps - 1) >> 1) * o.xs.pair_stride;   // (the same for both)
+    const int wave = wave_id();
+    const uint32_t off = TS::LS == 1 || i == 0 ? s_off[0] : s_off[TS::LS - 1];   // (an index that is no constant would put the array in memory)
+    char* dst = s_stage(lds, pair % TS::S_STAGES) + (wave * TS::LS + i) * 1024;
+    if constexpr (TS::BM % 64 == 0) {
+      dma16(uniform_ptr(((wave * TS::LS + i) * 64 >= TS::BM ? o.ws.base : o.xs.base) + from), off, dst);
+    } else {   // rows of both operands in one load: one for each
+      if ((wave * TS::LS + i) * 64 + (int)(threadIdx.x & 63) >= TS::BM) dma16(o.ws.base + from, off, dst);
+      else dma16(o.xs.base + from, off, dst);
     }
   }
 
@@ -166,29 +169,58 @@ struct MxTile {
     __builtin_amdgcn_sched_barrier(0);
   }
 
-  template <int J, int FM>
-  MSLK_AMD_DEVINL static void multiply(const v4i& wf, const v4i (&xf)[FM], uint32_t sw, const uint32_t (&sx)[FM], v16f (&acc)[FM]) {
-#pragma unroll
-    for (int tm = 0; tm < FM; ++tm)
-      acc[tm] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(wf), mx_operand(xf[tm]), acc[tm], 4, 4, J, (int)sw, J, (int)sx[tm]);
+  // Chunk 4 h + j of this lane's row of a fragment of 32 W rows at `rows`; w: of the W waves that share it, this one.
+  MSLK_AMD_DEVINL static v4i chunk(const char* rows, int w, int j) {
+    const int lane = threadIdx.x & 63, i = lane & 31;
+    return *reinterpret_cast<const v4i*>(rows + (w * 32 + i) * kMxStep + (((4 * (lane >> 5) + j) ^ mx_swz(i)) << 4));
   }
-
-  // LDS row of W that lane i of fragment tn of this wave holds
-  MSLK_AMD_DEVINL static int frag_row_w(int wn, int tn, int i) {
-    return wn * (TS::BN / TS::WN) + (tn >> 1) * 64 + (tn & 1) * 4 + (i & 3) + (i >> 2) * 8;
+  MSLK_AMD_DEVINL static v4i x_chunk(const char* stage, int tm, int j) { return chunk(stage + tm * (32 * TS::WM * kMxStep), wave_id() / TS::WN, j); }
+  MSLK_AMD_DEVINL static v4i w_chunk(const char* stage, int tn, int j) { return chunk(stage + tn * (32 * TS::WN * kMxStep), wave_id() % TS::WN, j); }
+  MSLK_AMD_DEVINL static void load_scales(char* lds, int kt, uint32_t (&sx)[TS::FM], uint32_t (&sw)[TS::FN]) {
+    const int lane = threadIdx.x & 63, wave = wave_id();
+    const char* at = s_stage(lds, (kt >> 1) % TS::S_STAGES) + (kt & 1) * 8 + (lane >> 5) * 4 + (lane & 31) * 16;
+#pragma unroll
+    for (int tm = 0; tm < TS::FM; ++tm) sx[tm] = *reinterpret_cast<const uint32_t*>(at + (tm * TS::WM + wave / TS::WN) * 512);
+#pragma unroll
+    for (int tn = 0; tn < TS::FN; ++tn) sw[tn] = *reinterpret_cast<const uint32_t*>(at + TS::BM * 16 + (tn * TS::WN + wave % TS::WN) * 512);
+  }
+  template <int J>
+  MSLK_AMD_DEVINL static void multiply(const v4i& wf, const v4i& xf, uint32_t sw, uint32_t sx, v16f& acc) {
+    acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(wf), mx_operand(xf), acc, 4, 4, J, (int)sw, J, (int)sx);
   }
 
   // acc = the tile's sums.  Ends with a barrier: LDS is free.
   MSLK_AMD_DEVINL void run(char* lds, v16f (&acc)[TS::FN][TS::FM]) {
-    const int lane = threadIdx.x & 63, wave = wave_id();
-    const int wm = wave / TS::WN, wn = wave % TS::WN;
-    const int i = lane & 31, h = lane >> 5;
 #pragma unroll
     for (int tn = 0; tn < TS::FN; ++tn)
 #pragma unroll
       for (int tm = 0; tm < TS::FM; ++tm)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[tn][tm][r] = 0.f;
+    run_ring(lds, acc);
+    wait_and_barrier<0>();
+  }
+
+  // The loads of step kt into stage `at`, in front of them those of a pair's scales.
+  MSLK_AMD_DEVINL void issue(char* lds, int kt, int at) {
+    if ((kt & 1) == 0) {
+#pragma unroll
+      for (int i = 0; i < TS::LS; ++i) copy_scales(lds, kt >> 1, i);
+    }
+    const Adjust a = adjust(kt);
+    const uint8_t *x = o.x + (int64_t)kt * kMxStep, *w = o.w + (int64_t)kt * kMxStep;
+#pragma unroll
+    for (int q = 0; q < TS::LX; ++q) {
+      const int r = x_load_row(q);
+      dma16(x, x_off[q] + ((r >> 3) & 1 ? a.odd : a.even), x_stage(lds, at) + r * kMxStep);
+    }
+#pragma unroll
+    for (int q = 0; q < TS::LW; ++q) {
+      const int r = w_load_row(q);
+      dma16(w, w_off[q] + ((r >> 3) & 1 ? a.odd : a.even), w_stage(lds, at) + r * kMxStep);
+    }
+  }
+  MSLK_AMD_DEVINL void run_ring(char* lds, v16f (&acc)[TS::FN][TS::FM]) {
     constexpr int D = TS::NS - 1, PER = TS::LX + TS::LW;
     // In flight behind the loads of a step when its turn comes: those of the D - 1 steps after it, and of the scales of at least
     // (D - 1) / 2 pairs (a pair's scales go in front of its first step's codes).
@@ -200,26 +232,19 @@ struct MxTile {
       else wait_and_barrier<0>();
       // the stage of step kt - 1, which everybody has left, takes step kt + D
       if (kt + D < o.steps) issue(lds, kt + D, at == 0 ? TS::NS - 1 : at - 1);
-      const char *xb = x_stage(lds, at), *wb = w_stage(lds, at), *sb = s_stage(lds, (kt >> 1) % TS::S_STAGES) + (kt & 1) * 8 + h * 4;
+      const char *x = x_stage(lds, at), *w = w_stage(lds, at);
       uint32_t sx[TS::FM], sw[TS::FN];
-#pragma unroll
-      for (int tm = 0; tm < TS::FM; ++tm)
-        sx[tm] = *reinterpret_cast<const uint32_t*>(sb + (wm * (TS::BM / TS::WM) + tm * 32 + i) * 16);
-#pragma unroll
-      for (int tn = 0; tn < TS::FN; ++tn) sw[tn] = *reinterpret_cast<const uint32_t*>(sb + (TS::BM + frag_row_w(wn, tn, i)) * 16);
+      load_scales(lds, kt, sx, sw);
       auto product = [&](auto j) {
         constexpr int J = decltype(j)::value;
         v4i xf[TS::FM];
 #pragma unroll
-        for (int tm = 0; tm < TS::FM; ++tm) {
-          const int r = wm * (TS::BM / TS::WM) + tm * 32 + i;
-          xf[tm] = *reinterpret_cast<const v4i*>(xb + r * kMxStep + (((4 * h + J) ^ swz_x(r)) << 4));
-        }
+        for (int tm = 0; tm < TS::FM; ++tm) xf[tm] = x_chunk(x, tm, J);
 #pragma unroll
         for (int tn = 0; tn < TS::FN; ++tn) {
-          const int r = frag_row_w(wn, tn, i);
-          const v4i wf = *reinterpret_cast<const v4i*>(wb + r * kMxStep + (((4 * h + J) ^ swz_w(r)) << 4));
-          multiply<J, TS::FM>(wf, xf, sw[tn], sx, acc[tn]);
+          const v4i wf = w_chunk(w, tn, J);
+#pragma unroll
+          for (int tm = 0; tm < TS::FM; ++tm) multiply<J>(wf, xf[tm], sw[tn], sx[tm], acc[tn][tm]);
         }
       };
       product(std::integral_constant<int, 0>{});
@@ -228,7 +253,6 @@ struct MxTile {
       product(std::integral_constant<int, 3>{});
       at = at + 1 == TS::NS ? 0 : at + 1;
     }
-    wait_and_barrier<0>();
   }
 };
 
