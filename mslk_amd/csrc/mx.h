@@ -45,6 +45,7 @@ struct MxProblem {
 // Bytes of workspace that launch_mx_mm() wants for this problem (scales_aligned: both tensors of scales begin on 16 bytes).
 size_t mx_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated, int G, bool grouped, bool scales_aligned);
 // p.xs.data and p.ws.data: the tensors; the rest of p.xs and p.ws is filled in.
+hipError_t launch_mx_stream(const MxProblem& p, hipStream_t s);   // of it, few rows of X (mx_stream.hip): tensors of scales as they are
 hipError_t launch_mx_mm(MxProblem p, void* workspace, bool scales_aligned, hipStream_t s);
 
 }  // namespace mslk_amd

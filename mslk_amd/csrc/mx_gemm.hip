@@ -1,16 +1,10 @@
 // Products of MXFP4 matrices for gfx950: dense, with a gated activation, and for groups of rows (formats: mx.h, tile: mx_tile.h).
 #include "kernels.h"
+#include "mx_device.h"
 #include "mx_tile_large.h"
 
 namespace mslk_amd {
 namespace {
-
-constexpr int kXcds = 8;
-constexpr int kPanel = 4;   // row tiles that share the weights of a panel in an XCD's L2
-
-// y = silu(gate) * up in fp32.  For gates below -88 exp(-gate) is infinite and the result -0, as it should be; the exponential and the
-// reciprocal are good to about 2 units of fp32, far below the rounding to 16 bits that follows.
-MSLK_AMD_DEVINL float gated_value(float gate, float up) { return gate * __builtin_amdgcn_rcpf(1.f + __expf(-gate)) * up; }
 
 // Eight columns n ... n + 7 of a row's bias, as fp32; `whole`: they exist and lie on 16 bytes.
 template <int BIAS>
@@ -141,83 +135,6 @@ MSLK_AMD_DEVINL void store_tile(const MxProblem& p, const v16f (&acc)[TS::FN][TS
       else store_tile<TS, false, 2, false>(p, acc, m0, rows, n0);
     }
   }
-}
-
-// Entry t of the tiles of `tiles_m` x `tiles_n`: panels of up to kPanel row tiles, column by column.
-MSLK_AMD_DEVINL void tile_at(int t, int tiles_m, int tiles_n, int& tm, int& tn) {
-  const int panel = kPanel * tiles_n, first = (t / panel) * kPanel;
-  const int rows = min(tiles_m - first, kPanel);
-  tm = __builtin_amdgcn_readfirstlane(first + (t % panel) % rows);
-  tn = __builtin_amdgcn_readfirstlane((t % panel) / rows);
-}
-
-// Workgroup ids are dealt to the XCDs in turn: XCD x takes a run of neighbouring entries of the list.
-MSLK_AMD_DEVINL int entry_of(int wg, int total) {
-  const int per_xcd = (total + kXcds - 1) / kXcds, t = (wg % kXcds) * per_xcd + wg / kXcds;
-  return wg / kXcds < per_xcd && t < total ? t : -1;
-}
-
-// Group and tile of entry t among the row tiles of all groups (R_g = ceil(size / BM) each) times tiles_n.  Returns false behind the
-// last one.  Every lane takes part.
-struct GroupTile { int g, row0, rows, tm, tn; };
-template <int BM>
-MSLK_AMD_DEVINL bool find_group_tile(const MxProblem& p, int tiles_n, int wg, GroupTile& out) {
-  const int lane = threadIdx.x & 63;
-  auto size_at = [&](int g) { return g < p.G ? (int)max((int64_t)0, min(p.m_sizes[g], (int64_t)p.M)) : 0; };
-  // all row tiles (rows beyond M do not exist, whatever the sizes say)
-  int tiles = 0;
-  int64_t rows_before = 0;
-  for (int g0 = 0; g0 < p.G; g0 += 64) {
-    int64_t end = size_at(g0 + lane);
-    const int mine = (int)end;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int64_t up = __shfl_up(end, d, 64);
-      if (lane >= d) end += up;
-    }
-    const int64_t start = rows_before + end - mine;
-    int r = (int)max((int64_t)0, min((int64_t)mine, p.M - start));
-    r = (r + BM - 1) / BM;
-#pragma unroll
-    for (int d = 32; d > 0; d /= 2) r += __shfl_xor(r, d, 64);
-    tiles += r;
-    rows_before += __shfl(end, 63, 64);
-  }
-  const int t = entry_of(wg, tiles * tiles_n);
-  if (t < 0) return false;
-  int before = 0;
-  rows_before = 0;
-  for (int g0 = 0; g0 < p.G; g0 += 64) {
-    int64_t end = size_at(g0 + lane);
-    const int mine = (int)end;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int64_t up = __shfl_up(end, d, 64);
-      if (lane >= d) end += up;
-    }
-    const int64_t start = rows_before + end - mine;
-    const int live = (int)max((int64_t)0, min((int64_t)mine, p.M - start));
-    int last = (live + BM - 1) / BM * tiles_n;   // entries up to and with this group's
-    const int own = last;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int up = __shfl_up(last, d, 64);
-      if (lane >= d) last += up;
-    }
-    const uint64_t holds = __ballot(t >= before + last - own && t < before + last);
-    if (holds != 0) {
-      const int src = __ffsll((unsigned long long)holds) - 1;
-      out.g = __builtin_amdgcn_readfirstlane(g0 + src);
-      const int row0 = __shfl((int)start, src, 64), size = __shfl(live, src, 64), at = t - (before + __shfl(last - own, src, 64));
-      tile_at(at, (size + BM - 1) / BM, tiles_n, out.tm, out.tn);
-      out.row0 = __builtin_amdgcn_readfirstlane(row0) + out.tm * BM;
-      out.rows = min(__builtin_amdgcn_readfirstlane(size) - out.tm * BM, BM);
-      return true;
-    }
-    before += __shfl(last, 63, 64);
-    rows_before += __shfl(end, 63, 64);
-  }
-  return false;
 }
 
 // Operands of the tile of rows m0 ..., columns n0 ...; w_row: first row of W's group.
@@ -365,19 +282,23 @@ hipError_t launch(const MxProblem& p, hipStream_t s) {
   return p.gated ? launch<TS, true, false>(p, s) : launch<TS, false, false>(p, s);
 }
 
-// Whether the 256 x 256 tiles take the problem (at least two steps).
-bool takes_large(int64_t M, int64_t K) { return M > 64 && K > 256; }
+// Few rows: the weights are streamed (mx_stream.hip).
+constexpr int kStreamTiles = 384;
+bool takes_stream(int64_t M, int64_t N, int gated, bool grouped) { return !grouped && M <= 64 && N * (gated ? 2 : 1) <= 32 * kStreamTiles; }
+// Whether the 256 x 256 tiles take the others (at least two steps).
+bool takes_large(int64_t K) { return K > 256; }
 
 }  // namespace
 
 size_t mx_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated, int G, bool grouped, bool scales_aligned) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  if (K % 512 == 0 && scales_aligned && !takes_large(M, K)) return 0;
+  if (takes_stream(M, N, gated, grouped) || (K % 512 == 0 && scales_aligned && !(takes_large(K) && M > 64))) return 0;
   return (size_t)(arranged_bytes(M, K) + arranged_bytes(N * (gated ? 2 : 1) * (grouped ? G : 1), K));
 }
 
 hipError_t launch_mx_mm(MxProblem p, void* workspace, bool scales_aligned, hipStream_t s) {
-  const bool large = takes_large(p.M, p.K);
+  if (takes_stream(p.M, p.N, p.gated, p.m_sizes != nullptr)) return launch_mx_stream(p, s);
+  const bool large = takes_large(p.K) && p.M > 64;
   const int from = p.K / kMxBlock, pairs = (int)pairs_of(p.K);
   if (p.K > 0 && (large || p.K % 512 != 0 || !scales_aligned)) {
     const int64_t rows_w = (int64_t)p.N * (p.gated ? 2 : 1) * (p.m_sizes != nullptr ? p.G : 1);

@@ -40,7 +40,7 @@ struct MxShape {
   static constexpr int X_BYTES = BM * kMxStep, W_BYTES = BN * kMxStep;
   static constexpr int LX = BM / 8 / NW, LW = BN / 8 / NW;          // DMA loads per wave and step
   // scales of two steps: DMA loads per wave (the rows of X, then of W, 64 rows a load; the last ones may have none)
-  static constexpr int LS = ((BM + BN) / 64 + NW - 1) / NW;
+  static constexpr int LS = ((BM + BN + 63) / 64 + NW - 1) / NW;
   static constexpr int S_BYTES = LS * NW * 1024;
   static_assert(LS <= 2, "copy_scales()");
   // A pair's place is taken again by the pair S_STAGES further, NS - 1 steps before that begins and after the last step of this one.
