@@ -33,14 +33,14 @@ struct MxProblem {
   MxScales xs, ws;
   const void* bias;
   uint16_t* y;
-  float* part;                     // sums of K slices [slices][M][N], nullptr without
   const int64_t* m_sizes;
+  const void* row_tiles;           // list of the groups' row tiles in device memory, nullptr without
+  int tile_rows;
   int M, N, K;                     // N: columns of Y
   int G;
   int bias_dtype;                  // 0 none, 1 fp32, 2 bf16
   int out_f16;
   int gated;
-  int slices;
 };
 // Bytes of workspace that launch_mx_mm() wants for this problem (scales_aligned: both tensors of scales begin on 16 bytes).
 size_t mx_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated, int G, bool grouped, bool scales_aligned);

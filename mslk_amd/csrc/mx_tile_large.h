@@ -12,6 +12,9 @@
 // barrier, fragments 2 and 3 (places that this step has left) and X (the stage that this step has left).  At the barrier the loads of
 // groups 1 and 2 may be in flight.  The last two steps of a tile issue the first two of the next one.
 //
+// Rows.  LDS row r of X is row r of the tile: fragment t of a wave's four is 32 of rows 64 t ... 64 t + 63.  A tile of at most 64 or 128 rows
+// (the last one of an operand or of a group; small operands are cut into such) takes a loop over one or two fragments.
+//
 // No branch is taken inside a step: the compiler moves products, which touch no memory, behind one, and away from the loads and reads
 // that they are to be issued between.
 #pragma once
@@ -38,8 +41,8 @@ struct MxLargeTile {
 
   MSLK_AMD_DEVINL static int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
-  // A load covers 8 LDS rows, or the 16 bytes of scales of 64 rows.  Wave v makes loads 8 v ... 8 v + 7 of X, loads 2 v and 2 v + 1 of each
-  // fragment of W, and 2 v and 2 v + 1 of the scales (of X, then of W).
+  // A load covers 8 LDS rows, or the 16 bytes of scales of 64 rows.  The loads of X are dealt to the waves in turn; wave v makes loads
+  // 2 v and 2 v + 1 of each fragment of W, and 2 v and 2 v + 1 of the scales (of X, then of W).
   MSLK_AMD_DEVINL void init(const MxOperands& o) {
     int lane = threadIdx.x & 63;
     asm volatile("" : "+v"(lane));   // formed again for each tile, not kept
@@ -49,8 +52,8 @@ struct MxLargeTile {
     bool up;
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
-      const int r = (wave * 8 + q) * 8 + (lane >> 3);
-      x_off[q] = (uint32_t)min(Rows::x_row(r), o.rows_x - 1) * o.ld + (((lane & 7) ^ mx_swz(r)) << 4);
+      const int r = (q * 4 + wave) * 8 + (lane >> 3);
+      x_off[q] = (uint32_t)min(r, o.rows_x - 1) * o.ld + (((lane & 7) ^ mx_swz(r)) << 4);
     }
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
@@ -63,7 +66,7 @@ struct MxLargeTile {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = ((wave & 1) * 2 + i) * 64 + lane;
-      const uint32_t sx = o.xs.offset(min(Rows::x_row(r), o.rows_x - 1));
+      const uint32_t sx = o.xs.offset(min(r, o.rows_x - 1));
       const int row = min(Rows::w_row(r, up), o.rows_w - 1);
       const uint32_t sw = o.ws.offset(row + (up ? o.up_rows : 0));
       s_off[i] = wave < 2 ? sx : sw;
@@ -77,7 +80,7 @@ struct MxLargeTile {
   MSLK_AMD_DEVINL static int wrap(int place) { return place < TS::PLACES ? place : place - TS::PLACES; }
 
   // Where the loads of step kt come from.  MAY_END: it may be the last one, with fewer chunks; lanes of missing chunks go back to chunk 0.
-  struct From { const uint8_t *x, *w; uint32_t even, odd; };   // rows of even and odd loads: swz() differs in bit 2
+  struct From { const uint8_t *x, *w; uint32_t even, odd; };   // rows of an even and an odd eight: swz() differs in bit 2
   template <bool MAY_END>
   MSLK_AMD_DEVINL From from(int kt) const {
     From f{x + (int64_t)kt * kMxStep, w + (int64_t)kt * kMxStep, 0, 0};
@@ -90,7 +93,7 @@ struct MxLargeTile {
   }
   template <bool MAY_END>
   MSLK_AMD_DEVINL void copy_x(char* stage, const From& f, int q) {
-    dma16(f.x, x_off[q] + (MAY_END ? q & 1 ? f.odd : f.even : 0u), stage + (wave_id() * 8 + q) * 1024);
+    dma16(f.x, x_off[q] + (MAY_END ? wave_id() & 1 ? f.odd : f.even : 0u), stage + (q * 4 + wave_id()) * 1024);
   }
   template <bool MAY_END>
   MSLK_AMD_DEVINL void copy_w(char* place, const From& f, int q) {   // place: of fragment q / 2
@@ -107,7 +110,7 @@ struct MxLargeTile {
   MSLK_AMD_DEVINL static v4i x_chunk(const char* stage, int tm, int j) { return Rows::chunk(stage + tm * 64 * kMxStep, wave_id() / 2, j); }
   MSLK_AMD_DEVINL static v4i w_chunk(const char* place, int j) { return Rows::chunk(place, wave_id() % 2, j); }
 
-  struct Held {   // of the step at hand
+  struct Held {   // of the step at hand (of X, the fragments with valid rows)
     v4i x[4][4], w[2][4];
     uint32_t sx[4], sw[4];
     int stage, place, quad;   // of its X, of its first fragment of W, of its scales
@@ -122,11 +125,11 @@ struct MxLargeTile {
     for (int tn = 0; tn < 4; ++tn) sw[tn] = *reinterpret_cast<const uint32_t*>(at + TS::BM * 16 + (tn * 2 + wave % 2) * 512);
   }
 
-  // quad_next, odd_next: of the scales of the step that follows.
-  template <int TN, bool MAY_END>
-  MSLK_AMD_DEVINL void group(char* lds, const From& f, int quad_next, int odd_next, Held& held, v16f (&acc)[4][4]) {
+  // F: fragments of X with valid rows.  XL: loads of X that the step issues.  quad_next, odd_next: of the scales of the step that follows.
+  template <int TN, int F, int XL, bool MAY_END>
+  MSLK_AMD_DEVINL void group(char* lds, const From& f, int quad_next, int odd_next, Held& held, v16f (&acc)[4][F]) {
     constexpr bool LAST = TN == 3;
-    constexpr int ND = TN == 0 ? 0 : LAST ? 12 : 2;
+    constexpr int SLOTS = 4 * F, ND = TN == 0 ? 0 : LAST ? 4 + XL : 2;
     uint32_t sx[4], sw[4];
     const char *w_next = w_place(lds, wrap(held.place + TN + 1)), *x_next = x_stage(lds, held.stage ^ 1);
     const int to = wrap(held.place + 8);
@@ -138,11 +141,11 @@ struct MxLargeTile {
       constexpr int J = decltype(jj)::value;
       held.w[(TN + 1) & 1][J] = w_chunk(w_next, J);
 #pragma unroll
-      for (int tm = 0; tm < 4; ++tm) {
+      for (int tm = 0; tm < F; ++tm) {
         Rows::template multiply<J>(held.w[TN & 1][J], held.x[tm][J], held.sw[TN], held.sx[tm], acc[TN][tm]);
-        const int slot = J * 4 + tm;
+        const int slot = J * F + tm;
 #pragma unroll
-        for (int q = slot * ND / 16; q < (slot + 1) * ND / 16; ++q) {
+        for (int q = slot * ND / SLOTS; q < (slot + 1) * ND / SLOTS; ++q) {
           if constexpr (!LAST) copy_w<MAY_END>(w_place(lds, wrap(to + TN - 1)), f, (TN - 1) * 2 + q);
           else if (q < 4) copy_w<MAY_END>(w_place(lds, wrap(to + 2 + (q >> 1))), f, 4 + q);
           else copy_x<MAY_END>(x_stage(lds, held.stage), f, q - 4);
@@ -166,14 +169,14 @@ struct MxLargeTile {
     }
   }
   // One step, with the loads of step `kt` of the tile that init() took last; ends_tile: the next step is the first of a tile.
-  template <bool MAY_END>
-  MSLK_AMD_DEVINL void step(char* lds, int kt, bool ends_tile, Held& held, v16f (&acc)[4][4]) {
+  template <int F, int XL, bool MAY_END>
+  MSLK_AMD_DEVINL void step(char* lds, int kt, bool ends_tile, Held& held, v16f (&acc)[4][F]) {
     const From f = from<MAY_END>(kt);
     const int quad_next = held.quad + (held.odd | (int)ends_tile), odd_next = ends_tile ? 0 : held.odd ^ 1;
-    group<0, MAY_END>(lds, f, quad_next, odd_next, held, acc);
-    group<1, MAY_END>(lds, f, quad_next, odd_next, held, acc);
-    group<2, MAY_END>(lds, f, quad_next, odd_next, held, acc);
-    group<3, MAY_END>(lds, f, quad_next, odd_next, held, acc);
+    group<0, F, XL, MAY_END>(lds, f, quad_next, odd_next, held, acc);
+    group<1, F, XL, MAY_END>(lds, f, quad_next, odd_next, held, acc);
+    group<2, F, XL, MAY_END>(lds, f, quad_next, odd_next, held, acc);
+    group<3, F, XL, MAY_END>(lds, f, quad_next, odd_next, held, acc);
     held.quad = quad_next;
     held.odd = odd_next;
   }
@@ -195,26 +198,28 @@ struct MxLargeTile {
     }
     wait_and_barrier<16>();
     held.stage = held.place = held.quad = held.odd = 0;
-    load_scales(lds, 0, 0, held.sx, held.sw);
+  }
+  // acc = the sums of the tile that was begun, of which the first 64 F rows are valid; begins with tile `next` (any valid one if there is none).
+  template <int F>
+  MSLK_AMD_DEVINL void run(char* lds, const MxOperands& next, Held& held, v16f (&acc)[4][F]) {
+    // (Read here and not in the last step before: they would be held over its sums' way out.)
+    load_scales(lds, held.quad, 0, held.sx, held.sw);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      held.w[0][j] = w_chunk(w_place(lds, 0), j);
+      held.w[0][j] = w_chunk(w_place(lds, held.place), j);
 #pragma unroll
-      for (int tm = 0; tm < 4; ++tm) held.x[tm][j] = x_chunk(x_stage(lds, 0), tm, j);
+      for (int tm = 0; tm < F; ++tm) held.x[tm][j] = x_chunk(x_stage(lds, held.stage), tm, j);
     }
-  }
-  // acc = the sums of the tile that was begun; begins with tile `next` (any valid one if there is none).
-  MSLK_AMD_DEVINL void run(char* lds, const MxOperands& next, Held& held, v16f (&acc)[4][4]) {
 #pragma unroll
     for (int tn = 0; tn < 4; ++tn)
 #pragma unroll
-      for (int tm = 0; tm < 4; ++tm)
+      for (int tm = 0; tm < F; ++tm)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[tn][tm][r] = 0.f;
     int kt = 0;
     for (; kt + 3 < steps; ++kt) {
       if ((kt & 1) == 0) copy_scales(lds, (kt >> 1) + 1);   // of steps kt + 2 and kt + 3
-      step<false>(lds, kt + 2, false, held, acc);
+      step<F, 2 * F, false>(lds, kt + 2, false, held, acc);
     }
     for (; kt < steps; ++kt) {
       if ((kt & 1) == 0 && kt + 2 < steps) copy_scales(lds, (kt >> 1) + 1);
@@ -223,7 +228,7 @@ struct MxLargeTile {
         quad += (steps + 1) >> 1;
         copy_scales(lds, 0);
       }
-      step<true>(lds, kt + 2 < steps ? kt + 2 : kt + 2 - steps, kt + 1 == steps, held, acc);
+      step<F, 8, true>(lds, kt + 2 < steps ? kt + 2 : kt + 2 - steps, kt + 1 == steps, held, acc);
     }
   }
 };
