@@ -26,11 +26,18 @@ MSLK_AMD_DEVINL void load_bias(const MxProblem& p, int n, bool whole, float (&b)
   }
 }
 
+// As store16_stream(), at a scalar base and a lane's offset.  (The data registers may be reused behind the statement: its wait states.)
+MSLK_AMD_DEVINL void store16_at(char* base, uint32_t off, uint4 val) {
+  const v4i v = {(int)val.x, (int)val.y, (int)val.z, (int)val.w};
+  asm volatile("global_store_dwordx4 %0, %1, %2 nt\n\ts_nop 1" : : "v"(off), "v"(v), "s"(base) : "memory");
+}
+
 // Sums of a tile to Y: rows m0 ... m0 + rows - 1, columns from n0.  Fragment tm of wave row wm begins at row wm * WAVE_ROW + tm * FRAG_ROW.
 // A lane's pieces of eight columns (16 bytes) are four of the eight of a row's line: by register bits r1, r0; the others have the other h.
 // Exchanging r0 with bit 4 of the lane and r1 with bit 3 leaves a register eight rows' whole lines, which are then written past the L2:
 // left in 32-byte pieces they reached the memory as such.
-template <int FM, int FN, int WN, int WAVE_ROW, int FRAG_ROW, bool GATED, bool BIAS, bool F16>
+// FULL: every row and column of the tile is valid and its rows begin on 16 bytes; N < 2^25.
+template <int FM, int FN, int WN, int WAVE_ROW, int FRAG_ROW, bool GATED, bool BIAS, bool F16, bool FULL>
 MSLK_AMD_DEVINL void store_tile(const MxProblem& p, const v16f (&acc)[FN][FM], int m0, int rows, int n0) {
   int lane = threadIdx.x & 63;
   asm volatile("" : "+v"(lane));   // formed again here, not kept over the products
@@ -40,25 +47,24 @@ MSLK_AMD_DEVINL void store_tile(const MxProblem& p, const v16f (&acc)[FN][FM], i
   constexpr int LINES = GATED ? (FN + 3) / 4 : FN / 2, PIECES = GATED && FN == 2 ? 2 : 4;   // of 64 columns; of a lane in a line
   // column of piece r of line t for the lanes of half h
   auto column = [&](int t, int r, int half) { return GATED ? t * 64 + (r >> 1) * 32 + half * 16 + (r & 1) * 8 : t * 64 + r * 16 + half * 8; };
-  float b[BIAS ? LINES : 1][4][8];
-  if constexpr (BIAS) {
-    const bool bias_aligned = (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0;
+  // after the exchange: this lane's piece and row of each register
+  const int piece = ((lane >> 3) & 1) * 2 + ((lane >> 4) & 1), row8 = lane & 7;
+  const uint32_t lane_off = 2u * ((uint32_t)row8 * (uint32_t)p.N + (uint32_t)column(0, piece, h));
 #pragma unroll
-    for (int t = 0; t < LINES; ++t)
+  for (int t = 0; t < LINES; ++t) {
+    float b[4][8];
+    if constexpr (BIAS) {
+      const bool bias_aligned = (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const int n = first + column(t, r, h);
-        load_bias(p, n, bias_aligned && n + 8 <= p.N, b[t][r]);
+        load_bias(p, n, bias_aligned && (FULL || n + 8 <= p.N), b[r]);
       }
-  }
-  // after the exchange: this lane's piece and row of each register
-  const int piece = ((lane >> 3) & 1) * 2 + ((lane >> 4) & 1), row8 = lane & 7;
+    }
 #pragma unroll
-  for (int tm = 0; tm < FM; ++tm) {
-    const int row0 = wm * WAVE_ROW + tm * FRAG_ROW;
-    if (row0 >= rows) break;
-#pragma unroll
-    for (int t = 0; t < LINES; ++t) {
+    for (int tm = 0; tm < FM; ++tm) {
+      const int row0 = wm * WAVE_ROW + tm * FRAG_ROW;
+      if (!FULL && row0 >= rows) break;
       uint32_t w[4][4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
@@ -70,7 +76,7 @@ MSLK_AMD_DEVINL void store_tile(const MxProblem& p, const v16f (&acc)[FN][FM], i
             v[e] = r < PIECES ? gated_value(acc[2 * T][tm][at], acc[2 * T + 1][tm][at]) : 0.f;
           } else {
             v[e] = acc[2 * t + (e >> 2)][tm][4 * r + (e & 3)];
-            if constexpr (BIAS) v[e] += b[t][r][e];
+            if constexpr (BIAS) v[e] += b[r][e];
           }
         }
 #pragma unroll
@@ -90,6 +96,14 @@ MSLK_AMD_DEVINL void store_tile(const MxProblem& p, const v16f (&acc)[FN][FM], i
           w[r][e] = __builtin_amdgcn_update_dpp(lo, hi, 0x128, 0xF, 0xC, false);
           w[r + 2][e] = __builtin_amdgcn_update_dpp(hi, lo, 0x128, 0xF, 0x3, false);
         }
+      }
+      if constexpr (FULL) {
+        // one address for all lanes, and the lane's place in the eight rows
+        char* const base = reinterpret_cast<char*>(p.y + (int64_t)(m0 + row0) * p.N + first + t * 64);
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          store16_at(base + (int64_t)((r & 1) * 16 + (r >> 1) * 8) * p.N * 2, lane_off, make_uint4(w[r][0], w[r][1], w[r][2], w[r][3]));
+        continue;
       }
       const int n = first + column(t, piece, h), columns = p.N - n;
       const bool mine = columns > 0 && piece < PIECES;
@@ -159,7 +173,7 @@ __global__ __launch_bounds__(TS::NTHREADS) void mx_kernel(MxProblem p, int tiles
   MxTile<TS, GATED> tile;
   tile.init(operands_of<GATED>(p, m0, rows, w_row, n0, COLUMNS));
   tile.run(lds, acc);
-  store_tile<TS::FM, TS::FN, TS::WN, TS::BM / TS::WM, 32, GATED, BIAS, F16>(p, acc, m0, rows, n0);
+  store_tile<TS::FM, TS::FN, TS::WN, TS::BM / TS::WM, 32, GATED, BIAS, F16, false>(p, acc, m0, rows, n0);
 }
 
 // Row tiles: of p.tile_rows rows, or as listed in device memory.
@@ -178,6 +192,7 @@ __global__ __launch_bounds__(256) void mx_walk_kernel(MxProblem p, int tiles_m, 
   const int end = min(per_xcd, total - first);
   int j = blockIdx.x / kXcds;
   if (j >= end) return;
+  const bool aligned = (p.N & 7) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
   struct Place { int m0, rows, n0; int64_t w_row; };
   auto place_of = [&](int t) {
     int tm, tn;
@@ -201,7 +216,8 @@ __global__ __launch_bounds__(256) void mx_walk_kernel(MxProblem p, int tiles_m, 
       constexpr int F = decltype(fragments)::value;
       v16f acc[4][F];
       tile.template run<F>(lds, operands(at), held, acc);
-      store_tile<F, 4, 2, 32, 64, GATED, BIAS, F16>(p, acc, here.m0, here.rows, here.n0);
+      if (here.rows == 64 * F && here.n0 + COLUMNS <= p.N && aligned) store_tile<F, 4, 2, 32, 64, GATED, BIAS, F16, true>(p, acc, here.m0, here.rows, here.n0);
+      else store_tile<F, 4, 2, 32, 64, GATED, BIAS, F16, false>(p, acc, here.m0, here.rows, here.n0);
     };
     if (here.rows > 128) make(std::integral_constant<int, 4>{});
     else if (here.rows > 64) make(std::integral_constant<int, 2>{});
@@ -336,7 +352,7 @@ enum Way : int {
 Way way_of(int64_t M, int64_t N, int64_t K, int gated, bool grouped) {
   constexpr int kStreamTiles = 384;
   if (!grouped && M <= 64 && N * (gated ? 2 : 1) <= 32 * kStreamTiles) return kStream;
-  return M <= 64 || K <= 256 ? kTiles : kWalk;
+  return M <= 64 || K <= 256 || N >= (1 << 25) ? kTiles : kWalk;
 }
 
 // Rows of a row tile: as many as leave every CU a tile.

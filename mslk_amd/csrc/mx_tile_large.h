@@ -38,17 +38,27 @@ struct MxLargeTile {
   const uint8_t *x, *w, *s_base;
   int pair_stride, steps, last_chunks;
   int quad;   // place of the scales of its first two steps
+  int rows_x, rows_w;
+  uint32_t first_x, first_w;   // what the offsets were formed for
 
   MSLK_AMD_DEVINL static int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
   // A load covers 8 LDS rows, or the 16 bytes of scales of 64 rows.  The loads of X are dealt to the waves in turn; wave v makes loads
   // 2 v and 2 v + 1 of each fragment of W, and 2 v and 2 v + 1 of the scales (of X, then of W).
+  template <bool FIRST>
   MSLK_AMD_DEVINL void init(const MxOperands& o) {
+    x = uniform_ptr(o.x);
+    w = uniform_ptr(o.w);
+    s_base = uniform_ptr(wave_id() < 2 ? o.xs.base : o.ws.base);
+    // (most tiles have all their rows and columns, and the offsets of the one before)
+    if (!FIRST && o.rows_x == rows_x && o.rows_w == rows_w && o.xs.first == first_x && o.ws.first == first_w) return;
+    rows_x = o.rows_x;
+    rows_w = o.rows_w;
+    first_x = o.xs.first;
+    first_w = o.ws.first;
     int lane = threadIdx.x & 63;
     asm volatile("" : "+v"(lane));   // formed again for each tile, not kept
     const int wave = wave_id();
-    x = uniform_ptr(o.x);
-    w = uniform_ptr(o.w);
     bool up;
 #pragma unroll
     for (int q = 0; q < 8; ++q) {
@@ -61,8 +71,6 @@ struct MxLargeTile {
       const int row = min(Rows::w_row(r, up), o.rows_w - 1);
       w_off[q] = (uint32_t)row * o.ld + (up ? o.up : 0u) + (((lane & 7) ^ mx_swz(r)) << 4);
     }
-    s_base = uniform_ptr(wave < 2 ? o.xs.base : o.ws.base);
-    pair_stride = o.xs.pair_stride;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = ((wave & 1) * 2 + i) * 64 + lane;
@@ -125,8 +133,8 @@ struct MxLargeTile {
     for (int tn = 0; tn < 4; ++tn) sw[tn] = *reinterpret_cast<const uint32_t*>(at + TS::BM * 16 + (tn * 2 + wave % 2) * 512);
   }
 
-  // F: fragments of X with valid rows.  XL: loads of X that the step issues.  quad_next, odd_next: of the scales of the step that follows.
-  template <int TN, int F, int XL, bool MAY_END>
+  // F: fragments of X with valid rows.  XL: loads of X that the step issues.  FIRST: of a tile, sums begin with it.  quad_next, odd_next: of the scales of the step that follows.
+  template <int TN, int F, int XL, bool MAY_END, bool FIRST>
   MSLK_AMD_DEVINL void group(char* lds, const From& f, int quad_next, int odd_next, Held& held, v16f (&acc)[4][F]) {
     constexpr bool LAST = TN == 3;
     constexpr int SLOTS = 4 * F, ND = TN == 0 ? 0 : LAST ? 4 + XL : 2;
@@ -142,6 +150,9 @@ struct MxLargeTile {
       held.w[(TN + 1) & 1][J] = w_chunk(w_next, J);
 #pragma unroll
       for (int tm = 0; tm < F; ++tm) {
+        if constexpr (FIRST && J == 0)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[TN][tm][r] = 0.f;
         Rows::template multiply<J>(held.w[TN & 1][J], held.x[tm][J], held.sw[TN], held.sx[tm], acc[TN][tm]);
         const int slot = J * F + tm;
 #pragma unroll
@@ -169,14 +180,14 @@ struct MxLargeTile {
     }
   }
   // One step, with the loads of step `kt` of the tile that init() took last; ends_tile: the next step is the first of a tile.
-  template <int F, int XL, bool MAY_END>
+  template <int F, int XL, bool MAY_END, bool FIRST>
   MSLK_AMD_DEVINL void step(char* lds, int kt, bool ends_tile, Held& held, v16f (&acc)[4][F]) {
     const From f = from<MAY_END>(kt);
     const int quad_next = held.quad + (held.odd | (int)ends_tile), odd_next = ends_tile ? 0 : held.odd ^ 1;
-    group<0, F, XL, MAY_END>(lds, f, quad_next, odd_next, held, acc);
-    group<1, F, XL, MAY_END>(lds, f, quad_next, odd_next, held, acc);
-    group<2, F, XL, MAY_END>(lds, f, quad_next, odd_next, held, acc);
-    group<3, F, XL, MAY_END>(lds, f, quad_next, odd_next, held, acc);
+    group<0, F, XL, MAY_END, FIRST>(lds, f, quad_next, odd_next, held, acc);
+    group<1, F, XL, MAY_END, FIRST>(lds, f, quad_next, odd_next, held, acc);
+    group<2, F, XL, MAY_END, FIRST>(lds, f, quad_next, odd_next, held, acc);
+    group<3, F, XL, MAY_END, FIRST>(lds, f, quad_next, odd_next, held, acc);
     held.quad = quad_next;
     held.odd = odd_next;
   }
@@ -186,7 +197,8 @@ struct MxLargeTile {
     steps = o.steps;
     last_chunks = o.last_chunks;
     quad = 0;
-    init(o);
+    pair_stride = o.xs.pair_stride;
+    init<true>(o);
     copy_scales(lds, 0);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -210,25 +222,26 @@ struct MxLargeTile {
 #pragma unroll
       for (int tm = 0; tm < F; ++tm) held.x[tm][j] = x_chunk(x_stage(lds, held.stage), tm, j);
     }
-#pragma unroll
-    for (int tn = 0; tn < 4; ++tn)
-#pragma unroll
-      for (int tm = 0; tm < F; ++tm)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[tn][tm][r] = 0.f;
-    int kt = 0;
-    for (; kt + 3 < steps; ++kt) {
-      if ((kt & 1) == 0) copy_scales(lds, (kt >> 1) + 1);   // of steps kt + 2 and kt + 3
-      step<F, 2 * F, false>(lds, kt + 2, false, held, acc);
-    }
-    for (; kt < steps; ++kt) {
-      if ((kt & 1) == 0 && kt + 2 < steps) copy_scales(lds, (kt >> 1) + 1);
-      if (kt + 2 == steps) init(next);
+    // What a step begins with: the scales of a pair; the next tile.
+    auto begin = [&](int kt) {
+      if ((kt & 1) == 0 && kt + 2 < steps) copy_scales(lds, (kt >> 1) + 1);   // of steps kt + 2 and kt + 3
+      if (kt + 2 == steps) init<false>(next);
       if (kt + 1 == steps) {   // (with an odd number of steps the place is in use until now)
         quad += (steps + 1) >> 1;
         copy_scales(lds, 0);
       }
-      step<F, 8, true>(lds, kt + 2 < steps ? kt + 2 : kt + 2 - steps, kt + 1 == steps, held, acc);
+    };
+    auto issued = [&](int kt) { return kt + 2 < steps ? kt + 2 : kt + 2 - steps; };
+    begin(0);
+    step<F, 8, true, true>(lds, issued(0), false, held, acc);
+    int kt = 1;
+    for (; kt + 3 < steps; ++kt) {
+      if ((kt & 1) == 0) copy_scales(lds, (kt >> 1) + 1);
+      step<F, 2 * F, false, false>(lds, kt + 2, false, held, acc);
+    }
+    for (; kt < steps; ++kt) {
+      begin(kt);
+      step<F, 8, true, false>(lds, issued(kt), kt + 1 == steps, held, acc);
     }
   }
 };
