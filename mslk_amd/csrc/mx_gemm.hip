@@ -6,12 +6,9 @@
 namespace mslk_amd {
 namespace {
 
-// Eight columns n ... n + 7 of the bias, as fp32; `whole`: they exist and lie on 16 bytes.
-MSLK_AMD_DEVINL void load_bias(const MxProblem& p, int n, bool whole, float (&b)[8]) {
-  if (!whole) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) b[e] = bias_at(p, min(n + e, p.N - 1));
-  } else if (p.bias_dtype == 1) {
+// Eight columns n ... n + 7 of the bias, which lie on 16 bytes, as fp32.
+MSLK_AMD_DEVINL void load_bias(const MxProblem& p, int n, float (&b)[8]) {
+  if (p.bias_dtype == 1) {
     const float4 *f = reinterpret_cast<const float4*>(static_cast<const float*>(p.bias) + n), lo = f[0], hi = f[1];
     b[0] = lo.x; b[1] = lo.y; b[2] = lo.z; b[3] = lo.w;
     b[4] = hi.x; b[5] = hi.y; b[6] = hi.z; b[7] = hi.w;
@@ -36,7 +33,7 @@ MSLK_AMD_DEVINL void store16_at(char* base, uint32_t off, uint4 val) {
 // A lane's pieces of eight columns (16 bytes) are four of the eight of a row's line: by register bits r1, r0; the others have the other h.
 // Exchanging r0 with bit 4 of the lane and r1 with bit 3 leaves a register eight rows' whole lines, which are then written past the L2:
 // left in 32-byte pieces they reached the memory as such.
-// FULL: every row and column of the tile is valid and its rows begin on 16 bytes; N < 2^25.
+// FULL: every row and column of the tile is valid, its rows and the bias begin on 16 bytes; N < 2^25.
 template <int FM, int FN, int WN, int WAVE_ROW, int FRAG_ROW, bool GATED, bool BIAS, bool F16, bool FULL>
 MSLK_AMD_DEVINL void store_tile(const MxProblem& p, const v16f (&acc)[FN][FM], int m0, int rows, int n0) {
   int lane = threadIdx.x & 63;
@@ -53,13 +50,9 @@ MSLK_AMD_DEVINL void store_tile(const MxProblem& p, const v16f (&acc)[FN][FM], i
 #pragma unroll
   for (int t = 0; t < LINES; ++t) {
     float b[4][8];
-    if constexpr (BIAS) {
-      const bool bias_aligned = (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0;
+    if constexpr (BIAS && FULL) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int n = first + column(t, r, h);
-        load_bias(p, n, bias_aligned && (FULL || n + 8 <= p.N), b[r]);
-      }
+      for (int r = 0; r < 4; ++r) load_bias(p, first + column(t, r, h), b[r]);
     }
 #pragma unroll
     for (int tm = 0; tm < FM; ++tm) {
@@ -76,7 +69,8 @@ MSLK_AMD_DEVINL void store_tile(const MxProblem& p, const v16f (&acc)[FN][FM], i
             v[e] = r < PIECES ? gated_value(acc[2 * T][tm][at], acc[2 * T + 1][tm][at]) : 0.f;
           } else {
             v[e] = acc[2 * t + (e >> 2)][tm][4 * r + (e & 3)];
-            if constexpr (BIAS) v[e] += b[r][e];
+            if constexpr (BIAS && FULL) v[e] += b[r][e];
+            else if constexpr (BIAS) v[e] += bias_at(p, min(first + column(t, r, h) + e, p.N - 1));
           }
         }
 #pragma unroll
@@ -179,7 +173,11 @@ __global__ __launch_bounds__(TS::NTHREADS) void mx_kernel(MxProblem p, int tiles
 // Row tiles: of p.tile_rows rows, or as listed in device memory.
 struct RowTile { int row0, rows, group, unused; };
 
-// A workgroup per CU that walks the 256-column tiles: XCD x keeps its run of neighbouring entries, its workgroups take them in turn.
+// A workgroup per CU that walks the 256-column tiles.
+// One matrix: XCD x keeps a run of neighbouring entries of the list, its workgroups take them in turn: the XCDs then ask for the same weights at
+// about the same time, and the Infinity Cache serves all but the first (dealt in rounds as below, 8192 x 28672 x 4096 takes 686 us instead of 490).
+// Groups: in rounds; of each round's entries, neighbours all, XCD x takes a run.  The list has long tiles first, so those of a round are about
+// as long, where runs of the whole list leave the XCDs different amounts (16 experts of 8192 rows 236 us instead of 225).
 template <bool GATED, bool BIAS, bool F16>
 __global__ __launch_bounds__(256) void mx_walk_kernel(MxProblem p, int tiles_m, int tiles_n) {
   using TS = MxLarge;
@@ -188,11 +186,15 @@ __global__ __launch_bounds__(256) void mx_walk_kernel(MxProblem p, int tiles_m, 
   constexpr int COLUMNS = GATED ? TS::BN / 2 : TS::BN;
   const RowTile* const list = static_cast<const RowTile*>(p.row_tiles);
   if (list != nullptr) tiles_m = list[0].rows;   // (the first entry holds their number)
-  const int total = tiles_m * tiles_n, per_xcd = (total + kXcds - 1) / kXcds, first = (int)(blockIdx.x % kXcds) * per_xcd, stride = gridDim.x / kXcds;
-  const int end = min(per_xcd, total - first);
-  int j = blockIdx.x / kXcds;
-  if (j >= end) return;
-  const bool aligned = (p.N & 7) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0;
+  const int total = tiles_m * tiles_n, wgs = gridDim.x, xcd = blockIdx.x % kXcds, slot = blockIdx.x / kXcds;
+  auto entry = [&](int round) {   // this workgroup's `round`th entry, -1: none
+    const int first = list != nullptr ? round * wgs : 0, here = list != nullptr ? min(total - first, wgs) : total;
+    const int run = (here + kXcds - 1) / kXcds, in_run = list != nullptr ? slot : slot + round * (wgs / kXcds), at = xcd * run + in_run;
+    return in_run < run && at < here ? first + at : -1;
+  };
+  int t = entry(0), round = 0;
+  if (t < 0) return;
+  const bool aligned = (p.N & 7) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && (!BIAS || (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0);
   struct Place { int m0, rows, n0; int64_t w_row; };
   auto place_of = [&](int t) {
     int tm, tn;
@@ -204,14 +206,14 @@ __global__ __launch_bounds__(256) void mx_walk_kernel(MxProblem p, int tiles_m, 
     return Place{tm * p.tile_rows, min(p.M - tm * p.tile_rows, p.tile_rows), tn * COLUMNS, 0};
   };
   auto operands = [&](const Place& at) { return operands_of<GATED>(p, at.m0, at.rows, at.w_row, at.n0, COLUMNS); };
-  Place at = place_of(first + j);
+  Place at = place_of(t);
   Tile tile;
   typename Tile::Held held;
   tile.start(lds, operands(at), held);
   for (;;) {
     const Place here = at;
-    j += stride;
-    if (j < end) at = place_of(first + j);   // (behind the last tile: itself once more)
+    t = entry(++round);
+    if (t >= 0) at = place_of(t);   // (behind the last tile: itself once more)
     auto make = [&](auto fragments) {
       constexpr int F = decltype(fragments)::value;
       v16f acc[4][F];
@@ -219,88 +221,129 @@ __global__ __launch_bounds__(256) void mx_walk_kernel(MxProblem p, int tiles_m, 
       if (here.rows == 64 * F && here.n0 + COLUMNS <= p.N && aligned) store_tile<F, 4, 2, 32, 64, GATED, BIAS, F16, true>(p, acc, here.m0, here.rows, here.n0);
       else store_tile<F, 4, 2, 32, 64, GATED, BIAS, F16, false>(p, acc, here.m0, here.rows, here.n0);
     };
-    if (here.rows > 128) make(std::integral_constant<int, 4>{});
+    if (here.rows > 192) make(std::integral_constant<int, 4>{});
+    else if (here.rows > 128) make(std::integral_constant<int, 3>{});
     else if (here.rows > 64) make(std::integral_constant<int, 2>{});
     else make(std::integral_constant<int, 1>{});
-    if (j >= end) break;
+    if (t < 0) break;
   }
   wait_vmcnt0();   // the loads of a tile that does not follow end before the LDS is given away
 }
 
-// Tensors of scales, rows of `from` bytes, to the arranged layout (MxScales); both operands in one launch.  A lane moves 16 bytes, eight
-// lanes a line of one row, eight rows to the lines of eight pairs.
+// Tensors of scales, rows of `from` bytes, to the arranged layout (MxScales), of both operands in one launch.  A workgroup takes up to 32 pairs
+// of 64 rows through LDS, so that it reads and writes whole lines; the first one makes the list of row tiles.
+constexpr int kArrangePairs = 32;
 struct ArrangeJob {
   const uint8_t* src;
   uint8_t* dst;
-  int64_t rows, workgroups;
+  int64_t rows;
+  int workgroups;
 };
-// Row tiles of the groups (at most 256 rows each), in the first workgroup: list[0].rows of them behind list[0].
+// Row tiles of the groups, at most 256 rows each, the longest first (by the fragments that they take): list[0].rows of them behind list[0].
 struct ListJob {
   const int64_t* m_sizes;   // nullptr: none
   RowTile* list;
   int G, M;
 };
-MSLK_AMD_DEVINL void list_row_tiles(const ListJob& job) {
-  __shared__ int64_t rows_to[512];   // rows of the groups up to and with this one, tiles likewise
-  __shared__ int tiles_to[512];
-  int64_t rows_before = 0;
-  int tiles_before = 0;
-  const int i = threadIdx.x;
-  for (int g0 = 0; g0 < job.G; g0 += 512) {
-    const int g = g0 + i;
-    const int64_t size = g < job.G ? max((int64_t)0, min(job.m_sizes[g], (int64_t)job.M)) : 0;
-    rows_to[i] = size;
-    __syncthreads();
-    for (int d = 1; d < 512; d *= 2) {
-      const int64_t add = i >= d ? rows_to[i - d] : 0;
-      __syncthreads();
-      rows_to[i] += add;
-      __syncthreads();
-    }
-    const int64_t start = rows_before + rows_to[i] - size;
-    const int live = (int)max((int64_t)0, min(size, job.M - start)), tiles = (live + MxLarge::BM - 1) / MxLarge::BM;
-    tiles_to[i] = tiles;
-    __syncthreads();
-    for (int d = 1; d < 512; d *= 2) {
-      const int add = i >= d ? tiles_to[i - d] : 0;
-      __syncthreads();
-      tiles_to[i] += add;
-      __syncthreads();
-    }
-    RowTile* out = job.list + 1 + tiles_before + tiles_to[i] - tiles;
-    for (int t = 0; t < tiles; ++t) out[t] = RowTile{(int)start + t * MxLarge::BM, min(live - t * MxLarge::BM, MxLarge::BM), g, 0};
-    rows_before += rows_to[511];
-    tiles_before += tiles_to[511];
-    __syncthreads();
-  }
-  if (i == 0) job.list[0] = RowTile{0, tiles_before, 0, 0};
+
+// Sums over the lanes up to and with this one, at most `most` (< 2^31).
+template <int CTRL, int ROWS>
+MSLK_AMD_DEVINL uint32_t add_from(uint32_t v, uint32_t most) {
+  return min(v + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false), most);
+}
+MSLK_AMD_DEVINL uint32_t lanes_to(uint32_t v, uint32_t most) {
+  v = add_from<0x111, 0xF>(v, most);   // from 1, 2, 4, 8 lanes below inside 16
+  v = add_from<0x112, 0xF>(v, most);
+  v = add_from<0x114, 0xF>(v, most);
+  v = add_from<0x118, 0xF>(v, most);
+  v = add_from<0x142, 0xA>(v, most);   // lane 15 of a row to the second and fourth row
+  return add_from<0x143, 0xC>(v, most);   // lane 31 to the upper half
 }
 
-__global__ __launch_bounds__(512) void arrange_scales_kernel(ArrangeJob a, ArrangeJob b, ListJob tiles, int from, int pairs) {
-  if (tiles.m_sizes != nullptr && blockIdx.x == 0) list_row_tiles(tiles);
-  const bool second = blockIdx.x >= a.workgroups;
-  const ArrangeJob job = second ? b : a;
-  const int64_t at = blockIdx.x - (second ? a.workgroups : 0);
-  const int slabs = (pairs + 7) / 8;   // a workgroup: 64 rows, eight pairs
-  const int64_t block = at / slabs;
-  const int pair = (int)(at - block * slabs) * 8 + (threadIdx.x & 7), r = threadIdx.x >> 3;
-  const int64_t row = block * 64 + r;
-  if (pair >= pairs || row >= job.rows) return;
-  const int col = pair * 16;
-  const uint8_t* in = job.src + row * from + col;
-  uint32_t w[4];
-  if (col + 16 <= from) {
-    __builtin_memcpy(w, in, 16);
-  } else {
+// By one wave; `held` of the sizes are in LDS.
+MSLK_AMD_DEVINL uint32_t group_size(const ListJob& job, int g) { return (uint32_t)max((int64_t)0, min(job.m_sizes[g], (int64_t)job.M)); }
+MSLK_AMD_DEVINL void list_row_tiles(const ListJob& job, const uint32_t* sizes, int held) {
+  constexpr int ROWS = MxLarge::BM;
+  const int lane = threadIdx.x & 63;
+  int at[4] = {0, 0, 0, 0};   // where the next tile of 4, 3, 2, 1 fragments goes; first their numbers
+  for (int pass = 0; pass < 2; ++pass) {
+    uint32_t before = 0;      // rows of the groups before these 64
+    for (int g0 = 0; g0 < job.G; g0 += 64) {
+      const int g = g0 + lane;
+      const uint32_t size = g >= job.G ? 0u : g < held ? sizes[g] : group_size(job, g);
+      const uint32_t to = lanes_to(size, (uint32_t)job.M);
+      const uint32_t start = min(before + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)to, 0x138, 0xF, 0xF, false), (uint32_t)job.M);   // of the lane below
+      const int live = (int)min(size, (uint32_t)job.M - start), rest = live % ROWS;
+      const int whole = live / ROWS + (rest > 192 ? 1 : 0);                                      // tiles of four fragments
+      const int other = rest == 0 || rest > 192 ? 0 : rest > 128 ? 1 : rest > 64 ? 2 : 3;        // place in `at` of the last one
+      const uint32_t whole_to = lanes_to((uint32_t)whole, 0xFFFFFFFFu);
+      if (pass == 1) {
+        RowTile* out = job.list + 1 + at[0] + (int)whole_to - whole;
+        for (int t = 0; t < whole; ++t) out[t] = RowTile{(int)start + t * ROWS, min(live - t * ROWS, ROWS), g, 0};
+      }
+      at[0] += __builtin_amdgcn_readlane((int)whole_to, 63);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      w[i] = 0;
+      for (int c = 1; c < 4; ++c) {
+        const uint64_t mine = __ballot(other == c);
+        if (pass == 1 && other == c)
+          job.list[1 + at[c] + __popcll(mine & ((uint64_t(1) << lane) - 1))] = RowTile{(int)start + live - rest, rest, g, 0};
+        at[c] += __popcll(mine);
+      }
+      before = min(before + (uint32_t)__builtin_amdgcn_readlane((int)to, 63), (uint32_t)job.M);
+    }
+    if (pass == 0) {   // numbers to places
+      int sum = 0;
 #pragma unroll
-      for (int b = 0; b < 4; ++b)
-        if (col + 4 * i + b < from) w[i] |= (uint32_t)in[4 * i + b] << (8 * b);
+      for (int c = 0; c < 4; ++c) {
+        const int n = at[c];
+        at[c] = sum;
+        sum += n;
+      }
+      if (lane == 0) job.list[0] = RowTile{0, sum, 0, 0};
     }
   }
-  reinterpret_cast<uint4*>(job.dst)[(block * pairs + pair) * 64 + r] = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__global__ __launch_bounds__(256) void arrange_scales_kernel(ArrangeJob a, ArrangeJob b, ListJob tiles, int from, int pairs) {
+  extern __shared__ __attribute__((aligned(16))) uint4 piece[];   // [row][pair], an odd number of pieces per row
+  int at = blockIdx.x;
+  if (tiles.m_sizes != nullptr && at-- == 0) {
+    uint32_t* const sizes = reinterpret_cast<uint32_t*>(piece);
+    const int held = min(tiles.G, 64 * 4);
+    for (int g = threadIdx.x; g < held; g += 256) sizes[g] = group_size(tiles, g);
+    __syncthreads();
+    if (threadIdx.x < 64) list_row_tiles(tiles, sizes, held);
+    return;
+  }
+  const bool second = at >= a.workgroups;
+  const ArrangeJob job = second ? b : a;
+  if (second) at -= a.workgroups;
+  const int slabs = (pairs + kArrangePairs - 1) / kArrangePairs, block = at / slabs, pair0 = (at - block * slabs) * kArrangePairs;
+  const int n = min(pairs - pair0, kArrangePairs), rows = (int)min((int64_t)64, job.rows - (int64_t)block * 64);
+  const int pitch = n | 1;
+  const uint32_t inverse = (65536u + (uint32_t)n - 1) / (uint32_t)n;   // i / n = i * inverse >> 16 for i < 64 n, n <= 32
+  const uint8_t* src = job.src + (int64_t)block * 64 * from + pair0 * 16;
+  for (int i = threadIdx.x; i < rows * n; i += 256) {
+    const int r = (int)(((uint32_t)i * inverse) >> 16), q = i - r * n, left = from - (pair0 + q) * 16;
+    const uint8_t* in = src + (int64_t)r * from + q * 16;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (left >= 16) {
+      __builtin_memcpy(&v, in, 16);   // (rows begin anywhere)
+    } else {
+      uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (e < left) w[e >> 2] |= (uint32_t)in[e] << (8 * (e & 3));
+      v = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    piece[r * pitch + q] = v;
+  }
+  __syncthreads();
+  uint4* dst = reinterpret_cast<uint4*>(job.dst) + ((int64_t)block * pairs + pair0) * 64;
+  for (int i = threadIdx.x; i < 64 * n; i += 256) {
+    const int r = i & 63, q = i >> 6;
+    if (r < rows) dst[i] = piece[r * pitch + q];
+  }
 }
 
 int64_t pairs_of(int64_t K) { return (K + 511) / 512; }
@@ -344,6 +387,7 @@ hipError_t launch_walk(const MxProblem& p, hipStream_t s) {
   return p.bias_dtype != 0 ? launch_walk<false, true, F16>(p, s) : launch_walk<false, false, F16>(p, s);
 }
 
+constexpr int kFewRows = 64;
 enum Way : int {
   kStream,   // few rows: mx_stream.hip
   kTiles,    // 64 x 128 tiles
@@ -353,6 +397,12 @@ Way way_of(int64_t M, int64_t N, int64_t K, int gated, bool grouped) {
   constexpr int kStreamTiles = 384;
   if (!grouped && M <= 64 && N * (gated ? 2 : 1) <= 32 * kStreamTiles) return kStream;
   return M <= 64 || K <= 256 || N >= (1 << 25) ? kTiles : kWalk;
+}
+
+// Whether the scales are arranged first.  Not where the product waits for the weights (few rows per group), if they can be fetched as they are.
+bool arranges(Way way, int64_t M, int64_t K, int G, bool grouped, bool scales_aligned) {
+  if (K % 512 != 0 || !scales_aligned) return true;
+  return way == kWalk && !(grouped && M <= kFewRows * G);
 }
 
 // Rows of a row tile: as many as leave every CU a tile.
@@ -367,9 +417,10 @@ int rows_of_tile(int64_t M, int64_t N, int gated) {
 size_t mx_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated, int G, bool grouped, bool scales_aligned) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
   const Way way = way_of(M, N, K, gated, grouped);
-  if (way == kStream || (way == kTiles && K % 512 == 0 && scales_aligned)) return 0;
+  if (way == kStream) return 0;
   const int64_t list = way == kWalk && grouped ? (1 + most_row_tiles(M, G, MxLarge::BM)) * (int64_t)sizeof(RowTile) : 0;
-  return (size_t)(arranged_bytes(M, K) + arranged_bytes(N * (gated ? 2 : 1) * (grouped ? G : 1), K) + list);
+  if (!arranges(way, M, K, G, grouped, scales_aligned)) return (size_t)list;
+  return (size_t)(list + arranged_bytes(M, K) + arranged_bytes(N * (gated ? 2 : 1) * (grouped ? G : 1), K));
 }
 
 hipError_t launch_mx_mm(MxProblem p, void* workspace, bool scales_aligned, hipStream_t s) {
@@ -378,24 +429,33 @@ hipError_t launch_mx_mm(MxProblem p, void* workspace, bool scales_aligned, hipSt
   if (way == kStream) return launch_mx_stream(p, s);
   const int from = p.K / kMxBlock, pairs = (int)pairs_of(p.K);
   p.tile_rows = grouped ? MxLarge::BM : rows_of_tile(p.M, p.N, p.gated);
-  if (p.K > 0 && (way == kWalk || p.K % 512 != 0 || !scales_aligned)) {
-    const int64_t rows_w = (int64_t)p.N * (p.gated ? 2 : 1) * (grouped ? p.G : 1);
-    uint8_t *xs = static_cast<uint8_t*>(workspace), *ws = xs + arranged_bytes(p.M, p.K), *list = ws + arranged_bytes(rows_w, p.K);
-    const int64_t slabs = (pairs + 7) / 8;
-    const ArrangeJob a{p.xs.data, xs, p.M, (p.M + 63) / 64 * slabs}, b{p.ws.data, ws, rows_w, (rows_w + 63) / 64 * slabs};
-    ListJob tiles{};
-    if (way == kWalk && grouped) {
-      tiles = ListJob{p.m_sizes, reinterpret_cast<RowTile*>(list), p.G, p.M};
-      p.row_tiles = list;
-    }
-    if ((a.workgroups + b.workgroups) * 512 >= (int64_t(1) << 32)) return hipErrorInvalidValue;
-    arrange_scales_kernel<<<(unsigned)(a.workgroups + b.workgroups), 512, 0, s>>>(a, b, tiles, from, pairs);
+  const bool listed = way == kWalk && grouped, arranged = p.K > 0 && arranges(way, p.M, p.K, p.G, grouped, scales_aligned);
+  ArrangeJob a{}, b{};
+  ListJob tiles{};
+  uint8_t* room = static_cast<uint8_t*>(workspace);
+  if (listed) {
+    tiles = ListJob{p.m_sizes, reinterpret_cast<RowTile*>(room), p.G, p.M};
+    p.row_tiles = room;
+    room += (1 + most_row_tiles(p.M, p.G, MxLarge::BM)) * (int64_t)sizeof(RowTile);
+  }
+  const MxScales in_tensor{nullptr, (int64_t)from * 64, from, 16}, in_order{nullptr, (int64_t)pairs * 1024, 16, 1024};
+  auto scales = [&](MxScales& s, int64_t rows, ArrangeJob& job) {
+    const uint8_t* tensor = s.data;
+    s = arranged ? in_order : in_tensor;
+    s.data = tensor;
+    if (!arranged) return true;
+    const int64_t wgs = (rows + 63) / 64 * ((pairs + kArrangePairs - 1) / kArrangePairs);
+    if (wgs * 256 >= (int64_t(1) << 31)) return false;
+    job = ArrangeJob{tensor, room, rows, (int)wgs};
+    s.data = room;
+    room += arranged_bytes(rows, p.K);
+    return true;
+  };
+  if (!scales(p.xs, p.M, a) || !scales(p.ws, (int64_t)p.N * (p.gated ? 2 : 1) * (grouped ? p.G : 1), b)) return hipErrorInvalidValue;
+  if (listed || arranged) {
+    const int most = pairs < kArrangePairs ? pairs : kArrangePairs;
+    arrange_scales_kernel<<<(unsigned)(a.workgroups + b.workgroups + (listed ? 1 : 0)), 256, 64 * (most | 1) * 16, s>>>(a, b, tiles, from, pairs);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
-    p.xs = MxScales{xs, (int64_t)pairs * 1024, 16, 1024};
-    p.ws = MxScales{ws, (int64_t)pairs * 1024, 16, 1024};
-  } else {
-    p.xs = MxScales{p.xs.data, (int64_t)from * 64, from, 16};
-    p.ws = MxScales{p.ws.data, (int64_t)from * 64, from, 16};
   }
   if (way == kWalk) return p.out_f16 ? launch_walk<true>(p, s) : launch_walk<false>(p, s);
   return p.out_f16 ? launch_tiles<MxShape<64, 128, 2, 2, 4>, true>(p, s) : launch_tiles<MxShape<64, 128, 2, 2, 4>, false>(p, s);

@@ -79,6 +79,10 @@ struct MxLargeTile {
       const uint32_t sw = o.ws.offset(row + (up ? o.up_rows : 0));
       s_off[i] = wave < 2 ? sx : sw;
     }
+    // (one register each: formed by a 64-bit multiply-add they would keep both halves)
+#pragma unroll
+    for (int q = 0; q < 8; ++q) asm volatile("" : "+v"(x_off[q]), "+v"(w_off[q]));
+    asm volatile("" : "+v"(s_off[0]), "+v"(s_off[1]));
   }
   MSLK_AMD_DEVINL static int w_load_row(int wave, int q) { return (q >> 1) * 64 + (wave * 2 + (q & 1)) * 8; }
 
