@@ -35,7 +35,6 @@ struct MxProblem {
   uint16_t* y;
   const int64_t* m_sizes;
   const void* row_tiles;           // list of the groups' row tiles in device memory, nullptr without
-  int tile_rows;
   int M, N, K;                     // N: columns of Y
   int G;
   int bias_dtype;                  // 0 none, 1 fp32, 2 bf16

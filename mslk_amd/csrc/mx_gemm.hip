@@ -167,10 +167,11 @@ __global__ __launch_bounds__(TS::NTHREADS) void mx_kernel(MxProblem p, int tiles
   MxTile<TS, GATED> tile;
   tile.init(operands_of<GATED>(p, m0, rows, w_row, n0, COLUMNS));
   tile.run(lds, acc);
-  store_tile<TS::FM, TS::FN, TS::WN, TS::BM / TS::WM, 32, GATED, BIAS, F16, false>(p, acc, m0, rows, n0);
+  if (MxTile<TS, GATED>::turn_id() == 0)
+    store_tile<TS::FM, TS::FN, TS::WN, TS::BM / TS::WM, 32, GATED, BIAS, F16, false>(p, acc, m0, rows, n0);
 }
 
-// Row tiles: of p.tile_rows rows, or as listed in device memory.
+// Row tiles of at most 256 rows, as listed in device memory.
 struct RowTile { int row0, rows, group, unused; };
 
 // A workgroup per CU that walks the 256-column tiles.
@@ -203,7 +204,7 @@ __global__ __launch_bounds__(256) void mx_walk_kernel(MxProblem p, int tiles_m, 
       const RowTile r = list[1 + tm];
       return Place{r.row0, r.rows, tn * COLUMNS, (int64_t)r.group * p.N * (GATED ? 2 : 1)};
     }
-    return Place{tm * p.tile_rows, min(p.M - tm * p.tile_rows, p.tile_rows), tn * COLUMNS, 0};
+    return Place{tm * MxLarge::BM, min(p.M - tm * MxLarge::BM, MxLarge::BM), tn * COLUMNS, 0};
   };
   auto operands = [&](const Place& at) { return operands_of<GATED>(p, at.m0, at.rows, at.w_row, at.n0, COLUMNS); };
   Place at = place_of(t);
@@ -230,9 +231,9 @@ __global__ __launch_bounds__(256) void mx_walk_kernel(MxProblem p, int tiles_m, 
   wait_vmcnt0();   // the loads of a tile that does not follow end before the LDS is given away
 }
 
-// Tensors of scales, rows of `from` bytes, to the arranged layout (MxScales), of both operands in one launch.  A workgroup takes up to 32 pairs
+// Tensors of scales, rows of `from` bytes, to the arranged layout (MxScales), of both operands in one launch.  A workgroup takes up to 8 pairs
 // of 64 rows through LDS, so that it reads and writes whole lines; the first one makes the list of row tiles.
-constexpr int kArrangePairs = 32;
+constexpr int kArrangePairs = 8;
 struct ArrangeJob {
   const uint8_t* src;
   uint8_t* dst;
@@ -321,22 +322,28 @@ __global__ __launch_bounds__(256) void arrange_scales_kernel(ArrangeJob a, Arran
   const int slabs = (pairs + kArrangePairs - 1) / kArrangePairs, block = at / slabs, pair0 = (at - block * slabs) * kArrangePairs;
   const int n = min(pairs - pair0, kArrangePairs), rows = (int)min((int64_t)64, job.rows - (int64_t)block * 64);
   const int pitch = n | 1;
-  const uint32_t inverse = (65536u + (uint32_t)n - 1) / (uint32_t)n;   // i / n = i * inverse >> 16 for i < 64 n, n <= 32
+  const uint32_t inverse = (65536u + (uint32_t)n - 1) / (uint32_t)n;   // i / n = i * inverse >> 16 for i < 64 n, n <= 8
   const uint8_t* src = job.src + (int64_t)block * 64 * from + pair0 * 16;
-  for (int i = threadIdx.x; i < rows * n; i += 256) {
-    const int r = (int)(((uint32_t)i * inverse) >> 16), q = i - r * n, left = from - (pair0 + q) * 16;
+  uint4 v[kArrangePairs / 4];
+#pragma unroll
+  for (int t = 0; t < kArrangePairs / 4; ++t) {   // (all loads before the first store)
+    const int i = t * 256 + threadIdx.x, r = (int)(((uint32_t)i * inverse) >> 16), q = i - r * n, left = from - (pair0 + q) * 16;
     const uint8_t* in = src + (int64_t)r * from + q * 16;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (left >= 16) {
-      __builtin_memcpy(&v, in, 16);   // (rows begin anywhere)
-    } else {
+    v[t] = make_uint4(0, 0, 0, 0);
+    if (r < rows && left >= 16) {
+      __builtin_memcpy(&v[t], in, 16);   // (rows begin anywhere)
+    } else if (r < rows) {
       uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
       for (int e = 0; e < 16; ++e)
         if (e < left) w[e >> 2] |= (uint32_t)in[e] << (8 * (e & 3));
-      v = make_uint4(w[0], w[1], w[2], w[3]);
+      v[t] = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    piece[r * pitch + q] = v;
+  }
+#pragma unroll
+  for (int t = 0; t < kArrangePairs / 4; ++t) {
+    const int i = t * 256 + threadIdx.x, r = (int)(((uint32_t)i * inverse) >> 16), q = i - r * n;
+    if (r < rows) piece[r * pitch + q] = v[t];
   }
   __syncthreads();
   uint4* dst = reinterpret_cast<uint4*>(job.dst) + ((int64_t)block * pairs + pair0) * 64;
@@ -363,18 +370,24 @@ hipError_t launch_tiles(const MxProblem& p, hipStream_t s) {
   return hipGetLastError();
 }
 
-template <typename TS, bool F16>
-hipError_t launch_tiles(const MxProblem& p, hipStream_t s) {
-  if (p.m_sizes != nullptr) return p.gated ? launch_tiles<TS, true, true, false, F16>(p, s) : launch_tiles<TS, false, true, false, F16>(p, s);
-  if (p.gated) return launch_tiles<TS, true, false, false, F16>(p, s);
-  return p.bias_dtype != 0 ? launch_tiles<TS, false, false, true, F16>(p, s) : launch_tiles<TS, false, false, false, F16>(p, s);
+template <typename TS>
+hipError_t launch_dense(const MxProblem& p, hipStream_t s) {
+  if (p.gated) return p.out_f16 ? launch_tiles<TS, true, false, false, true>(p, s) : launch_tiles<TS, true, false, false, false>(p, s);
+  if (p.bias_dtype != 0) return p.out_f16 ? launch_tiles<TS, false, false, true, true>(p, s) : launch_tiles<TS, false, false, true, false>(p, s);
+  return p.out_f16 ? launch_tiles<TS, false, false, false, true>(p, s) : launch_tiles<TS, false, false, false, false>(p, s);
+}
+template <typename TS>
+hipError_t launch_groups(const MxProblem& p, hipStream_t s) {
+  if (p.gated) return p.out_f16 ? launch_tiles<TS, true, true, false, true>(p, s) : launch_tiles<TS, true, true, false, false>(p, s);
+  return p.out_f16 ? launch_tiles<TS, false, true, false, true>(p, s) : launch_tiles<TS, false, true, false, false>(p, s);
 }
 
 template <bool GATED, bool BIAS, bool F16>
 hipError_t launch_walk(const MxProblem& p, hipStream_t s) {
   constexpr int COLUMNS = GATED ? MxLarge::BN / 2 : MxLarge::BN;
+  if (p.K <= 256) return hipErrorInvalidValue;   // (the tiles load two steps ahead)
   const int64_t tiles_n = (p.N + COLUMNS - 1) / COLUMNS;
-  const int64_t tiles_m = p.row_tiles != nullptr ? most_row_tiles(p.M, p.G, p.tile_rows) : (p.M + p.tile_rows - 1) / p.tile_rows;
+  const int64_t tiles_m = p.row_tiles != nullptr ? most_row_tiles(p.M, p.G, MxLarge::BM) : (p.M + MxLarge::BM - 1) / MxLarge::BM;
   if (tiles_m * tiles_n >= (int64_t(1) << 31)) return hipErrorInvalidValue;
   const int64_t grid = (tiles_m * tiles_n + kXcds - 1) / kXcds * kXcds, cus = device_compute_units();
   mx_walk_kernel<GATED, BIAS, F16><<<(unsigned)(grid < cus ? grid : cus), MxLarge::NTHREADS, 0, s>>>(p, (int)tiles_m, (int)tiles_n);
@@ -387,36 +400,45 @@ hipError_t launch_walk(const MxProblem& p, hipStream_t s) {
   return p.bias_dtype != 0 ? launch_walk<false, true, F16>(p, s) : launch_walk<false, false, F16>(p, s);
 }
 
-constexpr int kFewRows = 64;
 enum Way : int {
-  kStream,   // few rows: mx_stream.hip
-  kTiles,    // 64 x 128 tiles
-  kWalk,     // 256-column tiles (at least two steps)
+  kStream,     // few rows: mx_stream.hip
+  k32x64, k64x64, k128x128,
+  k64x128,     // groups only
+  kWalk,       // 256-column tiles (at least two steps)
 };
-Way way_of(int64_t M, int64_t N, int64_t K, int gated, bool grouped) {
-  constexpr int kStreamTiles = 384;
-  if (!grouped && M <= 64 && N * (gated ? 2 : 1) <= 32 * kStreamTiles) return kStream;
-  return M <= 64 || K <= 256 || N >= (1 << 25) ? kTiles : kWalk;
+using Tile32x64 = MxShape<32, 64, 1, 1, 2, 4>;      // a workgroup per CU
+using Tile64x64 = MxShape<64, 64, 1, 1, 2, 2>;      // two
+using Tile64x128 = MxShape<64, 128, 2, 2, 2>;       // two
+using Tile128x128 = MxShape<128, 128, 2, 2, 2>;     // two
+
+// The smallest tiles of which each CU gets no more than it holds at once, since their steps' loads, not their products, are waited for.
+// At 8192 values (µs): 64 x 8192 32x64 11.1, 64x64 15.0, 128x128 25.7; 256 x 8192 64x64 22.0, 128x128 26.5, walk 30; 500 x 8192 128x128 29.0,
+// 64x64 40.6, walk 32.2; 1000 x 10240 walk 54, 128x128 64.9.
+// Up to 32 rows the weights stream past if there is a CU for every 32 columns (16 x 4096 x 14336 11.1 against 13.8; 16 x 10240 x 8192 14.8, 32x64 10.5).
+// Groups of few rows on average wait for weights, too: 64x128 tiles (16 groups of 256 rows, 2 x 5120 x 4096: 74.9, walk 79.4; 8 of 512 rows,
+// 4096 x 14336 77.3 and 102), but with a short K the walk, which has no gap between its tiles (128 of 512 rows, 2 x 768 x 2048: 35.5, 64x128 41.6).
+Way way_of(int64_t M, int64_t N, int64_t K, int gated, int64_t G, bool grouped) {
+  const int64_t cus = device_compute_units(), columns = N * (gated ? 2 : 1);
+  auto tiles = [&](int64_t bm, int64_t bn) { return (grouped ? most_row_tiles(M, G, bm) : (M + bm - 1) / bm) * ((columns + bn - 1) / bn); };
+  if (!grouped && M <= 32 && columns <= 32 * cus) return kStream;
+  if (!grouped && tiles(32, 64) <= cus) return k32x64;
+  if (tiles(64, 64) <= 2 * cus) return k64x64;
+  const bool short_k = K <= 256, wide = N >= (1 << 25);   // what the walk does not take
+  if (grouped) return M <= 64 || (M <= 64 * G && K >= 4096) || short_k || wide ? k64x128 : kWalk;
+  return tiles(128, 128) <= 2 * cus || short_k || wide ? k128x128 : kWalk;
 }
 
-// Whether the scales are arranged first.  Not where the product waits for the weights (few rows per group), if they can be fetched as they are.
+// Whether the scales are arranged first.  Not where the product waits for the weights (few rows, or few per group), if they can be fetched as they are.
 bool arranges(Way way, int64_t M, int64_t K, int G, bool grouped, bool scales_aligned) {
   if (K % 512 != 0 || !scales_aligned) return true;
-  return way == kWalk && !(grouped && M <= kFewRows * G);
-}
-
-// Rows of a row tile: as many as leave every CU a tile.
-int rows_of_tile(int64_t M, int64_t N, int gated) {
-  const int64_t tiles_n = (N * (gated ? 2 : 1) + 255) / 256, cus = device_compute_units();
-  if ((M + 255) / 256 * tiles_n > cus / 2) return 256;
-  return (M + 127) / 128 * tiles_n > cus / 2 ? 128 : 64;
+  return way == kWalk && M > 64 * (int64_t)(grouped ? G : 1);
 }
 
 }  // namespace
 
 size_t mx_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated, int G, bool grouped, bool scales_aligned) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  const Way way = way_of(M, N, K, gated, grouped);
+  const Way way = way_of(M, N, K, gated, G, grouped);
   if (way == kStream) return 0;
   const int64_t list = way == kWalk && grouped ? (1 + most_row_tiles(M, G, MxLarge::BM)) * (int64_t)sizeof(RowTile) : 0;
   if (!arranges(way, M, K, G, grouped, scales_aligned)) return (size_t)list;
@@ -425,10 +447,9 @@ size_t mx_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated, int G, boo
 
 hipError_t launch_mx_mm(MxProblem p, void* workspace, bool scales_aligned, hipStream_t s) {
   const bool grouped = p.m_sizes != nullptr;
-  const Way way = way_of(p.M, p.N, p.K, p.gated, grouped);
+  const Way way = way_of(p.M, p.N, p.K, p.gated, p.G, grouped);
   if (way == kStream) return launch_mx_stream(p, s);
   const int from = p.K / kMxBlock, pairs = (int)pairs_of(p.K);
-  p.tile_rows = grouped ? MxLarge::BM : rows_of_tile(p.M, p.N, p.gated);
   const bool listed = way == kWalk && grouped, arranged = p.K > 0 && arranges(way, p.M, p.K, p.G, grouped, scales_aligned);
   ArrangeJob a{}, b{};
   ListJob tiles{};
@@ -458,7 +479,9 @@ hipError_t launch_mx_mm(MxProblem p, void* workspace, bool scales_aligned, hipSt
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
   if (way == kWalk) return p.out_f16 ? launch_walk<true>(p, s) : launch_walk<false>(p, s);
-  return p.out_f16 ? launch_tiles<MxShape<64, 128, 2, 2, 4>, true>(p, s) : launch_tiles<MxShape<64, 128, 2, 2, 4>, false>(p, s);
+  if (way == k64x64) return grouped ? launch_groups<Tile64x64>(p, s) : launch_dense<Tile64x64>(p, s);
+  if (way == k64x128) return launch_groups<Tile64x128>(p, s);
+  return way == k32x64 ? launch_dense<Tile32x64>(p, s) : launch_dense<Tile128x128>(p, s);
 }
 
 }  // namespace mslk_amd

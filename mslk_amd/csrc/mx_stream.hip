@@ -1,6 +1,6 @@
 // Products of few rows of X with MXFP4 weights for gfx950 (formats: mx.h): the weights are read once, and they are what counts.
 //
-// A workgroup makes 32 columns (gated: 16, from 16 rows of the gate and their 16 partners) of up to 64 rows of X.  Its waves take K's
+// A workgroup makes 32 columns (gated: 16, from 16 rows of the gate and their 16 partners) of up to 32 rows of X.  Its waves take K's
 // pairs of steps, 512 values, in turn, each with a part of the LDS for itself: no barrier until their sums meet in LDS, and no sums
 // go through memory.  A wave asks for the rows of U pairs at once, 256 bytes of four rows per load (the 128-bit DMA load, mx_tile.h),
 // waits for them and multiplies.  (Loaded into registers as the instructions want them, 64 bytes of 16 rows at a time, a load takes the
@@ -24,12 +24,11 @@ MSLK_AMD_DEVINL int pair_swz(int r) { return (r & 3) | ((((r >> 2) ^ (r >> 3)) &
 template <int XR_, int WAVES_, int U_>
 struct StreamShape {
   static constexpr int XR = XR_, WAVES = WAVES_, U = U_;
-  static constexpr int MT = (XR + 31) / 32;                       // fragments of 32 rows
   static constexpr int W_BYTES = 32 * kPairBytes, X_BYTES = XR * kPairBytes;
   static constexpr int WAVE_BYTES = U * (W_BYTES + X_BYTES);
-  static constexpr int SUM_BYTES = WAVES * MT * 4096;             // behind the products, in the same place
+  static constexpr int SUM_BYTES = WAVES * 4096;                  // behind the products, in the same place
   static constexpr int LDS_BYTES = WAVES * WAVE_BYTES > SUM_BYTES ? WAVES * WAVE_BYTES : SUM_BYTES;
-  static_assert(XR % 4 == 0 && LDS_BYTES <= 160 * 1024, "whole loads, the LDS of a CU");
+  static_assert(XR % 4 == 0 && XR <= 32 && LDS_BYTES <= 160 * 1024, "whole loads, the LDS of a CU");
 };
 
 // Scales of this lane's eight chunks, 8 h ... 8 h + 7 of `blocks` (missing ones 0: products of two such blocks vanish).
@@ -49,7 +48,6 @@ MSLK_AMD_DEVINL uint2 load_scales8(const uint8_t* s, int blocks) {
 // Rows m0 ... m0 + rows - 1 (at most XR), columns from n0; w_row: first row of W's group.
 template <typename S, bool GATED>
 MSLK_AMD_DEVINL void stream_tile(const MxProblem& p, char* lds, int m0, int rows, int64_t w_row, int n0) {
-  constexpr int MT = S::MT;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 31, h = lane >> 5;
   const int64_t ld = p.K / 2, pitch = p.K / kMxBlock;
   const int blocks = p.K / kMxBlock, pairs = (blocks + 15) >> 4;
@@ -57,20 +55,16 @@ MSLK_AMD_DEVINL void stream_tile(const MxProblem& p, char* lds, int m0, int rows
   auto row_of_w = [&](int r) { return w_row + (GATED ? min(n0 + (r & 15), p.N - 1) + (int64_t)(r >> 4) * p.N : min(n0 + r, p.N - 1)); };
   auto row_of_x = [&](int r) { return (int64_t)m0 + min(r, rows - 1); };
   char* const mine = lds + wave * S::WAVE_BYTES;
-  const uint8_t *w_at[8], *x_at[S::XR / 4], *w_scale = p.ws.data + row_of_w(i) * pitch, *x_scale[MT];
+  const uint8_t *w_at[8], *x_at[S::XR / 4], *w_scale = p.ws.data + row_of_w(i) * pitch, *x_scale = p.xs.data + row_of_x(min(i, S::XR - 1)) * pitch;
 #pragma unroll
   for (int q = 0; q < 8; ++q) w_at[q] = p.wq + row_of_w(q * 4 + (lane >> 4)) * ld;
 #pragma unroll
   for (int q = 0; q < S::XR / 4; ++q) x_at[q] = p.xq + row_of_x(q * 4 + (lane >> 4)) * ld;
+  v16f acc;
 #pragma unroll
-  for (int tm = 0; tm < MT; ++tm) x_scale[tm] = p.xs.data + row_of_x(min(tm * 32 + i, S::XR - 1)) * pitch;
-  v16f acc[MT];
-#pragma unroll
-  for (int tm = 0; tm < MT; ++tm)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[tm][r] = 0.f;
+  for (int r = 0; r < 16; ++r) acc[r] = 0.f;
   for (int first = wave; first < pairs; first += S::U * S::WAVES) {
-    uint2 sw[S::U], sx[S::U][MT];
+    uint2 sw[S::U], sx[S::U];
 #pragma unroll
     for (int u = 0; u < S::U; ++u) {
       const int pair = min(first + u * S::WAVES, pairs - 1), there = blocks - pair * 16;   // (behind the last pair: it once more, not multiplied)
@@ -91,8 +85,7 @@ MSLK_AMD_DEVINL void stream_tile(const MxProblem& p, char* lds, int m0, int rows
         const int c = (lane & 15) ^ pair_swz(q * 4 + (lane >> 4));
         __builtin_amdgcn_global_load_lds((gbl_ptr_t)(x_at[q] + at + (c < there ? c * 16 : 0)), (lds_ptr_t)(mine + S::U * S::W_BYTES + u * S::X_BYTES + q * 1024), 16, 0, 0);
       }
-#pragma unroll
-      for (int tm = 0; tm < MT; ++tm) sx[u][tm] = load_scales8(x_scale[tm] + pair * 16, there);
+      sx[u] = load_scales8(x_scale + pair * 16, there);
     }
     __builtin_amdgcn_s_waitcnt(0x0F70);   // vmcnt(0): this wave's rows are in its part of the LDS
 #pragma unroll
@@ -103,34 +96,27 @@ MSLK_AMD_DEVINL void stream_tile(const MxProblem& p, char* lds, int m0, int rows
           constexpr int J = decltype(jj)::value;
           auto chunk = [&](const char* b, int r) { return *reinterpret_cast<const v4i*>(b + r * kPairBytes + (((8 * h + J) ^ pair_swz(r)) << 4)); };
           auto operand = [](v4i a) { return v8i{a[0], a[1], a[2], a[3], 0, 0, 0, 0}; };
-          const v4i wf = chunk(wb, i);
-#pragma unroll
-          for (int tm = 0; tm < MT; ++tm) {
-            const v4i xf = chunk(xb, min(tm * 32 + i, S::XR - 1));
-            acc[tm] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(wf), operand(xf), acc[tm], 4, 4, J & 3, (int)(J < 4 ? sw[u].x : sw[u].y),
-                                                                      J & 3, (int)(J < 4 ? sx[u][tm].x : sx[u][tm].y));
-          }
+          const v4i wf = chunk(wb, i), xf = chunk(xb, min(i, S::XR - 1));
+          acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(wf), operand(xf), acc, 4, 4, J & 3, (int)(J < 4 ? sw[u].x : sw[u].y), J & 3,
+                                                                (int)(J < 4 ? sx[u].x : sx[u].y));
         };
         product(Int<0>{}); product(Int<1>{}); product(Int<2>{}); product(Int<3>{});
         product(Int<4>{}); product(Int<5>{}); product(Int<6>{}); product(Int<7>{});
       }
     }
   }
-  // Row m = 32 tm + i of a wave's sums: 32 columns, in pieces of four (q, h) at piece ^ (i & 7).
+  // Row m = i of a wave's sums: 32 columns, in pieces of four (q, h) at piece ^ (i & 7).
   __syncthreads();
-  char* const sums = lds + wave * MT * 4096;
+  char* const sums = lds + wave * 4096;
 #pragma unroll
-  for (int tm = 0; tm < MT; ++tm)
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      *reinterpret_cast<float4*>(sums + (tm * 32 + i) * 128 + (((2 * q + h) ^ (i & 7)) << 4)) =
-          make_float4(acc[tm][4 * q], acc[tm][4 * q + 1], acc[tm][4 * q + 2], acc[tm][4 * q + 3]);
+  for (int q = 0; q < 4; ++q)
+    *reinterpret_cast<float4*>(sums + i * 128 + (((2 * q + h) ^ (i & 7)) << 4)) = make_float4(acc[4 * q], acc[4 * q + 1], acc[4 * q + 2], acc[4 * q + 3]);
   __syncthreads();
   auto total = [&](int m, int piece) {   // columns 4 piece ... of row m
     const char* at = lds + m * 128 + ((piece ^ (m & 7)) << 4);
     v4f s = *reinterpret_cast<const v4f*>(at);
 #pragma unroll
-    for (int k = 1; k < S::WAVES; ++k) s += *reinterpret_cast<const v4f*>(at + k * MT * 4096);
+    for (int k = 1; k < S::WAVES; ++k) s += *reinterpret_cast<const v4f*>(at + k * 4096);
     return s;
   };
   constexpr int PIECES = GATED ? 4 : 8;
@@ -186,8 +172,7 @@ hipError_t launch_mx_stream(const MxProblem& p, hipStream_t s) {
   if (grid * 512 >= (int64_t(1) << 32)) return hipErrorInvalidValue;
   if (p.M <= 8) return launch<StreamShape<8, 8, 2>>(p, (unsigned)grid, s);
   if (p.M <= 16) return launch<StreamShape<16, 8, 1>>(p, (unsigned)grid, s);
-  if (p.M <= 32) return launch<StreamShape<32, 8, 1>>(p, (unsigned)grid, s);
-  return launch<StreamShape<64, 6, 1>>(p, (unsigned)grid, s);
+  return launch<StreamShape<32, 8, 1>>(p, (unsigned)grid, s);
 }
 
 }  // namespace mslk_amd

@@ -31,21 +31,26 @@ namespace mslk_amd {
 
 constexpr int kMxStep = 128;          // bytes of a row per step
 
-// NS stages: NS - 1 steps are in flight while one is multiplied.
-template <int BM_, int BN_, int WM_, int WN_, int NS_>
+// KS = 1: WM x WN waves share a step's products; of NS stages NS - 1 are in flight while one is multiplied.
+// KS > 1, for small tiles, which would otherwise wait a memory round trip and a barrier for every step's few products: KS waves take the steps
+// in turn, each with NS stages and the whole tile's sums of its own.  A wave has a step in registers before it multiplies, and its stage takes
+// the step NS further: no barrier, NS steps in flight per wave.  At the end the sums meet in LDS.
+template <int BM_, int BN_, int WM_, int WN_, int NS_, int KS_ = 1>
 struct MxShape {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NS = NS_;
-  static constexpr int NW = WM * WN, NTHREADS = NW * 64;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NS = NS_, KS = KS_;
+  static constexpr int NW = WM * WN, NTHREADS = NW * KS * 64;       // waves that share a step
   static constexpr int FM = BM / WM / 32, FN = BN / WN / 32;        // fragments of 32 rows per wave
   static constexpr int X_BYTES = BM * kMxStep, W_BYTES = BN * kMxStep;
   static constexpr int LX = BM / 8 / NW, LW = BN / 8 / NW;          // DMA loads per wave and step
   // scales of two steps: DMA loads per wave (the rows of X, then of W, 64 rows a load; the last ones may have none)
-  static constexpr int LS = ((BM + BN + 63) / 64 + NW - 1) / NW;
+  static constexpr int S_X = (BM + 63) / 64 * 64, LS = ((S_X + BN) / 64 + NW - 1) / NW;
   static constexpr int S_BYTES = LS * NW * 1024;
-  static_assert(LS <= 2, "copy_scales()");
-  // A pair's place is taken again by the pair S_STAGES further, NS - 1 steps before that begins and after the last step of this one.
-  static constexpr int S_STAGES = (NS + 2) / 2;
-  static constexpr int LDS_BYTES = NS * (X_BYTES + W_BYTES) + S_STAGES * S_BYTES;
+  // KS = 1: a pair's place is taken again by the pair S_STAGES further, NS - 1 steps before that begins and after the last step of this one.
+  // KS > 1: a step's scales, and those of the other step of its pair, are loaded with it.
+  static constexpr int S_STAGES = KS == 1 ? (NS + 2) / 2 : NS;
+  static constexpr int PART_BYTES = NS * (X_BYTES + W_BYTES) + S_STAGES * S_BYTES;   // of the waves that share steps
+  static constexpr int LDS_BYTES = KS * PART_BYTES;
+  static_assert(KS == 1 || NW == 1, "steps are shared, or taken in turn");
   static_assert(BM % (32 * WM) == 0 && BN % (64 * WN) == 0 && BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && (BM + BN) % 32 == 0, "whole fragments and loads");
   static_assert(LDS_BYTES <= 160 * 1024, "LDS of a CU");
 };
@@ -84,7 +89,9 @@ struct MxTile {
   uint32_t s_off[TS::LS];                  // of this lane's 16 bytes of scales, relative to xs or ws
   MxOperands o;
 
-  MSLK_AMD_DEVINL static int wave_id() { return __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
+  // Of a wave: its place among those that share a step, and which step of KS it takes.
+  MSLK_AMD_DEVINL static int wave_id() { return TS::KS == 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0; }
+  MSLK_AMD_DEVINL static int turn_id() { return TS::KS == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); }
 
   // Row of the tile that LDS row r of X holds.
   MSLK_AMD_DEVINL static int x_row(int r) { return ((r >> 5) % TS::WM) * (TS::BM / TS::WM) + r / (32 * TS::WM) * 32 + (r & 31); }
@@ -120,13 +127,13 @@ struct MxTile {
     }
 #pragma unroll
     for (int i = 0; i < TS::LS; ++i) {   // the list of LDS rows of X, then of W
-      const int r = min((wave * TS::LS + i) * 64 + lane, TS::BM + TS::BN - 1);
+      const int r = (wave * TS::LS + i) * 64 + lane;
       bool up = false;
-      if (r >= TS::BM) {
-        const int row = min(w_row(r - TS::BM, up), o.rows_w - 1);
+      if (r >= TS::S_X) {
+        const int row = min(w_row(min(r - TS::S_X, TS::BN - 1), up), o.rows_w - 1);
         s_off[i] = o.ws.offset(row + (up ? (int)o.up_rows : 0));
       } else {
-        s_off[i] = o.xs.offset(min(x_row(r), o.rows_x - 1));
+        s_off[i] = o.xs.offset(min(x_row(min(r, TS::BM - 1)), o.rows_x - 1));
       }
     }
   }
@@ -143,31 +150,28 @@ struct MxTile {
     const int chunks = kt + 1 < o.steps ? 8 : o.last_chunks;
     return Adjust{c < chunks ? 0u : (uint32_t)(-16 * c), (c ^ 4) < chunks ? 0u : (uint32_t)(-16 * (c ^ 4))};
   }
-  // Load i of the scales of steps 2 pair and 2 pair + 1 into the place of `pair`; behind the last pair, the last one's again.
-  MSLK_AMD_DEVINL void copy_scales(char* lds, int pair, int i) {
-    const int64_t from = (int64_t)min(pair, (o.steps - 1) >> 1) * o.xs.pair_stride;   // (the same for both)
+  // Load i of the scales of steps 2 pair and 2 pair + 1 into `stage`.
+  MSLK_AMD_DEVINL void copy_scales(char* stage, int pair, int i) {
+    const int64_t from = (int64_t)pair * o.xs.pair_stride;   // (the same for both)
     const int wave = wave_id();
-    const uint32_t off = TS::LS == 1 || i == 0 ? s_off[0] : s_off[TS::LS - 1];   // (an index that is no constant would put the array in memory)
-    char* dst = s_stage(lds, pair % TS::S_STAGES) + (wave * TS::LS + i) * 1024;
-    if constexpr (TS::BM % 64 == 0) {
-      dma16(uniform_ptr(((wave * TS::LS + i) * 64 >= TS::BM ? o.ws.base : o.xs.base) + from), off, dst);
-    } else {   // rows of both operands in one load: one for each
-      if ((wave * TS::LS + i) * 64 + (int)(threadIdx.x & 63) >= TS::BM) dma16(o.ws.base + from, off, dst);
-      else dma16(o.xs.base + from, off, dst);
-    }
+    char* dst = stage + (wave * TS::LS + i) * 1024;
+    dma16(uniform_ptr(((wave * TS::LS + i) * 64 >= TS::S_X ? o.ws.base : o.xs.base) + from), s_off[i], dst);
   }
 
   // At most `PENDING` of this wave's youngest loads are in flight and its LDS accesses are done; then the workgroup's barrier.
-  template <int PENDING>
+  template <int PENDING, bool BARRIER = true>
   MSLK_AMD_DEVINL static void wait_and_barrier() {
     static_assert(PENDING >= 0 && PENDING < 64, "vmcnt is a 6-bit counter");
     __builtin_amdgcn_sched_barrier(0);
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_waitcnt(0x0070 | (PENDING & 15) | ((PENDING >> 4) << 14));
-    __builtin_amdgcn_s_barrier();
+    if constexpr (BARRIER) __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   }
+
+  template <int PENDING>
+  MSLK_AMD_DEVINL static void wait() { wait_and_barrier<PENDING, false>(); }
 
   // Chunk 4 h + j of this lane's row of a fragment of 32 W rows at `rows`; w: of the W waves that share it, this one.
   MSLK_AMD_DEVINL static v4i chunk(const char* rows, int w, int j) {
@@ -176,20 +180,20 @@ struct MxTile {
   }
   MSLK_AMD_DEVINL static v4i x_chunk(const char* stage, int tm, int j) { return chunk(stage + tm * (32 * TS::WM * kMxStep), wave_id() / TS::WN, j); }
   MSLK_AMD_DEVINL static v4i w_chunk(const char* stage, int tn, int j) { return chunk(stage + tn * (32 * TS::WN * kMxStep), wave_id() % TS::WN, j); }
-  MSLK_AMD_DEVINL static void load_scales(char* lds, int kt, uint32_t (&sx)[TS::FM], uint32_t (&sw)[TS::FN]) {
+  MSLK_AMD_DEVINL static void load_scales(const char* stage, int kt, uint32_t (&sx)[TS::FM], uint32_t (&sw)[TS::FN]) {
     const int lane = threadIdx.x & 63, wave = wave_id();
-    const char* at = s_stage(lds, (kt >> 1) % TS::S_STAGES) + (kt & 1) * 8 + (lane >> 5) * 4 + (lane & 31) * 16;
+    const char* at = stage + (kt & 1) * 8 + (lane >> 5) * 4 + (lane & 31) * 16;
 #pragma unroll
     for (int tm = 0; tm < TS::FM; ++tm) sx[tm] = *reinterpret_cast<const uint32_t*>(at + (tm * TS::WM + wave / TS::WN) * 512);
 #pragma unroll
-    for (int tn = 0; tn < TS::FN; ++tn) sw[tn] = *reinterpret_cast<const uint32_t*>(at + TS::BM * 16 + (tn * TS::WN + wave % TS::WN) * 512);
+    for (int tn = 0; tn < TS::FN; ++tn) sw[tn] = *reinterpret_cast<const uint32_t*>(at + TS::S_X * 16 + (tn * TS::WN + wave % TS::WN) * 512);
   }
   template <int J>
   MSLK_AMD_DEVINL static void multiply(const v4i& wf, const v4i& xf, uint32_t sw, uint32_t sx, v16f& acc) {
     acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(wf), mx_operand(xf), acc, 4, 4, J, (int)sw, J, (int)sx);
   }
 
-  // acc = the tile's sums.  Ends with a barrier: LDS is free.
+  // acc (KS > 1: of the first wave) = the tile's sums.
   MSLK_AMD_DEVINL void run(char* lds, v16f (&acc)[TS::FN][TS::FM]) {
 #pragma unroll
     for (int tn = 0; tn < TS::FN; ++tn)
@@ -197,34 +201,19 @@ struct MxTile {
       for (int tm = 0; tm < TS::FM; ++tm)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[tn][tm][r] = 0.f;
-    run_ring(lds, acc);
-    wait_and_barrier<0>();
+    if constexpr (TS::KS == 1) {
+      run_ring(lds, acc);
+    } else {
+      run_alone(lds + turn_id() * TS::PART_BYTES, acc);
+      add_sums(lds, acc);
+    }
   }
 
-  // The loads of step kt into stage `at`, in front of them those of a pair's scales.
-  MSLK_AMD_DEVINL void issue(char* lds, int kt, int at) {
-    if ((kt & 1) == 0) {
-#pragma unroll
-      for (int i = 0; i < TS::LS; ++i) copy_scales(lds, kt >> 1, i);
-    }
-    const Adjust a = adjust(kt);
-    const uint8_t *x = o.x + (int64_t)kt * kMxStep, *w = o.w + (int64_t)kt * kMxStep;
-#pragma unroll
-    for (int q = 0; q < TS::LX; ++q) {
-      const int r = x_load_row(q);
-      dma16(x, x_off[q] + ((r >> 3) & 1 ? a.odd : a.even), x_stage(lds, at) + r * kMxStep);
-    }
-#pragma unroll
-    for (int q = 0; q < TS::LW; ++q) {
-      const int r = w_load_row(q);
-      dma16(w, w_off[q] + ((r >> 3) & 1 ? a.odd : a.even), w_stage(lds, at) + r * kMxStep);
-    }
-  }
+  // KS = 1.
   MSLK_AMD_DEVINL void run_ring(char* lds, v16f (&acc)[TS::FN][TS::FM]) {
-    constexpr int D = TS::NS - 1, PER = TS::LX + TS::LW;
     // In flight behind the loads of a step when its turn comes: those of the D - 1 steps after it, and of the scales of at least
     // (D - 1) / 2 pairs (a pair's scales go in front of its first step's codes).
-    constexpr int PENDING = (D - 1) * PER + (D - 1) / 2 * TS::LS;
+    constexpr int D = TS::NS - 1, PENDING = (D - 1) * (TS::LX + TS::LW) + (D - 1) / 2 * TS::LS;
     for (int kt = 0; kt < D && kt < o.steps; ++kt) issue(lds, kt, kt);
     int at = 0;
     for (int kt = 0; kt < o.steps; ++kt) {
@@ -234,7 +223,7 @@ struct MxTile {
       if (kt + D < o.steps) issue(lds, kt + D, at == 0 ? TS::NS - 1 : at - 1);
       const char *x = x_stage(lds, at), *w = w_stage(lds, at);
       uint32_t sx[TS::FM], sw[TS::FN];
-      load_scales(lds, kt, sx, sw);
+      load_scales(s_stage(lds, (kt >> 1) % TS::S_STAGES), kt, sx, sw);
       auto product = [&](auto j) {
         constexpr int J = decltype(j)::value;
         v4i xf[TS::FM];
@@ -252,6 +241,88 @@ struct MxTile {
       product(std::integral_constant<int, 2>{});
       product(std::integral_constant<int, 3>{});
       at = at + 1 == TS::NS ? 0 : at + 1;
+    }
+  }
+
+  // KS > 1: the steps of this wave, in its part of the LDS.
+  MSLK_AMD_DEVINL void run_alone(char* mine, v16f (&acc)[TS::FN][TS::FM]) {
+    constexpr int PENDING = (TS::NS - 1) * (TS::LX + TS::LW + TS::LS);
+    const int first = turn_id(), turns = (o.steps - first + TS::KS - 1) / TS::KS;
+    for (int t = 0; t < TS::NS && t < turns; ++t) issue(mine, first + t * TS::KS, t);
+    int at = 0;
+    for (int t = 0; t < turns; ++t) {
+      if (t + TS::NS - 1 < turns) wait<PENDING>();
+      else wait<0>();
+      const int kt = first + t * TS::KS;
+      const char *x = x_stage(mine, at), *w = w_stage(mine, at);
+      v4i xf[TS::FM][4], wf[TS::FN][4];
+      uint32_t sx[TS::FM], sw[TS::FN];
+      load_scales(s_stage(mine, at), kt, sx, sw);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int tm = 0; tm < TS::FM; ++tm) xf[tm][j] = x_chunk(x, tm, j);
+#pragma unroll
+        for (int tn = 0; tn < TS::FN; ++tn) wf[tn][j] = w_chunk(w, tn, j);
+      }
+      wait<63>();   // for the reads: the stage is free
+      if (t + TS::NS < turns) issue(mine, kt + TS::NS * TS::KS, at);
+      auto product = [&](auto j) {
+        constexpr int J = decltype(j)::value;
+#pragma unroll
+        for (int tn = 0; tn < TS::FN; ++tn)
+#pragma unroll
+          for (int tm = 0; tm < TS::FM; ++tm) multiply<J>(wf[tn][J], xf[tm][J], sw[tn], sx[tm], acc[tn][tm]);
+      };
+      product(std::integral_constant<int, 0>{});
+      product(std::integral_constant<int, 1>{});
+      product(std::integral_constant<int, 2>{});
+      product(std::integral_constant<int, 3>{});
+      at = at + 1 == TS::NS ? 0 : at + 1;
+    }
+  }
+
+  // The loads of step kt into stage `at`, in front of them those of scales.
+  MSLK_AMD_DEVINL void issue(char* mine, int kt, int at) {
+    if (TS::KS > 1 || (kt & 1) == 0) {
+#pragma unroll
+      for (int i = 0; i < TS::LS; ++i) copy_scales(s_stage(mine, TS::KS == 1 ? (kt >> 1) % TS::S_STAGES : at), kt >> 1, i);
+    }
+    const Adjust a = adjust(kt);
+    const uint8_t *x = o.x + (int64_t)kt * kMxStep, *w = o.w + (int64_t)kt * kMxStep;
+#pragma unroll
+    for (int q = 0; q < TS::LX; ++q) {
+      const int r = x_load_row(q);
+      dma16(x, x_off[q] + ((r >> 3) & 1 ? a.odd : a.even), x_stage(mine, at) + r * kMxStep);
+    }
+#pragma unroll
+    for (int q = 0; q < TS::LW; ++q) {
+      const int r = w_load_row(q);
+      dma16(w, w_off[q] + ((r >> 3) & 1 ? a.odd : a.even), w_stage(mine, at) + r * kMxStep);
+    }
+  }
+
+  // KS > 1: the first wave's sums become those of all, through LDS: [wave - 1][fragment][register][lane].
+  MSLK_AMD_DEVINL static void add_sums(char* lds, v16f (&acc)[TS::FN][TS::FM]) {
+    constexpr int SUMS = TS::BM * TS::BN;
+    static_assert((TS::KS - 1) * SUMS * 4 <= TS::LDS_BYTES, "room for the sums");
+    float* const at = reinterpret_cast<float*>(lds) + (threadIdx.x & 63);
+    const int wave = turn_id();
+    wait_and_barrier<0>();   // nobody reads or fills stages any more
+    if (wave > 0) {
+#pragma unroll
+      for (int f = 0; f < TS::FN * TS::FM; ++f)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) at[(wave - 1) * SUMS + (f * 16 + r) * 64] = acc[f / TS::FM][f % TS::FM][r];
+    }
+    __syncthreads();
+    if (wave == 0) {
+#pragma unroll
+      for (int k = 0; k < TS::KS - 1; ++k)
+#pragma unroll
+        for (int f = 0; f < TS::FN * TS::FM; ++f)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[f / TS::FM][f % TS::FM][r] += at[k * SUMS + (f * 16 + r) * 64];
     }
   }
 };
