@@ -174,11 +174,11 @@ __global__ __launch_bounds__(TS::NTHREADS) void mx_kernel(MxProblem p, int tiles
 // Row tiles of at most 256 rows, as listed in device memory.
 struct RowTile { int row0, rows, group, unused; };
 
-// A workgroup per CU that walks the 256-column tiles.
-// One matrix: XCD x keeps a run of neighbouring entries of the list, its workgroups take them in turn: the XCDs then ask for the same weights at
-// about the same time, and the Infinity Cache serves all but the first (dealt in rounds as below, 8192 x 28672 x 4096 takes 686 us instead of 490).
-// Groups: in rounds; of each round's entries, neighbours all, XCD x takes a run.  The list has long tiles first, so those of a round are about
-// as long, where runs of the whole list leave the XCDs different amounts (16 experts of 8192 rows 236 us instead of 225).
+// A workgroup per CU that walks the 256-column tiles, in rounds: of each round's entries, neighbours all, XCD x takes a run.  (A list has long
+// tiles first, so those of a round are about as long; runs of the whole list leave the XCDs different amounts, 16 experts of 8192 rows 236 us
+// instead of 225, and equal ones gain nothing: 8192 x 28672 x 4096 521 and 515.)
+// One matrix: tiles of a last round that half of the workgroups would be enough for are cut into two of 128 rows (2048 x 10240 x 8192 114 us, 100).
+// A list's last tiles are short already (cut, 16 experts of 8192 rows take 2 % more).
 template <bool GATED, bool BIAS, bool F16>
 __global__ __launch_bounds__(256) void mx_walk_kernel(MxProblem p, int tiles_m, int tiles_n) {
   using TS = MxLarge;
@@ -187,34 +187,43 @@ __global__ __launch_bounds__(256) void mx_walk_kernel(MxProblem p, int tiles_m, 
   constexpr int COLUMNS = GATED ? TS::BN / 2 : TS::BN;
   const RowTile* const list = static_cast<const RowTile*>(p.row_tiles);
   if (list != nullptr) tiles_m = list[0].rows;   // (the first entry holds their number)
-  const int total = tiles_m * tiles_n, wgs = gridDim.x, xcd = blockIdx.x % kXcds, slot = blockIdx.x / kXcds;
+  const int wgs = gridDim.x, xcd = blockIdx.x % kXcds, slot = blockIdx.x / kXcds;
+  const int whole = tiles_m * tiles_n / wgs * wgs, rest = tiles_m * tiles_n - whole;
+  const bool cut = list == nullptr && 2 * rest <= wgs;
+  const int total = cut ? whole + 2 * rest : whole + rest;
   auto entry = [&](int round) {   // this workgroup's `round`th entry, -1: none
-    const int first = list != nullptr ? round * wgs : 0, here = list != nullptr ? min(total - first, wgs) : total;
-    const int run = (here + kXcds - 1) / kXcds, in_run = list != nullptr ? slot : slot + round * (wgs / kXcds), at = xcd * run + in_run;
-    return in_run < run && at < here ? first + at : -1;
+    const int first = round * wgs, here = min(total - first, wgs), run = (here + kXcds - 1) / kXcds, at = xcd * run + slot;
+    return slot < run && at < here ? first + at : -1;
   };
-  int t = entry(0), round = 0;
-  if (t < 0) return;
   const bool aligned = (p.N & 7) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 15) == 0 && (!BIAS || (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0);
   struct Place { int m0, rows, n0; int64_t w_row; };
-  auto place_of = [&](int t) {
+  auto place_of = [&](int t, Place& at) {   // false: none, or the empty half of a tile
+    if (t < 0) return false;
+    const bool part = cut && t >= whole;
+    const int half = part ? (t - whole) & 1 : 0;
+    if (part) t = whole + ((t - whole) >> 1);
     int tm, tn;
     tile_at(t, tiles_m, tiles_n, tm, tn);
     if (list != nullptr) {
       const RowTile r = list[1 + tm];
-      return Place{r.row0, r.rows, tn * COLUMNS, (int64_t)r.group * p.N * (GATED ? 2 : 1)};
+      at = Place{r.row0, r.rows, tn * COLUMNS, (int64_t)r.group * p.N * (GATED ? 2 : 1)};
+      return true;
     }
-    return Place{tm * MxLarge::BM, min(p.M - tm * MxLarge::BM, MxLarge::BM), tn * COLUMNS, 0};
+    const int m0 = tm * MxLarge::BM + half * 128;
+    if (m0 >= p.M) return false;
+    at = Place{m0, min(p.M - m0, part ? 128 : MxLarge::BM), tn * COLUMNS, 0};
+    return true;
   };
   auto operands = [&](const Place& at) { return operands_of<GATED>(p, at.m0, at.rows, at.w_row, at.n0, COLUMNS); };
-  Place at = place_of(t);
+  int round = 0;
+  Place at;
+  if (!place_of(entry(0), at)) return;
   Tile tile;
   typename Tile::Held held;
   tile.start(lds, operands(at), held);
-  for (;;) {
+  for (bool more = true; more;) {
     const Place here = at;
-    t = entry(++round);
-    if (t >= 0) at = place_of(t);   // (behind the last tile: itself once more)
+    more = place_of(entry(++round), at);   // (behind the last tile: itself once more)
     auto make = [&](auto fragments) {
       constexpr int F = decltype(fragments)::value;
       v16f acc[4][F];
@@ -226,7 +235,6 @@ __global__ __launch_bounds__(256) void mx_walk_kernel(MxProblem p, int tiles_m, 
     else if (here.rows > 128) make(std::integral_constant<int, 3>{});
     else if (here.rows > 64) make(std::integral_constant<int, 2>{});
     else make(std::integral_constant<int, 1>{});
-    if (t < 0) break;
   }
   wait_vmcnt0();   // the loads of a tile that does not follow end before the LDS is given away
 }
@@ -388,8 +396,8 @@ hipError_t launch_walk(const MxProblem& p, hipStream_t s) {
   if (p.K <= 256) return hipErrorInvalidValue;   // (the tiles load two steps ahead)
   const int64_t tiles_n = (p.N + COLUMNS - 1) / COLUMNS;
   const int64_t tiles_m = p.row_tiles != nullptr ? most_row_tiles(p.M, p.G, MxLarge::BM) : (p.M + MxLarge::BM - 1) / MxLarge::BM;
-  if (tiles_m * tiles_n >= (int64_t(1) << 31)) return hipErrorInvalidValue;
-  const int64_t grid = (tiles_m * tiles_n + kXcds - 1) / kXcds * kXcds, cus = device_compute_units();
+  if (tiles_m * tiles_n >= (int64_t(1) << 30)) return hipErrorInvalidValue;
+  const int64_t grid = (2 * tiles_m * tiles_n + kXcds - 1) / kXcds * kXcds, cus = device_compute_units();
   mx_walk_kernel<GATED, BIAS, F16><<<(unsigned)(grid < cus ? grid : cus), MxLarge::NTHREADS, 0, s>>>(p, (int)tiles_m, (int)tiles_n);
   return hipGetLastError();
 }
