@@ -271,6 +271,82 @@ def test_leading_dimensions_torch_types_and_views():
     same_bits(one, want[0, 0])
 
 
+# Sizes for each kind of tile, beside those of few rows above (on 256 CUs): 32 x 64 and 64 x 64 tiles whose waves take the steps in turn, with
+# fewer steps than waves, as many and some more; 128 x 128 tiles; 256-column tiles in less than a round, in a last one that is cut in two (the
+# last rows have no second half), with 64, 128, 192 and 256 rows in the last tile.  K from one step to several, whole ones and not.
+TILED = [(5, 9000, 288), (32, 8200, 96), (40, 2000, 1280), (128, 1024, 2336), (70, 64, 4096), (1, 64, 2048),
+         (520, 1100, 32), (520, 1104, 512), (513, 1100, 800), (33, 20000, 1056),
+         (1100, 2000, 224), (1100, 2000, 512), (1025, 2056, 1312), (1, 40000, 64), (2600, 7000, 256),
+         (1500, 6000, 288), (1472, 6144, 512), (2600, 7000, 544), (4100, 4200, 800), (4240, 4096, 1024), (4050, 4360, 1056), (3, 70000, 512), (40, 66000, 320)]
+
+
+@pytest.mark.parametrize("m,n,k", TILED)
+def test_product_exact_with_every_tile(m, n, k):
+    g = rng(m + n + k)
+    xq, xs = operand(m, k, g)
+    wq, ws = operand(n, k, g)
+    want, _ = O.product(xq, wq, xs, ws)   # (sums of K products of at most 36 x 4: below 2^20)
+    args = gpu(xq, wq, xs, ws)
+    same_bits(mslk_amd.mxfp4_mm(*args), want)
+    for bias_dtype, out_dtype in ((F32, F16), (BF16, BF16)):
+        bias = torch.randint(-64, 65, (n,), generator=g).to(bias_dtype)
+        same_bits(mslk_amd.mxfp4_mm(*args, bias=bias.to(DEV), out_dtype=out_dtype), want + bias.double(), "bias")
+    if n % 2 == 0:
+        halves = args[3].view(2, n // 2, -1)
+        halves -= 7
+        want, (gate, up, _, _) = O.gated(xq, wq, xs, ws - 7)
+        within(mslk_amd.mxfp4_gated_mm(*args), want, (2.0 ** -20 + gate.abs() * 2.0 ** -22) * want.abs() + 1e-37, "gated")
+
+
+@pytest.mark.parametrize("m,n,k", [(40, 2000, 1024), (520, 1104, 512), (1100, 2000, 544), (2600, 7000, 512)])
+def test_unaligned_results_bias_and_scales(m, n, k):
+    """Addresses that are no multiple of 16 bytes, of everything but the codes, through the C interface."""
+    L = _lib.lib()
+    g = rng(m + k)
+    xq, xs = operand(m, k, g)
+    wq, ws = operand(n, k, g)
+    bias = torch.randint(-9, 10, (n,), generator=g).to(BF16)
+    want, _ = O.product(xq, wq, xs, ws)
+
+    def moved(t, by):
+        flat = torch.zeros(t.numel() + by, dtype=t.dtype, device=DEV)
+        flat[by:] = t.flatten().to(DEV)
+        return flat[by:]
+
+    xs_at, ws_at, bias_at = moved(xs, 1), moved(ws, 3), moved(bias, 1)
+    held = torch.full((m * n + 2,), 77.0, dtype=BF16, device=DEV)
+    y = held[1:]
+    room = L.mslk_amd_mxfp4_mm_workspace_bytes(m, n, k, 0, 0)
+    space = torch.empty(max(room, 16), dtype=torch.uint8, device=DEV)
+    args = gpu(xq, wq)
+    _lib.check(L.mslk_amd_mxfp4_mm(args[0].data_ptr(), args[1].data_ptr(), xs_at.data_ptr(), ws_at.data_ptr(), bias_at.data_ptr(), 2, 0, y.data_ptr(), 0, m, n,
+                                   k, space.data_ptr(), space.numel(), torch.cuda.current_stream().cuda_stream))
+    torch.cuda.synchronize()
+    same_bits(y[:-1].view(m, n), want + bias.double())
+    assert held[0] == 77 and held[-1] == 77
+
+
+@pytest.mark.parametrize("m,n,k", [(100, 2000, 4096), (520, 1104, 5152), (1100, 2000, 2080), (1472, 6144, 1056)])
+def test_wide_scales_with_every_tile(m, n, k):
+    g = rng(m + n + k)
+    xq, xs = operand(m, k, g, 117, 134)
+    wq, ws = operand(n, k, g, 110, 125)
+    want, size = O.product(xq, wq, xs, ws)
+    within(mslk_amd.mxfp4_mm(*gpu(xq, wq, xs, ws)), want, (k / 64 + 64) * 2.0 ** -23 * size)
+
+
+@pytest.mark.parametrize("m,n,k", [(520, 1100, 288), (1100, 2000, 544), (2600, 7000, 288)])
+def test_nan_scales_with_every_tile(m, n, k):
+    g = rng(k)
+    xq, xs = operand(m, k, g)
+    wq, ws = operand(n, k, g)
+    xs[m - 1, -1] = 255
+    ws[n // 2, 0] = 255
+    wq[n // 2] = 0
+    want, _ = O.product(xq, wq, xs, ws)
+    same_bits(mslk_amd.mxfp4_mm(*gpu(xq, wq, xs, ws)), want)
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # experts
 # ---------------------------------------------------------------------------------------------------------------------
@@ -303,6 +379,39 @@ def test_experts(sizes, n, k, gated):
     within(got, want, 2.0 ** -17 * want.abs() + 1e-37)   # gates of at most a few hundred: see test_gated
     each = torch.cat([mslk_amd.mxfp4_gated_mm(*gpu(x, wq[e], s, ws[e])) for e, (x, s) in enumerate(zip(xq.split(sizes), xs.split(sizes))) if len(x)])
     assert torch.equal(got, each)
+
+
+# Tiles of 64 x 128 (few rows, a K of one step) and the walk over a list of row tiles: more groups than a wave and a workgroup have lanes,
+# row tiles of every number of fragments, groups of no rows at both ends, several rounds.
+TILED_SIZES = [([1, 0, 3, 0] * 10, 900, 288), ([300, 1, 0, 256, 257, 2], 2000, 160), ([300, 1, 0, 256, 257, 2], 2000, 288), ([0] * 70 + [3, 0, 130] + [1] * 70, 400, 512),
+               ([1, 0, 2, 0, 0, 1] * 50, 200, 544), ([0, 64, 65, 128, 129, 192, 193, 255, 256, 257, 0], 2000, 512), ([2000, 0, 1500, 513], 4096, 768),
+               ([20, 0, 9, 1], 8320, 4096)]
+
+
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("sizes,n,k", TILED_SIZES, ids=lambda v: f"{len(v)}x{sum(v)}" if isinstance(v, list) else str(v))
+def test_experts_with_every_tile(sizes, n, k, gated):
+    n = n // 2 if gated else n
+    g = rng(len(sizes) + n)
+    xq, xs = operand(sum(sizes), k, g)
+    wq, ws = operand((len(sizes), 2 * n if gated else n), k, g)
+    if gated:
+        ws -= 7
+    want = grouped_oracle(xq, wq, xs, ws, sizes, gated)
+    args = gpu(xq, wq, xs, ws)
+    counts = torch.tensor(sizes, device=DEV)
+    got = mslk_amd.mxfp4_grouped_mm(*args, counts, gated=gated)
+    if gated:
+        within(got, want, 2.0 ** -17 * want.abs() + 1e-37)
+    else:
+        same_bits(got, want)
+    assert torch.equal(mslk_amd.mxfp4_grouped_mm(*args, counts, gated=gated), got)
+
+
+def test_no_experts():
+    xq, xs = gpu(*operand(5, 64, rng(2)))
+    wq, ws = gpu(*operand((0, 6), 64, rng(2)))
+    assert mslk_amd.mxfp4_grouped_mm(xq, wq, xs, ws, torch.zeros(0, dtype=torch.int64, device=DEV)).shape == (5, 6)
 
 
 def call_grouped(xq, wq, xs, ws, sizes, y, gated=False):
