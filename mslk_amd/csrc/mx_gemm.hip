@@ -436,9 +436,12 @@ Way way_of(int64_t M, int64_t N, int64_t K, int gated, int64_t G, bool grouped) 
   return tiles(128, 128) <= 2 * cus || short_k || wide ? k128x128 : kWalk;
 }
 
-// Whether the scales are arranged first.  Not where the product waits for the weights (few rows, or few per group), if they can be fetched as they are.
+// Whether the scales are arranged first.  Not where the product waits for the weights (few rows, or few per group) or has few steps, if they can
+// be fetched as they are: 128 x 128 tiles gain 0.1 to 0.27 us per step of the 500 to 2048 x 4096 to 10240 that were looked at, and the launch in
+// front takes 2.5 (K = 4096 21.6 us, arranged 22.8; K = 12288 55.7 and 51.0).
 bool arranges(Way way, int64_t M, int64_t K, int G, bool grouped, bool scales_aligned) {
   if (K % 512 != 0 || !scales_aligned) return true;
+  if (way == k128x128) return K >= 6144;
   return way == kWalk && M > 64 * (int64_t)(grouped ? G : 1);
 }
 

@@ -32,9 +32,9 @@ namespace mslk_amd {
 constexpr int kMxStep = 128;          // bytes of a row per step
 
 // KS = 1: WM x WN waves share a step's products; of NS stages NS - 1 are in flight while one is multiplied.
-// KS > 1, for small tiles, which would otherwise wait a memory round trip and a barrier for every step's few products: KS waves take the steps
-// in turn, each with NS stages and the whole tile's sums of its own.  A wave has a step in registers before it multiplies, and its stage takes
-// the step NS further: no barrier, NS steps in flight per wave.  At the end the sums meet in LDS.
+// KS > 1, for small tiles, which would otherwise wait a memory round trip and a barrier for every step's few products: KS waves take the pairs of
+// steps in turn, each with two stages and the whole tile's sums of its own.  A wave has a step in registers before it multiplies, and its stage
+// takes the one after the next: no barrier, two steps in flight per wave.  At the end the sums meet in LDS.
 template <int BM_, int BN_, int WM_, int WN_, int NS_, int KS_ = 1>
 struct MxShape {
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NS = NS_, KS = KS_;
@@ -45,12 +45,11 @@ struct MxShape {
   // scales of two steps: DMA loads per wave (the rows of X, then of W, 64 rows a load; the last ones may have none)
   static constexpr int S_X = (BM + 63) / 64 * 64, LS = ((S_X + BN) / 64 + NW - 1) / NW;
   static constexpr int S_BYTES = LS * NW * 1024;
-  // KS = 1: a pair's place is taken again by the pair S_STAGES further, NS - 1 steps before that begins and after the last step of this one.
-  // KS > 1: a step's scales, and those of the other step of its pair, are loaded with it.
-  static constexpr int S_STAGES = KS == 1 ? (NS + 2) / 2 : NS;
+  // A pair's place is taken again by the pair S_STAGES further, NS - 1 steps (KS > 1: two) before that begins and after the last step of this one.
+  static constexpr int S_STAGES = (NS + 2) / 2;
   static constexpr int PART_BYTES = NS * (X_BYTES + W_BYTES) + S_STAGES * S_BYTES;   // of the waves that share steps
   static constexpr int LDS_BYTES = KS * PART_BYTES;
-  static_assert(KS == 1 || NW == 1, "steps are shared, or taken in turn");
+  static_assert(KS == 1 || (NW == 1 && NS == 2), "steps are shared, or taken in turn");
   static_assert(BM % (32 * WM) == 0 && BN % (64 * WN) == 0 && BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && (BM + BN) % 32 == 0, "whole fragments and loads");
   static_assert(LDS_BYTES <= 160 * 1024, "LDS of a CU");
 };
@@ -214,13 +213,13 @@ struct MxTile {
     // In flight behind the loads of a step when its turn comes: those of the D - 1 steps after it, and of the scales of at least
     // (D - 1) / 2 pairs (a pair's scales go in front of its first step's codes).
     constexpr int D = TS::NS - 1, PENDING = (D - 1) * (TS::LX + TS::LW) + (D - 1) / 2 * TS::LS;
-    for (int kt = 0; kt < D && kt < o.steps; ++kt) issue(lds, kt, kt);
+    for (int kt = 0; kt < D && kt < o.steps; ++kt) issue(lds, kt, kt, (kt >> 1) % TS::S_STAGES);
     int at = 0;
     for (int kt = 0; kt < o.steps; ++kt) {
       if (kt + D - 1 < o.steps) wait_and_barrier<PENDING>();
       else wait_and_barrier<0>();
       // the stage of step kt - 1, which everybody has left, takes step kt + D
-      if (kt + D < o.steps) issue(lds, kt + D, at == 0 ? TS::NS - 1 : at - 1);
+      if (kt + D < o.steps) issue(lds, kt + D, at == 0 ? TS::NS - 1 : at - 1, ((kt + D) >> 1) % TS::S_STAGES);
       const char *x = x_stage(lds, at), *w = w_stage(lds, at);
       uint32_t sx[TS::FM], sw[TS::FN];
       load_scales(s_stage(lds, (kt >> 1) % TS::S_STAGES), kt, sx, sw);
@@ -244,20 +243,23 @@ struct MxTile {
     }
   }
 
-  // KS > 1: the steps of this wave, in its part of the LDS.
+  // KS > 1: the pairs of steps of this wave, in its part of the LDS.
   MSLK_AMD_DEVINL void run_alone(char* mine, v16f (&acc)[TS::FN][TS::FM]) {
-    constexpr int PENDING = (TS::NS - 1) * (TS::LX + TS::LW + TS::LS);
-    const int first = turn_id(), turns = (o.steps - first + TS::KS - 1) / TS::KS;
-    for (int t = 0; t < TS::NS && t < turns; ++t) issue(mine, first + t * TS::KS, t);
-    int at = 0;
+    constexpr int CODES = TS::LX + TS::LW;   // loads of a step; a pair's scales go in front of its first step's
+    const int pairs = ((o.steps + 1) / 2 - turn_id() + TS::KS - 1) / TS::KS, last = turn_id() + (pairs - 1) * TS::KS;
+    const int turns = 2 * pairs - (pairs > 0 && 2 * last + 1 == o.steps ? 1 : 0);
+    auto fetch = [&](int t) { issue(mine, 2 * (turn_id() + (t >> 1) * TS::KS) + (t & 1), t & 1, (t >> 1) & 1); };
+    if (turns > 0) fetch(0);
+    if (turns > 1) fetch(1);
     for (int t = 0; t < turns; ++t) {
-      if (t + TS::NS - 1 < turns) wait<PENDING>();
-      else wait<0>();
-      const int kt = first + t * TS::KS;
-      const char *x = x_stage(mine, at), *w = w_stage(mine, at);
+      // in flight behind the loads of this turn: those of the next
+      if (t + 1 == turns) wait<0>();
+      else if ((t & 1) == 0) wait<CODES>();
+      else wait<CODES + TS::LS>();
+      const char *x = x_stage(mine, t & 1), *w = w_stage(mine, t & 1);
       v4i xf[TS::FM][4], wf[TS::FN][4];
       uint32_t sx[TS::FM], sw[TS::FN];
-      load_scales(s_stage(mine, at), kt, sx, sw);
+      load_scales(s_stage(mine, (t >> 1) & 1), t, sx, sw);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
 #pragma unroll
@@ -266,7 +268,7 @@ struct MxTile {
         for (int tn = 0; tn < TS::FN; ++tn) wf[tn][j] = w_chunk(w, tn, j);
       }
       wait<63>();   // for the reads: the stage is free
-      if (t + TS::NS < turns) issue(mine, kt + TS::NS * TS::KS, at);
+      if (t + 2 < turns) fetch(t + 2);
       auto product = [&](auto j) {
         constexpr int J = decltype(j)::value;
 #pragma unroll
@@ -278,15 +280,14 @@ struct MxTile {
       product(std::integral_constant<int, 1>{});
       product(std::integral_constant<int, 2>{});
       product(std::integral_constant<int, 3>{});
-      at = at + 1 == TS::NS ? 0 : at + 1;
     }
   }
 
-  // The loads of step kt into stage `at`, in front of them those of scales.
-  MSLK_AMD_DEVINL void issue(char* mine, int kt, int at) {
-    if (TS::KS > 1 || (kt & 1) == 0) {
+  // The loads of step kt into stage `at`; with a pair's first step, in front of them those of its scales into `scales`.
+  MSLK_AMD_DEVINL void issue(char* mine, int kt, int at, int scales) {
+    if ((kt & 1) == 0) {
 #pragma unroll
-      for (int i = 0; i < TS::LS; ++i) copy_scales(s_stage(mine, TS::KS == 1 ? (kt >> 1) % TS::S_STAGES : at), kt >> 1, i);
+      for (int i = 0; i < TS::LS; ++i) copy_scales(s_stage(mine, scales), kt >> 1, i);
     }
     const Adjust a = adjust(kt);
     const uint8_t *x = o.x + (int64_t)kt * kMxStep, *w = o.w + (int64_t)kt * kMxStep;
