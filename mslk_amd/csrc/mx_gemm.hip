@@ -409,28 +409,36 @@ hipError_t launch_walk(const MxProblem& p, hipStream_t s) {
 }
 
 enum Way : int {
-  kStream,     // few rows: mx_stream.hip
-  k32x64, k64x64, k128x128,
+  kStream,     // few rows, scales that the DMA cannot take: mx_stream.hip
+  k32x64, k64x64Long, k64x64, k128x128,
   k64x128,     // groups only
   kWalk,       // 256-column tiles (at least two steps)
 };
-using Tile32x64 = MxShape<32, 64, 1, 1, 2, 4>;      // a workgroup per CU
-using Tile64x64 = MxShape<64, 64, 1, 1, 2, 2>;      // two
-using Tile64x128 = MxShape<64, 128, 2, 2, 2>;       // two
-using Tile128x128 = MxShape<128, 128, 2, 2, 2>;     // two
+using Tile32x64 = MxShape<32, 64, 1, 1, 2, 4>;         // one workgroup per CU
+using Tile64x64Long = MxShape<64, 64, 1, 1, 2, 4>;     // one
+using Tile64x64 = MxShape<64, 64, 1, 1, 2, 2>;         // two
+using Tile64x128 = MxShape<64, 128, 2, 2, 2>;          // two
+using Tile128x128 = MxShape<128, 128, 2, 2, 2>;        // two
 
-// The smallest tiles of which each CU gets no more than it holds at once, since their steps' loads, not their products, are waited for.
-// At 8192 values (µs): 64 x 8192 32x64 11.1, 64x64 15.0, 128x128 25.7; 256 x 8192 64x64 22.0, 128x128 26.5, walk 30; 500 x 8192 128x128 29.0,
-// 64x64 40.6, walk 32.2; 1000 x 10240 walk 54, 128x128 64.9.
-// Up to 32 rows the weights stream past if there is a CU for every 32 columns (16 x 4096 x 14336 11.1 against 13.8; 16 x 10240 x 8192 14.8, 32x64 10.5).
+// Scales are fetched by 16 bytes.
+bool fetched_in_place(int64_t K, bool scales_aligned) { return K % 512 == 0 && scales_aligned; }
+
+// The smallest tiles of which each CU gets no more than it holds at once, since their steps' loads, not their products, are waited for.  µs:
+//   64 x 8192 x 8192    32x64 9.9, 64x64 13.2 (two waves 14.3), 128x128 25.7
+//   128 x 8192 x 8192   64x64 13.9 (two waves 15.1), 32x64 17.1, 128x128 26.3
+//   256 x 8192 x 8192   64x64 of two waves 19.7 (four 24.8), 128x128 27.0
+//   500 x 8192 x 4096   128x128 16.4, 64x64 22.1, walk 23.1
+//   1000 x 10240 x 8192 walk 55.2, 128x128 64.9
+// Up to 32 rows whose scales would have to be arranged first take the kernel that needs no such launch, if there is a CU for every 32 columns
+// (32 x 8192 x 8448 12.8, arranged 14; where they need not be, 1 x 8192 x 8192 takes 9.7 with it and 8.4 with 32x64).
 // Groups of few rows on average wait for weights, too: 64x128 tiles (16 groups of 256 rows, 2 x 5120 x 4096: 74.9, walk 79.4; 8 of 512 rows,
 // 4096 x 14336 77.3 and 102), but with a short K the walk, which has no gap between its tiles (128 of 512 rows, 2 x 768 x 2048: 35.5, 64x128 41.6).
-Way way_of(int64_t M, int64_t N, int64_t K, int gated, int64_t G, bool grouped) {
+Way way_of(int64_t M, int64_t N, int64_t K, int gated, int64_t G, bool grouped, bool scales_aligned) {
   const int64_t cus = device_compute_units(), columns = N * (gated ? 2 : 1);
   auto tiles = [&](int64_t bm, int64_t bn) { return (grouped ? most_row_tiles(M, G, bm) : (M + bm - 1) / bm) * ((columns + bn - 1) / bn); };
-  if (!grouped && M <= 32 && columns <= 32 * cus) return kStream;
+  if (!grouped && M <= 32 && columns <= 32 * cus && !fetched_in_place(K, scales_aligned)) return kStream;
   if (!grouped && tiles(32, 64) <= cus) return k32x64;
-  if (tiles(64, 64) <= 2 * cus) return k64x64;
+  if (tiles(64, 64) <= 2 * cus) return tiles(64, 64) <= cus ? k64x64Long : k64x64;
   const bool short_k = K <= 256, wide = N >= (1 << 25);   // what the walk does not take
   if (grouped) return M <= 64 || (M <= 64 * G && K >= 4096) || short_k || wide ? k64x128 : kWalk;
   return tiles(128, 128) <= 2 * cus || short_k || wide ? k128x128 : kWalk;
@@ -440,7 +448,7 @@ Way way_of(int64_t M, int64_t N, int64_t K, int gated, int64_t G, bool grouped) 
 // be fetched as they are: 128 x 128 tiles gain 0.1 to 0.27 us per step of the 500 to 2048 x 4096 to 10240 that were looked at, and the launch in
 // front takes 2.5 (K = 4096 21.6 us, arranged 22.8; K = 12288 55.7 and 51.0).
 bool arranges(Way way, int64_t M, int64_t K, int G, bool grouped, bool scales_aligned) {
-  if (K % 512 != 0 || !scales_aligned) return true;
+  if (!fetched_in_place(K, scales_aligned)) return true;
   if (way == k128x128) return K >= 6144;
   return way == kWalk && M > 64 * (int64_t)(grouped ? G : 1);
 }
@@ -449,7 +457,7 @@ bool arranges(Way way, int64_t M, int64_t K, int G, bool grouped, bool scales_al
 
 size_t mx_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated, int G, bool grouped, bool scales_aligned) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  const Way way = way_of(M, N, K, gated, G, grouped);
+  const Way way = way_of(M, N, K, gated, G, grouped, scales_aligned);
   if (way == kStream) return 0;
   const int64_t list = way == kWalk && grouped ? (1 + most_row_tiles(M, G, MxLarge::BM)) * (int64_t)sizeof(RowTile) : 0;
   if (!arranges(way, M, K, G, grouped, scales_aligned)) return (size_t)list;
@@ -458,7 +466,7 @@ size_t mx_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated, int G, boo
 
 hipError_t launch_mx_mm(MxProblem p, void* workspace, bool scales_aligned, hipStream_t s) {
   const bool grouped = p.m_sizes != nullptr;
-  const Way way = way_of(p.M, p.N, p.K, p.gated, p.G, grouped);
+  const Way way = way_of(p.M, p.N, p.K, p.gated, p.G, grouped, scales_aligned);
   if (way == kStream) return launch_mx_stream(p, s);
   const int from = p.K / kMxBlock, pairs = (int)pairs_of(p.K);
   const bool listed = way == kWalk && grouped, arranged = p.K > 0 && arranges(way, p.M, p.K, p.G, grouped, scales_aligned);
@@ -490,6 +498,7 @@ hipError_t launch_mx_mm(MxProblem p, void* workspace, bool scales_aligned, hipSt
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
   if (way == kWalk) return p.out_f16 ? launch_walk<true>(p, s) : launch_walk<false>(p, s);
+  if (way == k64x64Long) return grouped ? launch_groups<Tile64x64Long>(p, s) : launch_dense<Tile64x64Long>(p, s);
   if (way == k64x64) return grouped ? launch_groups<Tile64x64>(p, s) : launch_dense<Tile64x64>(p, s);
   if (way == k64x128) return launch_groups<Tile64x128>(p, s);
   return way == k32x64 ? launch_dense<Tile32x64>(p, s) : launch_dense<Tile128x128>(p, s);

@@ -277,7 +277,8 @@ def test_leading_dimensions_torch_types_and_views():
 TILED = [(5, 9000, 288), (32, 8200, 96), (40, 2000, 1280), (128, 1024, 2336), (70, 64, 4096), (1, 64, 2048),
          (520, 1100, 32), (520, 1104, 512), (513, 1100, 800), (33, 20000, 1056),
          (1100, 2000, 224), (1100, 2000, 512), (1025, 2056, 1312), (1, 40000, 64), (2600, 7000, 256),
-         (1500, 6000, 288), (1472, 6144, 512), (2600, 7000, 544), (4100, 4200, 800), (4240, 4096, 1024), (4050, 4360, 1056), (3, 70000, 512), (40, 66000, 320)]
+         (1500, 6000, 288), (1472, 6144, 512), (2600, 7000, 544), (4100, 4200, 800), (4240, 4096, 1024), (4050, 4360, 1056), (3, 70000, 512), (40, 66000, 320),
+         (8, 300, 8224), (16, 2000, 5152), (32, 100, 12320), (9, 40, 4128)]   # (the last ones: weights streamed, several rounds of pairs)
 
 
 @pytest.mark.parametrize("m,n,k", TILED)
@@ -285,7 +286,8 @@ def test_product_exact_with_every_tile(m, n, k):
     g = rng(m + n + k)
     xq, xs = operand(m, k, g)
     wq, ws = operand(n, k, g)
-    want, _ = O.product(xq, wq, xs, ws)   # (sums of K products of at most 36 x 4: below 2^20)
+    want, size = O.product(xq, wq, xs, ws)
+    assert size.max() < 1 << 20
     args = gpu(xq, wq, xs, ws)
     same_bits(mslk_amd.mxfp4_mm(*args), want)
     for bias_dtype, out_dtype in ((F32, F16), (BF16, BF16)):
