@@ -6,21 +6,25 @@
 namespace mslk_amd {
 namespace {
 
-// Eight columns n ... n + 7 of the bias, which lie on 16 bytes, as fp32.
-MSLK_AMD_DEVINL void load_bias(const MxProblem& p, int n, float (&b)[8]) {
+// Columns n + 8 h ... of the bias, which lie on 16 bytes, as fp32; n is the same for all lanes.  By scalar loads: a vector load's wait would be
+// one for the stores and the DMA loads in front of it, too.
+MSLK_AMD_DEVINL void load_bias(const MxProblem& p, int n, int h, float (&b)[8]) {
+  typedef const __attribute__((address_space(4))) uint32_t* constant_ptr;
+  const constant_ptr at = (constant_ptr)((uintptr_t)p.bias + (uintptr_t)n * (p.bias_dtype == 1 ? 4 : 2));
+  uint32_t v[8];
   if (p.bias_dtype == 1) {
-    const float4 *f = reinterpret_cast<const float4*>(static_cast<const float*>(p.bias) + n), lo = f[0], hi = f[1];
-    b[0] = lo.x; b[1] = lo.y; b[2] = lo.z; b[3] = lo.w;
-    b[4] = hi.x; b[5] = hi.y; b[6] = hi.z; b[7] = hi.w;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = h ? at[8 + e] : at[e];
   } else {
-    const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.bias) + n);
-    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      b[2 * e] = bf16_bits_to_f32(v[e] & 0xFFFFu);
-      b[2 * e + 1] = bf16_bits_to_f32(v[e] >> 16);
+      const uint32_t two = h ? at[4 + e] : at[e];
+      v[2 * e] = two << 16;
+      v[2 * e + 1] = two & 0xFFFF0000u;
     }
   }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) b[e] = __uint_as_float(v[e]);
 }
 
 // As store16_stream(), at a scalar base and a lane's offset.  (The data registers may be reused behind the statement: its wait states.)
@@ -52,7 +56,7 @@ MSLK_AMD_DEVINL void store_tile(const MxProblem& p, const v16f (&acc)[FN][FM], i
     float b[4][8];
     if constexpr (BIAS && FULL) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) load_bias(p, first + column(t, r, h), b[r]);
+      for (int r = 0; r < 4; ++r) load_bias(p, first + column(t, r, 0), h, b[r]);
     }
 #pragma unroll
     for (int tm = 0; tm < FM; ++tm) {
@@ -173,6 +177,7 @@ __global__ __launch_bounds__(TS::NTHREADS) void mx_kernel(MxProblem p, int tiles
 
 // Row tiles of at most 256 rows, as listed in device memory.
 struct RowTile { int row0, rows, group, unused; };
+static_assert(sizeof(RowTile) == 16, "read as four words");
 
 // A workgroup per CU that walks the 256-column tiles, in rounds: of each round's entries, neighbours all, XCD x takes a run.  (A list has long
 // tiles first, so those of a round are about as long; runs of the whole list leave the XCDs different amounts, 16 experts of 8192 rows 236 us
@@ -185,8 +190,10 @@ __global__ __launch_bounds__(256) void mx_walk_kernel(MxProblem p, int tiles_m, 
   using Tile = MxLargeTile<GATED>;
   __shared__ __attribute__((aligned(1024))) char lds[TS::LDS_BYTES];
   constexpr int COLUMNS = GATED ? TS::BN / 2 : TS::BN;
-  const RowTile* const list = static_cast<const RowTile*>(p.row_tiles);
-  if (list != nullptr) tiles_m = list[0].rows;   // (the first entry holds their number)
+  // (read by scalar loads, which wait for no store)
+  typedef const __attribute__((address_space(4))) int* constant_ptr;
+  const constant_ptr list = (constant_ptr)(uintptr_t)p.row_tiles;
+  if (list != nullptr) tiles_m = list[1];   // (the first entry holds their number as its rows)
   const int wgs = gridDim.x, xcd = blockIdx.x % kXcds, slot = blockIdx.x / kXcds;
   const int whole = tiles_m * tiles_n / wgs * wgs, rest = tiles_m * tiles_n - whole;
   const bool cut = list == nullptr && 2 * rest <= wgs;
@@ -205,8 +212,8 @@ __global__ __launch_bounds__(256) void mx_walk_kernel(MxProblem p, int tiles_m, 
     int tm, tn;
     tile_at(t, tiles_m, tiles_n, tm, tn);
     if (list != nullptr) {
-      const RowTile r = list[1 + tm];
-      at = Place{r.row0, r.rows, tn * COLUMNS, (int64_t)r.group * p.N * (GATED ? 2 : 1)};
+      const constant_ptr r = list + 4 * (1 + tm);   // row0, rows, group
+      at = Place{r[0], r[1], tn * COLUMNS, (int64_t)r[2] * p.N * (GATED ? 2 : 1)};
       return true;
     }
     const int m0 = tm * MxLarge::BM + half * 128;
@@ -228,8 +235,10 @@ __global__ __launch_bounds__(256) void mx_walk_kernel(MxProblem p, int tiles_m, 
       constexpr int F = decltype(fragments)::value;
       v16f acc[4][F];
       tile.template run<F>(lds, operands(at), held, acc);
-      if (here.rows == 64 * F && here.n0 + COLUMNS <= p.N && aligned) store_tile<F, 4, 2, 32, 64, GATED, BIAS, F16, true>(p, acc, here.m0, here.rows, here.n0);
+      const bool full = here.rows == 64 * F && here.n0 + COLUMNS <= p.N && aligned;
+      if (full) store_tile<F, 4, 2, 32, 64, GATED, BIAS, F16, true>(p, acc, here.m0, here.rows, here.n0);
       else store_tile<F, 4, 2, 32, 64, GATED, BIAS, F16, false>(p, acc, here.m0, here.rows, here.n0);
+      if (!full || at.rows > 64 * F) wait_vmcnt0();   // fewer stores than the next tile counts on
     };
     if (here.rows > 192) make(std::integral_constant<int, 4>{});
     else if (here.rows > 128) make(std::integral_constant<int, 3>{});

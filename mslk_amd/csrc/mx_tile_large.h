@@ -10,7 +10,8 @@
 // Loads.  X has two stages of 32 KiB, W a ring of ten fragments of 8 KiB, of which a step takes four: that and the scales are the LDS of a
 // CU.  Step k issues, with groups 1 and 2, fragments 0 and 1 of W of step k + 2 (places 8 and 9 behind this step's first); behind the
 // barrier, fragments 2 and 3 (places that this step has left) and X (the stage that this step has left).  At the barrier the loads of
-// groups 1 and 2 may be in flight.  The last two steps of a tile issue the first two of the next one.
+// groups 1 and 2 may be in flight.  The last two steps of a tile issue the first two of the next one, so the first barrier of that one need
+// not wait for the stores of the one before, which are younger than what it waits for (loads and stores end in order).
 //
 // Rows.  LDS row r of X is row r of the tile: fragment t of a wave's four is 32 of rows 64 t ... 64 t + 63.  A tile of at most 64 or 128 rows
 // (the last one of an operand or of a group; small operands are cut into such) takes a loop over one or two fragments.
@@ -146,7 +147,7 @@ struct MxLargeTile {
     const char *w_next = w_place(lds, wrap(held.place + TN + 1)), *x_next = x_stage(lds, held.stage ^ 1);
     const int to = wrap(held.place + 8);
     if constexpr (LAST) {
-      wait_and_barrier<4>();
+      wait_and_barrier<FIRST ? 4 + stores(F) : 4>();
       load_scales(lds, quad_next, odd_next, sx, sw);
     }
     auto product = [&](auto jj) {
@@ -212,10 +213,13 @@ struct MxLargeTile {
 #pragma unroll
       for (int q = 0; q < 8; ++q) copy_w<true>(w_place(lds, s * 4 + (q >> 1)), f, q);
     }
-    wait_and_barrier<16>();
+    wait_and_barrier<0>();   // (no stores: see run())
     held.stage = held.place = held.quad = held.odd = 0;
   }
+  // Stores of a whole tile, per wave.
+  MSLK_AMD_DEVINL static constexpr int stores(int f) { return (GATED ? 4 : 8) * f; }
   // acc = the sums of the tile that was begun, of which the first 64 F rows are valid; begins with tile `next` (any valid one if there is none).
+  // Since the loads of this tile's first two steps were issued there have been at least stores(F) stores, or a wait for everything.
   template <int F>
   MSLK_AMD_DEVINL void run(char* lds, const MxOperands& next, Held& held, v16f (&acc)[4][F]) {
     // (Read here and not in the last step before: they would be held over its sums' way out.)
