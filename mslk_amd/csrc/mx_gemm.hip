@@ -147,6 +147,7 @@ MSLK_AMD_DEVINL MxOperands operands_of(const MxProblem& p, int m0, int rows, int
 // One tile per workgroup.
 template <typename TS, bool GATED, bool GROUPS, bool BIAS, bool F16>
 __global__ __launch_bounds__(TS::NTHREADS) void mx_kernel(MxProblem p, int tiles_m, int tiles_n) {
+  static_assert(TS::LDS_BYTES <= 160 * 1024, "LDS of a CU");
   __shared__ __attribute__((aligned(1024))) char lds[TS::LDS_BYTES];
   constexpr int COLUMNS = GATED ? TS::BN / 2 : TS::BN;
   int m0, rows, tn;
@@ -423,12 +424,11 @@ enum Way : int {
   k64x128,     // groups only
   kWalk,       // 256-column tiles (at least two steps)
 };
-using Tile32x64 = MxShape<32, 64, 1, 1, 2, 4>;         // one workgroup per CU
-using Tile64x64Long = MxShape<64, 64, 1, 1, 2, 4>;     // one
-using Tile64x64 = MxShape<64, 64, 1, 1, 2, 2>;         // two
-using Tile64x128 = MxShape<64, 128, 2, 2, 2>;          // two
-using Tile128x128 = MxShape<128, 128, 2, 2, 2>;        // two
-
+using Tile32x64 = MxShape<32, 64, 1, 1, 4>;         // one workgroup per CU
+using Tile64x64Long = MxShape<64, 64, 1, 1, 4>;     // one
+using Tile64x64 = MxShape<64, 64, 1, 1, 2>;         // two
+using Tile64x128 = MxShape<64, 128, 2, 2, 1>;       // two
+using Tile128x128 = MxShape<128, 128, 2, 2, 1>;     // two
 // Scales are fetched by 16 bytes.
 bool fetched_in_place(int64_t K, bool scales_aligned) { return K % 512 == 0 && scales_aligned; }
 
@@ -453,12 +453,12 @@ Way way_of(int64_t M, int64_t N, int64_t K, int gated, int64_t G, bool grouped, 
   return tiles(128, 128) <= 2 * cus || short_k || wide ? k128x128 : kWalk;
 }
 
-// Whether the scales are arranged first.  Not where the product waits for the weights (few rows, or few per group) or has few steps, if they can
-// be fetched as they are: 128 x 128 tiles gain 0.1 to 0.27 us per step of the 500 to 2048 x 4096 to 10240 that were looked at, and the launch in
-// front takes 2.5 (K = 4096 21.6 us, arranged 22.8; K = 12288 55.7 and 51.0).
-bool arranges(Way way, int64_t M, int64_t K, int G, bool grouped, bool scales_aligned) {
+// Whether the scales are arranged first.  Not where the product waits for the weights (few rows, or few per group) or has little to do, if they
+// can be fetched in place: 128 x 128 tiles, two to a CU, gain 0.1 us per step, and the launch in front takes 2.5 and more (600 x 8192, K = 4096
+// 20.8 us, arranged 23.2; 8192 36.3 and 36.9; 14336 61.8 and 57.6; one to a CU, 256 x 10240, 14336 46.1 and 47.8).
+bool arranges(Way way, int64_t M, int64_t N, int64_t K, int gated, int G, bool grouped, bool scales_aligned) {
   if (!fetched_in_place(K, scales_aligned)) return true;
-  if (way == k128x128) return K >= 6144;
+  if (way == k128x128) return K >= 8192 && (M + 127) / 128 * ((N * (gated ? 2 : 1) + 127) / 128) > device_compute_units();
   return way == kWalk && M > 64 * (int64_t)(grouped ? G : 1);
 }
 
@@ -469,7 +469,7 @@ size_t mx_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated, int G, boo
   const Way way = way_of(M, N, K, gated, G, grouped, scales_aligned);
   if (way == kStream) return 0;
   const int64_t list = way == kWalk && grouped ? (1 + most_row_tiles(M, G, MxLarge::BM)) * (int64_t)sizeof(RowTile) : 0;
-  if (!arranges(way, M, K, G, grouped, scales_aligned)) return (size_t)list;
+  if (!arranges(way, M, N, K, gated, G, grouped, scales_aligned)) return (size_t)list;
   return (size_t)(list + arranged_bytes(M, K) + arranged_bytes(N * (gated ? 2 : 1) * (grouped ? G : 1), K));
 }
 
@@ -478,7 +478,7 @@ hipError_t launch_mx_mm(MxProblem p, void* workspace, bool scales_aligned, hipSt
   const Way way = way_of(p.M, p.N, p.K, p.gated, p.G, grouped, scales_aligned);
   if (way == kStream) return launch_mx_stream(p, s);
   const int from = p.K / kMxBlock, pairs = (int)pairs_of(p.K);
-  const bool listed = way == kWalk && grouped, arranged = p.K > 0 && arranges(way, p.M, p.K, p.G, grouped, scales_aligned);
+  const bool listed = way == kWalk && grouped, arranged = p.K > 0 && arranges(way, p.M, p.N, p.K, p.gated, p.G, grouped, scales_aligned);
   ArrangeJob a{}, b{};
   ListJob tiles{};
   uint8_t* room = static_cast<uint8_t*>(workspace);

@@ -31,13 +31,14 @@ namespace mslk_amd {
 
 constexpr int kMxStep = 128;          // bytes of a row per step
 
-// KS = 1: WM x WN waves share a step's products; of NS stages NS - 1 are in flight while one is multiplied.
-// KS > 1, for small tiles, which would otherwise wait a memory round trip and a barrier for every step's few products: KS waves take the pairs of
-// steps in turn, each with two stages and the whole tile's sums of its own.  A wave has a step in registers before it multiplies, and its stage
-// takes the one after the next: no barrier, two steps in flight per wave.  At the end the sums meet in LDS.
-template <int BM_, int BN_, int WM_, int WN_, int NS_, int KS_ = 1>
+// Two stages.  What a wave multiplies is in registers before its step's stage takes the step after the next: two steps are in flight, which the
+// memory's latency asks for (with one in flight, 16 groups of 64 rows, gated 5120 x 4096, take 71 us instead of 62).
+// WM x WN waves share a step's products (between barriers), or KS waves take the pairs of steps in turn, each with stages and the whole tile's
+// sums of its own and without a barrier; at the end the sums meet in LDS.  The latter for small tiles, which would otherwise wait a memory round
+// trip and a barrier for every step's few products.
+template <int BM_, int BN_, int WM_, int WN_, int KS_>
 struct MxShape {
-  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, NS = NS_, KS = KS_;
+  static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_, KS = KS_;
   static constexpr int NW = WM * WN, NTHREADS = NW * KS * 64;       // waves that share a step
   static constexpr int FM = BM / WM / 32, FN = BN / WN / 32;        // fragments of 32 rows per wave
   static constexpr int X_BYTES = BM * kMxStep, W_BYTES = BN * kMxStep;
@@ -45,13 +46,10 @@ struct MxShape {
   // scales of two steps: DMA loads per wave (the rows of X, then of W, 64 rows a load; the last ones may have none)
   static constexpr int S_X = (BM + 63) / 64 * 64, LS = ((S_X + BN) / 64 + NW - 1) / NW;
   static constexpr int S_BYTES = LS * NW * 1024;
-  // A pair's place is taken again by the pair S_STAGES further, NS - 1 steps (KS > 1: two) before that begins and after the last step of this one.
-  static constexpr int S_STAGES = (NS + 2) / 2;
-  static constexpr int PART_BYTES = NS * (X_BYTES + W_BYTES) + S_STAGES * S_BYTES;   // of the waves that share steps
+  static constexpr int PART_BYTES = 2 * (X_BYTES + W_BYTES + S_BYTES);   // of the waves that share steps
   static constexpr int LDS_BYTES = KS * PART_BYTES;
-  static_assert(KS == 1 || (NW == 1 && NS == 2), "steps are shared, or taken in turn");
+  static_assert(KS == 1 || NW == 1, "steps are shared, or taken in turn");
   static_assert(BM % (32 * WM) == 0 && BN % (64 * WN) == 0 && BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && (BM + BN) % 32 == 0, "whole fragments and loads");
-  static_assert(LDS_BYTES <= 160 * 1024, "LDS of a CU");
 };
 
 // Scales of a tile: row r of it is row `first` + r behind `base`, which is the first of 64.
@@ -138,8 +136,8 @@ struct MxTile {
   }
 
   MSLK_AMD_DEVINL static char* x_stage(char* lds, int i) { return lds + i * TS::X_BYTES; }
-  MSLK_AMD_DEVINL static char* w_stage(char* lds, int i) { return lds + TS::NS * TS::X_BYTES + i * TS::W_BYTES; }
-  MSLK_AMD_DEVINL static char* s_stage(char* lds, int i) { return lds + TS::NS * (TS::X_BYTES + TS::W_BYTES) + i * TS::S_BYTES; }
+  MSLK_AMD_DEVINL static char* w_stage(char* lds, int i) { return lds + 2 * TS::X_BYTES + i * TS::W_BYTES; }
+  MSLK_AMD_DEVINL static char* s_stage(char* lds, int i) { return lds + 2 * (TS::X_BYTES + TS::W_BYTES) + i * TS::S_BYTES; }
 
   // What is added to the offsets of a step's loads: 0, but in a last step of fewer blocks lanes of missing chunks go back to chunk 0.
   // Loads of even and of odd number differ: swz() of their rows does, in bit 2.
@@ -169,8 +167,9 @@ struct MxTile {
     __builtin_amdgcn_sched_barrier(0);
   }
 
+  // The same, with the barrier where waves share steps.
   template <int PENDING>
-  MSLK_AMD_DEVINL static void wait() { wait_and_barrier<PENDING, false>(); }
+  MSLK_AMD_DEVINL static void wait() { wait_and_barrier<PENDING, TS::KS == 1>(); }
 
   // Chunk 4 h + j of this lane's row of a fragment of 32 W rows at `rows`; w: of the W waves that share it, this one.
   MSLK_AMD_DEVINL static v4i chunk(const char* rows, int w, int j) {
@@ -200,54 +199,13 @@ struct MxTile {
       for (int tm = 0; tm < TS::FM; ++tm)
 #pragma unroll
         for (int r = 0; r < 16; ++r) acc[tn][tm][r] = 0.f;
-    if constexpr (TS::KS == 1) {
-      run_ring(lds, acc);
-    } else {
-      run_alone(lds + turn_id() * TS::PART_BYTES, acc);
-      add_sums(lds, acc);
-    }
-  }
-
-  // KS = 1.
-  MSLK_AMD_DEVINL void run_ring(char* lds, v16f (&acc)[TS::FN][TS::FM]) {
-    // In flight behind the loads of a step when its turn comes: those of the D - 1 steps after it, and of the scales of at least
-    // (D - 1) / 2 pairs (a pair's scales go in front of its first step's codes).
-    constexpr int D = TS::NS - 1, PENDING = (D - 1) * (TS::LX + TS::LW) + (D - 1) / 2 * TS::LS;
-    for (int kt = 0; kt < D && kt < o.steps; ++kt) issue(lds, kt, kt, (kt >> 1) % TS::S_STAGES);
-    int at = 0;
-    for (int kt = 0; kt < o.steps; ++kt) {
-      if (kt + D - 1 < o.steps) wait_and_barrier<PENDING>();
-      else wait_and_barrier<0>();
-      // the stage of step kt - 1, which everybody has left, takes step kt + D
-      if (kt + D < o.steps) issue(lds, kt + D, at == 0 ? TS::NS - 1 : at - 1, ((kt + D) >> 1) % TS::S_STAGES);
-      const char *x = x_stage(lds, at), *w = w_stage(lds, at);
-      uint32_t sx[TS::FM], sw[TS::FN];
-      load_scales(s_stage(lds, (kt >> 1) % TS::S_STAGES), kt, sx, sw);
-      auto product = [&](auto j) {
-        constexpr int J = decltype(j)::value;
-        v4i xf[TS::FM];
-#pragma unroll
-        for (int tm = 0; tm < TS::FM; ++tm) xf[tm] = x_chunk(x, tm, J);
-#pragma unroll
-        for (int tn = 0; tn < TS::FN; ++tn) {
-          const v4i wf = w_chunk(w, tn, J);
-#pragma unroll
-          for (int tm = 0; tm < TS::FM; ++tm) multiply<J>(wf, xf[tm], sw[tn], sx[tm], acc[tn][tm]);
-        }
-      };
-      product(std::integral_constant<int, 0>{});
-      product(std::integral_constant<int, 1>{});
-      product(std::integral_constant<int, 2>{});
-      product(std::integral_constant<int, 3>{});
-      at = at + 1 == TS::NS ? 0 : at + 1;
-    }
-  }
-
-  // KS > 1: the pairs of steps of this wave, in its part of the LDS.
-  MSLK_AMD_DEVINL void run_alone(char* mine, v16f (&acc)[TS::FN][TS::FM]) {
+    char* const mine = lds + turn_id() * TS::PART_BYTES;
     constexpr int CODES = TS::LX + TS::LW;   // loads of a step; a pair's scales go in front of its first step's
-    const int pairs = ((o.steps + 1) / 2 - turn_id() + TS::KS - 1) / TS::KS, last = turn_id() + (pairs - 1) * TS::KS;
-    const int turns = 2 * pairs - (pairs > 0 && 2 * last + 1 == o.steps ? 1 : 0);
+    int turns = o.steps;
+    if constexpr (TS::KS > 1) {
+      const int pairs = ((o.steps + 1) / 2 - turn_id() + TS::KS - 1) / TS::KS, last = turn_id() + (pairs - 1) * TS::KS;
+      turns = 2 * pairs - (pairs > 0 && 2 * last + 1 == o.steps ? 1 : 0);
+    }
     auto fetch = [&](int t) { issue(mine, 2 * (turn_id() + (t >> 1) * TS::KS) + (t & 1), t & 1, (t >> 1) & 1); };
     if (turns > 0) fetch(0);
     if (turns > 1) fetch(1);
@@ -267,8 +225,10 @@ struct MxTile {
 #pragma unroll
         for (int tn = 0; tn < TS::FN; ++tn) wf[tn][j] = w_chunk(w, tn, j);
       }
-      wait<63>();   // for the reads: the stage is free
-      if (t + 2 < turns) fetch(t + 2);
+      if (t + 2 < turns) {
+        wait<63>();   // for the reads: the stage is free
+        fetch(t + 2);
+      }
       auto product = [&](auto j) {
         constexpr int J = decltype(j)::value;
 #pragma unroll
@@ -281,6 +241,7 @@ struct MxTile {
       product(std::integral_constant<int, 2>{});
       product(std::integral_constant<int, 3>{});
     }
+    if constexpr (TS::KS > 1) add_sums(lds, acc);
   }
 
   // The loads of step kt into stage `at`; with a pair's first step, in front of them those of its scales into `scales`.

@@ -33,7 +33,7 @@ struct MxLarge {
 template <bool GATED>
 struct MxLargeTile {
   using TS = MxLarge;
-  using Rows = MxTile<MxShape<256, 256, 2, 2, 2>, GATED>;   // which row of the tile an LDS row holds
+  using Rows = MxTile<MxShape<256, 256, 2, 2, 1>, GATED>;   // which row of the tile an LDS row holds
   // Of the tile whose loads are being issued; `steps` and the layout are the same for all.
   uint32_t x_off[8], w_off[8], s_off[2];
   const uint8_t *x, *w, *s_base;
