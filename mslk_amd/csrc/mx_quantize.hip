@@ -6,6 +6,7 @@
 //
 // Both are bound by memory.  A lane holds 8 values (16 bytes of 16-bit ones), so that a wave reads and writes whole lines; four
 // neighbouring lanes are a block and find its maximum by data-parallel moves, on the bits, where NaN > infinity > numbers.
+// 8192 x 28672 bf16 values: 134 us there (4.4 TB/s read and written) and 88 back (6.8: the codes are still in the Infinity Cache).
 #include "mx.h"
 #include "quant_math.h"
 

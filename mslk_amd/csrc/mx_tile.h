@@ -1,6 +1,7 @@
 // Tile of a product of two MXFP4 matrices for gfx950 (formats: mx.h): Y[m, n] = sum_k X[m, k] W[n, k].
 //
-// One workgroup (a WM x WN grid of wavefronts) makes a BM x BN tile of sums.
+// One workgroup (a WM x WN grid of wavefronts, or KS of them one behind the other) makes a BM x BN tile of sums.  What bounds these tiles are the
+// loads of their steps, 60 KB per us and CU where the DMA alone reaches 100: 64 x 64 tiles, two to a CU, 0.5 us per step, 128 x 128 ones 1.05.
 //
 // Steps.  K is consumed 256 values (128 bytes of a row) at a time, copied global -> LDS by the 128-bit DMA load (gemm_tile.h).  Eight
 // 16-byte chunks make a row of 128 bytes in LDS, one chunk being one block of 32 values; they are permuted by chunk ^ swz(row), so that
