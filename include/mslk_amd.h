@@ -392,7 +392,7 @@ int mslk_amd_dequantize_mxfp4(const void* codes, const void* scales, int64_t row
 
 /*
  * y[m, n] = sum_k X[m, k] W[n, k] + bias[n], fp32 sums rounded once to y_dtype (bf16, fp16).
- * gated != 0: W has 2 N rows, a gate's N rows and then N more, and y = silu(X Wg^T) * (X Wu^T) (no bias); N K < 2^32.
+ * gated != 0: W has 2 N rows, a gate's N rows and then N more, and y = silu(X Wg^T) * (X Wu^T) (no bias); N K < 2^33.
  *   xq [M, K / 2], wq [N or 2 N, K / 2] codes, 16-byte aligned; x_scale, w_scale their scales; y [M, N].  K < 2^24.
  *   workspace: mslk_amd_mxfp4_mm_workspace_bytes() of it, 16-byte aligned; `aligned` != 0 says that both scale pointers are 16-byte
  *   aligned.  Nothing in it is kept from one call to the next.

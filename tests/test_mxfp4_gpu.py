@@ -442,6 +442,59 @@ def test_rows_of_no_expert_stay_and_sizes_beyond_the_rows_end_with_them(sizes):
     assert (y[total - left:] == 77).all()
 
 
+@pytest.mark.parametrize("sizes", [[3, 0, 100, 0], [0, 0, 0, 0], [-5, 90, -1, 70], [50, 1 << 40, 7, 1], [1 << 62, 1 << 62, 1 << 62, 1 << 62], [300, 300, 300, 300]])
+@pytest.mark.parametrize("n,k", [(6000, 512), (6000, 160)], ids=["listed", "looked_up"])
+def test_sizes_that_do_not_fit_with_every_tile(sizes, n, k):
+    total = 280
+    g = rng(19)
+    xq, xs = operand(total, k, g)
+    wq, ws = operand((4, n), k, g)
+    y = torch.full((total + 4, n), 77.0, dtype=BF16, device=DEV)
+    call_grouped(*gpu(xq, wq, xs, ws), torch.tensor(sizes, device=DEV), y[:total])
+    left, clipped = total, []
+    for s in sizes:
+        clipped.append(min(max(s, 0), left))
+        left -= clipped[-1]
+    same_bits(y[: total - left], grouped_oracle(xq, wq, xs, ws, clipped, False))
+    assert (y[total - left:] == 77).all()
+
+
+# Operands and results of more than 2^32 bytes, with the kernels that each size takes; looked at are rows and columns from all over.
+@pytest.mark.parametrize("m,n,k,gated", [(3, 300000, 32768, False), (300000, 3, 32768, False), (70000, 70000, 288, False), (66000, 66000, 64, False),
+                                         (40, 140000, 32768, True)])
+def test_offsets_beyond_32_bits(m, n, k, gated):
+    gen = torch.Generator(DEV).manual_seed(m + n)
+    byte = lambda low, high, *shape: torch.randint(low, high, shape, generator=gen, device=DEV, dtype=torch.uint8)  # noqa: E731
+    wide = 2 * n if gated else n
+    xq, xs, wq, ws = byte(0, 256, m, k // 2), byte(126, 129, m, k // 32), byte(0, 256, wide, k // 2), byte(126 - 7 * gated, 129 - 7 * gated, wide, k // 32)
+    assert max(xq.numel(), wq.numel(), 2 * m * n) > 1 << 32
+    y = mslk_amd.mxfp4_gated_mm(xq, wq, xs, ws) if gated else mslk_amd.mxfp4_mm(xq, wq, xs, ws)
+    some = lambda size: torch.unique(torch.cat([torch.arange(3), torch.randint(0, size, (20,), generator=rng(1)), torch.arange(size - 3, size)]).clamp(0, size - 1))  # noqa: E731
+    rows, columns = some(m).to(DEV), some(n).to(DEV)
+    got = y[rows][:, columns]
+    if gated:
+        both = torch.cat([columns, columns + n])
+        want, (gate, up, size_gate, size_up) = O.gated(xq[rows], wq[both], xs[rows], ws[both])
+        # sums of 32768 products are not exact here (test_product_of_wide_scales); d silu(g) / dg is below 1.1
+        off = (k / 64 + 64) * 2.0 ** -23
+        within(got, want, (2.0 ** -20 + gate.abs() * 2.0 ** -22) * want.abs() + 1.1 * off * size_gate * (up.abs() + off * size_up) + gate.abs() * off * size_up)
+    else:
+        want, size = O.product(xq[rows], wq[columns], xs[rows], ws[columns])
+        within(got, want, (k / 64 + 64) * 2.0 ** -23 * size)
+
+
+def test_offsets_beyond_32_bits_of_experts():
+    gen = torch.Generator(DEV).manual_seed(5)
+    byte = lambda low, high, *shape: torch.randint(low, high, shape, generator=gen, device=DEV, dtype=torch.uint8)  # noqa: E731
+    n, k, sizes = 40000, 8192, [100, 0, 0, 30, 1, 0, 0, 0, 0, 200, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 60]
+    xq, xs, wq, ws = byte(0, 256, sum(sizes), k // 2), byte(126, 129, sum(sizes), k // 32), byte(0, 256, 30, n, k // 2), byte(126, 129, 30, n, k // 32)
+    assert wq.numel() > 1 << 32
+    y = mslk_amd.mxfp4_grouped_mm(xq, wq, xs, ws, torch.tensor(sizes, device=DEV))
+    columns = torch.arange(0, n, 1999, device=DEV)
+    want = grouped_oracle(xq.cpu(), wq[:, columns].cpu(), xs.cpu(), ws[:, columns].cpu(), sizes, False)
+    same_bits(y[:, columns], want)
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # as programs use them
 # ---------------------------------------------------------------------------------------------------------------------
@@ -478,6 +531,35 @@ def test_captured_products_follow_their_inputs():
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.equal(a, b), i
+
+
+def test_captured_experts_with_listed_tiles_follow_their_sizes():
+    """Two graphs of one program, each with workspaces of its own, replayed in turn: row tiles are listed again in each replay."""
+    g = rng(29)
+    k, n, experts, total = 544, 2400, 6, 600
+    wq, ws = gpu(*operand((experts, n), k, g))
+    operands = [gpu(*operand(total, k, g)) for _ in range(2)]
+    sizes = [torch.tensor([100] * 6, device=DEV), torch.tensor([600, 0, 0, 0, 0, 0], device=DEV)]
+    run = lambda i: mslk_amd.mxfp4_grouped_mm(operands[i][0], wq, operands[i][1], ws, sizes[i])  # noqa: E731
+    run(0)
+    torch.cuda.synchronize()
+    graphs, held = [], []
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i]):
+            held.append(run(i))
+    for step, now in enumerate([[100] * 6, [0, 0, 0, 0, 0, 600], [1, 2, 3, 4, 5, 585], [257, 0, 256, 0, 87, 0], [0, 300, 0, 0, 300, 0]]):
+        for i in range(2):
+            sizes[i].copy_(torch.tensor(now if i == 0 else now[::-1]))
+            operands[i][0].copy_(torch.randint(0, 256, (total, k // 2), generator=g, dtype=torch.uint8))
+            held[i].fill_(-1)
+        for graph in graphs:
+            graph.replay()
+        got = [y.clone() for y in held]
+        for i in range(2):
+            assert torch.equal(got[i], run(i)), (step, i)
+            counts = sizes[i].tolist()
+            same_bits(got[i], grouped_oracle(operands[i][0].cpu(), wq.cpu(), operands[i][1].cpu(), ws.cpu(), counts, False))
 
 
 def test_on_another_stream_with_memory_of_its_own():
