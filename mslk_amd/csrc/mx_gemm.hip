@@ -453,13 +453,16 @@ Way way_of(int64_t M, int64_t N, int64_t K, int gated, int64_t G, bool grouped, 
   return tiles(128, 128) <= 2 * cus || short_k || wide ? k128x128 : kWalk;
 }
 
-// Whether the scales are arranged first.  Not where the product waits for the weights (few rows, or few per group) or has little to do, if they
-// can be fetched in place: 128 x 128 tiles, two to a CU, gain 0.1 us per step, and the launch in front takes 2.5 and more (600 x 8192, K = 4096
-// 20.8 us, arranged 23.2; 8192 36.3 and 36.9; 14336 61.8 and 57.6; one to a CU, 256 x 10240, 14336 46.1 and 47.8).
-bool arranges(Way way, int64_t M, int64_t N, int64_t K, int gated, int G, bool grouped, bool scales_aligned) {
+// Whether the scales are arranged first.  If they can be fetched in place, the launch in front has to be worth it.
+// The walk: from 128 steps of 256 x 256 sums per CU on (arranged / in place, us: 4096 x 4096 x 4096 43.4 / 41.4, 16 experts, 2048 rows, 8192 x 5120
+// 126 / 119, 8192 x 8192 x 2048 92 / 91, 8192 x 8192 x 8192 263 / 265, 16384 x 8192 x 16384 938 / 959, 16 experts, 32768 rows 756 / 774).
+// 128 x 128 tiles: two of them to a CU, and a long K (600 x 8192, K = 4096 23.2 / 20.8, 8192 36.9 / 36.3, 14336 57.6 / 61.8; 500 x 10240 x 8192 34.7 / 36.7;
+// one to a CU, 256 x 10240 x 14336 47.8 / 46.1).  Smaller tiles wait for codes.
+bool arranges(Way way, int64_t M, int64_t N, int64_t K, int gated, bool scales_aligned) {
   if (!fetched_in_place(K, scales_aligned)) return true;
-  if (way == k128x128) return K >= 8192 && (M + 127) / 128 * ((N * (gated ? 2 : 1) + 127) / 128) > device_compute_units();
-  return way == kWalk && M > 64 * (int64_t)(grouped ? G : 1);
+  const int64_t columns = N * (gated ? 2 : 1), cus = device_compute_units();
+  if (way == k128x128) return K >= 8192 && (M + 127) / 128 * ((columns + 127) / 128) > cus;
+  return way == kWalk && (double)M * (double)columns * (double)K >= 128. * (double)cus * (256 * 256 * 256);
 }
 
 }  // namespace
@@ -469,7 +472,7 @@ size_t mx_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated, int G, boo
   const Way way = way_of(M, N, K, gated, G, grouped, scales_aligned);
   if (way == kStream) return 0;
   const int64_t list = way == kWalk && grouped ? (1 + most_row_tiles(M, G, MxLarge::BM)) * (int64_t)sizeof(RowTile) : 0;
-  if (!arranges(way, M, N, K, gated, G, grouped, scales_aligned)) return (size_t)list;
+  if (!arranges(way, M, N, K, gated, scales_aligned)) return (size_t)list;
   return (size_t)(list + arranged_bytes(M, K) + arranged_bytes(N * (gated ? 2 : 1) * (grouped ? G : 1), K));
 }
 
@@ -478,7 +481,7 @@ hipError_t launch_mx_mm(MxProblem p, void* workspace, bool scales_aligned, hipSt
   const Way way = way_of(p.M, p.N, p.K, p.gated, p.G, grouped, scales_aligned);
   if (way == kStream) return launch_mx_stream(p, s);
   const int from = p.K / kMxBlock, pairs = (int)pairs_of(p.K);
-  const bool listed = way == kWalk && grouped, arranged = p.K > 0 && arranges(way, p.M, p.N, p.K, p.gated, p.G, grouped, scales_aligned);
+  const bool listed = way == kWalk && grouped, arranged = p.K > 0 && arranges(way, p.M, p.N, p.K, p.gated, scales_aligned);
   ArrangeJob a{}, b{};
   ListJob tiles{};
   uint8_t* room = static_cast<uint8_t*>(workspace);

@@ -10,7 +10,7 @@
 // Scales.  A row's scales of two steps, a pair, are 16 bytes.  They travel by the same DMA into a ring of their own, 16 bytes per row.
 // (Loaded into registers instead, the compiler's wait for them would be one for the DMA loads too, which it does not know of.)  As
 // they lie in the tensor, each row's 16 bytes are a line for the L1 and the L2 to look up, and a pair of a 256 x 256 tile 512 lines next to
-// 1024 of codes: 0.28 of 1.94 us per step.  So large products have them arranged first, 64 rows to a KiB (MxScales).
+// 1024 of codes: up to 0.28 us per step, where power leaves that to be seen.  Large products have them arranged first, 64 rows to a KiB (MxScales).
 // K's end.  Of a last step of fewer than eight blocks the missing chunks are filled with chunk 0, and their scales are 0, 2^-127, in rows
 // that the caller has padded: products of two such blocks are below 2^-243 and vanish in fp32.
 // Products.  v_mfma_scale_f32_32x32x64_f8f6f4, W first: lane (i = l & 31, h = l >> 5) gives row i's chunk 4 h + j to product j of a
