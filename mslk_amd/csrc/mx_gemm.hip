@@ -124,6 +124,35 @@ MSLK_AMD_DEVINL void store_tile(const MxProblem& p, const v16f (&acc)[FN][FM], i
   }
 }
 
+// The same of a single fragment: pieces of four columns, 8 bytes.
+template <bool GATED, bool BIAS, bool F16>
+MSLK_AMD_DEVINL void store_fragment(const MxProblem& p, const v16f& acc, int m0, int rows, int n0) {
+  const int lane = threadIdx.x & 63, h = lane >> 5, m = lane & 31;
+  if (m >= rows) return;
+  const bool aligned = (p.N & 3) == 0 && (reinterpret_cast<uintptr_t>(p.y) & 7) == 0;
+#pragma unroll
+  for (int q = 0; q < (GATED ? 2 : 4); ++q) {
+    const int n = n0 + 8 * q + 4 * h;
+    if (n >= p.N) continue;
+    float v[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      v[r] = acc[4 * q + r];
+      if constexpr (GATED) v[r] = gated_value(v[r], acc[4 * q + 8 + r]);
+      if constexpr (BIAS) v[r] += bias_at(p, min(n + r, p.N - 1));
+    }
+    const uint32_t w[2] = {pack_out_x2<F16>(v[0], v[1]), pack_out_x2<F16>(v[2], v[3])};
+    uint16_t* dst = p.y + (int64_t)(m0 + m) * p.N + n;
+    if (aligned) {
+      *reinterpret_cast<uint2*>(dst) = make_uint2(w[0], w[1]);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (n + r < p.N) dst[r] = (uint16_t)(w[r >> 1] >> ((r & 1) * 16));
+    }
+  }
+}
+
 // Operands of the tile of rows m0 ..., columns n0 ...; w_row: first row of W's group.
 template <bool GATED>
 MSLK_AMD_DEVINL MxOperands operands_of(const MxProblem& p, int m0, int rows, int64_t w_row, int n0, int columns) {
@@ -172,7 +201,9 @@ __global__ __launch_bounds__(TS::NTHREADS) void mx_kernel(MxProblem p, int tiles
   MxTile<TS, GATED> tile;
   tile.init(operands_of<GATED>(p, m0, rows, w_row, n0, COLUMNS));
   tile.run(lds, acc);
-  if (MxTile<TS, GATED>::turn_id() == 0)
+  if (MxTile<TS, GATED>::turn_id() != 0) return;
+  if constexpr (TS::FN == 1) store_fragment<GATED, BIAS, F16>(p, acc[0][0], m0, rows, n0);
+  else
     store_tile<TS::FM, TS::FN, TS::WN, TS::BM / TS::WM, 32, GATED, BIAS, F16, false>(p, acc, m0, rows, n0);
 }
 
@@ -420,11 +451,12 @@ hipError_t launch_walk(const MxProblem& p, hipStream_t s) {
 
 enum Way : int {
   kStream,     // few rows, scales that the DMA cannot take: mx_stream.hip
-  k32x64, k64x64Long, k64x64, k128x128,
+  k32x32, k32x64, k64x64Long, k64x64, k128x128,
   k64x128,     // groups only
   kWalk,       // 256-column tiles (at least two steps)
 };
-using Tile32x64 = MxShape<32, 64, 1, 1, 4>;         // one workgroup per CU
+using Tile32x32 = MxShape<32, 32, 1, 1, 4>;         // two workgroups per CU
+using Tile32x64 = MxShape<32, 64, 1, 1, 4>;         // one
 using Tile64x64Long = MxShape<64, 64, 1, 1, 4>;     // one
 using Tile64x64 = MxShape<64, 64, 1, 1, 2>;         // two
 using Tile64x128 = MxShape<64, 128, 2, 2, 1>;       // two
@@ -433,19 +465,23 @@ using Tile128x128 = MxShape<128, 128, 2, 2, 1>;     // two
 bool fetched_in_place(int64_t K, bool scales_aligned) { return K % 512 == 0 && scales_aligned; }
 
 // The smallest tiles of which each CU gets no more than it holds at once, since their steps' loads, not their products, are waited for.  µs:
-//   64 x 8192 x 8192    32x64 9.9, 64x64 13.2 (two waves 14.3), 128x128 25.7
+//   16 x 4096 x 14336   32x32 8.3, 32x64 11.7, 64x64 14.3
+//   64 x 4096 x 14336   32x32 9.5, 32x64 13.0, 64x64 18.0
+//   64 x 8192 x 8192    32x64 9.9, 32x32 11.0, 64x64 13.2 (two waves 14.3), 128x128 25.7
+//   16 x 16384 x 4096   32x32 8.2, 32x64 8.5, 64x64 9.8 (up to 32 rows two of the smallest to a CU, as they read no weights twice)
 //   128 x 8192 x 8192   64x64 13.9 (two waves 15.1), 32x64 17.1, 128x128 26.3
 //   256 x 8192 x 8192   64x64 of two waves 19.7 (four 24.8), 128x128 27.0
 //   500 x 8192 x 4096   128x128 16.4, 64x64 22.1, walk 23.1
 //   1000 x 10240 x 8192 walk 55.2, 128x128 64.9
 // Up to 32 rows whose scales would have to be arranged first take the kernel that needs no such launch, if there is a CU for every 32 columns
-// (32 x 8192 x 8448 12.8, arranged 14; where they need not be, 1 x 8192 x 8192 takes 9.7 with it and 8.4 with 32x64).
+// (32 x 8192 x 8448 11.4, arranged 13.6; 16 x 4096 x 4128 8.8 and 11.2).
 // Groups of few rows on average wait for weights, too: 64x128 tiles (16 groups of 256 rows, 2 x 5120 x 4096: 74.9, walk 79.4; 8 of 512 rows,
 // 4096 x 14336 77.3 and 102), but with a short K the walk, which has no gap between its tiles (128 of 512 rows, 2 x 768 x 2048: 35.5, 64x128 41.6).
 Way way_of(int64_t M, int64_t N, int64_t K, int gated, int64_t G, bool grouped, bool scales_aligned) {
   const int64_t cus = device_compute_units(), columns = N * (gated ? 2 : 1);
   auto tiles = [&](int64_t bm, int64_t bn) { return (grouped ? most_row_tiles(M, G, bm) : (M + bm - 1) / bm) * ((columns + bn - 1) / bn); };
   if (!grouped && M <= 32 && columns <= 32 * cus && !fetched_in_place(K, scales_aligned)) return kStream;
+  if (!grouped && tiles(32, 32) <= (M <= 32 ? 2 : 1) * cus) return k32x32;
   if (!grouped && tiles(32, 64) <= cus) return k32x64;
   if (tiles(64, 64) <= 2 * cus) return tiles(64, 64) <= cus ? k64x64Long : k64x64;
   const bool short_k = K <= 256, wide = N >= (1 << 25);   // what the walk does not take
@@ -513,6 +549,7 @@ hipError_t launch_mx_mm(MxProblem p, void* workspace, bool scales_aligned, hipSt
   if (way == k64x64Long) return grouped ? launch_groups<Tile64x64Long>(p, s) : launch_dense<Tile64x64Long>(p, s);
   if (way == k64x64) return grouped ? launch_groups<Tile64x64>(p, s) : launch_dense<Tile64x64>(p, s);
   if (way == k64x128) return launch_groups<Tile64x128>(p, s);
+  if (way == k32x32) return launch_dense<Tile32x32>(p, s);
   return way == k32x64 ? launch_dense<Tile32x64>(p, s) : launch_dense<Tile128x128>(p, s);
 }
 

@@ -22,6 +22,7 @@
 // gives a lane eight neighbouring columns: 16 bytes of a row of Y, stored as they are.
 // GATED: a tile has BN / 2 columns; fragments with t = 0 are rows of the gate, those with t = 1 the rows N further, of columns
 // 32 T + 16 h + 4 q + r, so a lane holds both factors of its columns.
+// A single fragment (FN = 1) has columns 8 q + 4 h + r, gated: for q < 2 of the gate, for the others the rows N further of column - 16.
 #pragma once
 #include <type_traits>
 
@@ -45,12 +46,12 @@ struct MxShape {
   static constexpr int X_BYTES = BM * kMxStep, W_BYTES = BN * kMxStep;
   static constexpr int LX = BM / 8 / NW, LW = BN / 8 / NW;          // DMA loads per wave and step
   // scales of two steps: DMA loads per wave (the rows of X, then of W, 64 rows a load; the last ones may have none)
-  static constexpr int S_X = (BM + 63) / 64 * 64, LS = ((S_X + BN) / 64 + NW - 1) / NW;
+  static constexpr int S_X = (BM + 63) / 64 * 64, LS = ((S_X + BN + 63) / 64 + NW - 1) / NW;
   static constexpr int S_BYTES = LS * NW * 1024;
   static constexpr int PART_BYTES = 2 * (X_BYTES + W_BYTES + S_BYTES);   // of the waves that share steps
   static constexpr int LDS_BYTES = KS * PART_BYTES;
   static_assert(KS == 1 || NW == 1, "steps are shared, or taken in turn");
-  static_assert(BM % (32 * WM) == 0 && BN % (64 * WN) == 0 && BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && (BM + BN) % 32 == 0, "whole fragments and loads");
+  static_assert(BM % (32 * WM) == 0 && (BN % (64 * WN) == 0 || (KS > 1 && BN == 32)) && BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && (BM + BN) % 32 == 0, "whole fragments and loads");
 };
 
 // Scales of a tile: row r of it is row `first` + r behind `base`, which is the first of 64.
@@ -96,6 +97,10 @@ struct MxTile {
   // Row of W (of the tile's) that LDS row r of W holds, and whether it is one of the second half.
   MSLK_AMD_DEVINL static int w_row(int r, bool& up) {
     const int wn = (r >> 5) % TS::WN, tn = r / (32 * TS::WN), i = r & 31;
+    if constexpr (TS::FN == 1) {
+      up = GATED && i >= 16;
+      return GATED ? i & 15 : i;
+    }
     up = GATED && (tn & 1) != 0;
     if constexpr (GATED) return wn * (TS::BN / TS::WN / 2) + (tn >> 1) * 32 + ((i >> 2) & 1) * 16 + (i >> 3) * 4 + (i & 3);
     else return wn * (TS::BN / TS::WN) + (tn >> 1) * 64 + (tn & 1) * 4 + (i >> 2) * 8 + (i & 3);
@@ -265,27 +270,30 @@ struct MxTile {
     }
   }
 
-  // KS > 1: the first wave's sums become those of all, through LDS: [wave - 1][fragment][register][lane].
+  // KS > 1: the first wave's sums become those of all, through LDS: [wave - 1][fragment][q][lane] of four.
   MSLK_AMD_DEVINL static void add_sums(char* lds, v16f (&acc)[TS::FN][TS::FM]) {
-    constexpr int SUMS = TS::BM * TS::BN;
-    static_assert((TS::KS - 1) * SUMS * 4 <= TS::LDS_BYTES, "room for the sums");
-    float* const at = reinterpret_cast<float*>(lds) + (threadIdx.x & 63);
+    constexpr int QUADS = TS::FN * TS::FM * 4;
+    static_assert((TS::KS - 1) * QUADS * 1024 <= TS::LDS_BYTES, "room for the sums");
+    v4f* const at = reinterpret_cast<v4f*>(lds) + (threadIdx.x & 63);
     const int wave = turn_id();
     wait_and_barrier<0>();   // nobody reads or fills stages any more
     if (wave > 0) {
 #pragma unroll
-      for (int f = 0; f < TS::FN * TS::FM; ++f)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) at[(wave - 1) * SUMS + (f * 16 + r) * 64] = acc[f / TS::FM][f % TS::FM][r];
+      for (int i = 0; i < QUADS; ++i) {
+        const v16f& a = acc[(i >> 2) / TS::FM][(i >> 2) % TS::FM];
+        at[((wave - 1) * QUADS + i) * 64] = v4f{a[4 * (i & 3)], a[4 * (i & 3) + 1], a[4 * (i & 3) + 2], a[4 * (i & 3) + 3]};
+      }
     }
     __syncthreads();
     if (wave == 0) {
 #pragma unroll
       for (int k = 0; k < TS::KS - 1; ++k)
 #pragma unroll
-        for (int f = 0; f < TS::FN * TS::FM; ++f)
+        for (int i = 0; i < QUADS; ++i) {
+          const v4f v = at[(k * QUADS + i) * 64];
 #pragma unroll
-          for (int r = 0; r < 16; ++r) acc[f / TS::FM][f % TS::FM][r] += at[k * SUMS + (f * 16 + r) * 64];
+          for (int r = 0; r < 4; ++r) acc[(i >> 2) / TS::FM][(i >> 2) % TS::FM][4 * (i & 3) + r] += v[r];
+        }
     }
   }
 };

@@ -271,14 +271,15 @@ def test_leading_dimensions_torch_types_and_views():
     same_bits(one, want[0, 0])
 
 
-# Sizes for each kind of tile, beside those of few rows above (on 256 CUs): 32 x 64 and 64 x 64 tiles whose waves take the steps in turn, with
+# Sizes for each kind of tile, beside those of few rows above (on 256 CUs): 32 x 32, 32 x 64 and 64 x 64 tiles whose waves take the steps in turn, with
 # fewer steps than waves, as many and some more; 128 x 128 tiles; 256-column tiles in less than a round, in a last one that is cut in two (the
 # last rows have no second half), with 64, 128, 192 and 256 rows in the last tile.  K from one step to several, whole ones and not.
 TILED = [(5, 9000, 288), (32, 8200, 96), (40, 2000, 1280), (128, 1024, 2336), (70, 64, 4096), (1, 64, 2048),
          (520, 1100, 32), (520, 1104, 512), (513, 1100, 800), (33, 20000, 1056),
          (1100, 2000, 224), (1100, 2000, 512), (1025, 2056, 1312), (1, 40000, 64), (2600, 7000, 256),
          (1500, 6000, 288), (1472, 6144, 512), (2600, 7000, 544), (4100, 4200, 800), (4240, 4096, 1024), (4050, 4360, 1056), (3, 70000, 512), (40, 66000, 320),
-         (8, 300, 8224), (16, 2000, 5152), (32, 100, 12320), (9, 40, 4128)]   # (the last ones: weights streamed, several rounds of pairs)
+         (8, 300, 8224), (16, 2000, 5152), (32, 100, 12320), (9, 40, 4128),
+         (100, 2600, 1312), (64, 8192, 544), (97, 2621, 2048), (128, 4096, 512), (100, 2602, 64), (32, 16384, 512), (30, 16380, 1056)]   # (then: weights streamed, several rounds of pairs; 32 x 64 tiles again; as many 32 x 32 ones as there can be)
 
 
 @pytest.mark.parametrize("m,n,k", TILED)
