@@ -475,8 +475,9 @@ bool fetched_in_place(int64_t K, bool scales_aligned) { return K % 512 == 0 && s
 //   1000 x 10240 x 8192 walk 55.2, 128x128 64.9
 // Up to 32 rows whose scales would have to be arranged first take the kernel that needs no such launch, if there is a CU for every 32 columns
 // (32 x 8192 x 8448 11.4, arranged 13.6; 16 x 4096 x 4128 8.8 and 11.2).
-// Groups of few rows on average wait for weights, too: 64x128 tiles (16 groups of 256 rows, 2 x 5120 x 4096: 74.9, walk 79.4; 8 of 512 rows,
-// 4096 x 14336 77.3 and 102), but with a short K the walk, which has no gap between its tiles (128 of 512 rows, 2 x 768 x 2048: 35.5, 64x128 41.6).
+// Groups of few rows on average wait for weights, too: 64x128 tiles (16 groups, 256 rows, 2 x 5120 x 4096 74.0, walk 79.4; 8 groups, 512 rows,
+// 4096 x 14336 77 and 102; 32 groups, 256 rows, 2 x 1024 x 2048 16.4 and 19.1), but for many of a short K the walk, which has no gap between its
+// tiles and no workgroups for tiles that groups might have had (128 groups, 512 rows, 2 x 768 x 2048 35.5, 64x128 41.3).
 Way way_of(int64_t M, int64_t N, int64_t K, int gated, int64_t G, bool grouped, bool scales_aligned) {
   const int64_t cus = device_compute_units(), columns = N * (gated ? 2 : 1);
   auto tiles = [&](int64_t bm, int64_t bn) { return (grouped ? most_row_tiles(M, G, bm) : (M + bm - 1) / bm) * ((columns + bn - 1) / bn); };
@@ -485,7 +486,7 @@ Way way_of(int64_t M, int64_t N, int64_t K, int gated, int64_t G, bool grouped, 
   if (!grouped && tiles(32, 64) <= cus) return k32x64;
   if (tiles(64, 64) <= 2 * cus) return tiles(64, 64) <= cus ? k64x64Long : k64x64;
   const bool short_k = K <= 256, wide = N >= (1 << 25);   // what the walk does not take
-  if (grouped) return M <= 64 || (M <= 64 * G && K >= 4096) || short_k || wide ? k64x128 : kWalk;
+  if (grouped) return M <= 64 || (M <= 64 * G && (K >= 4096 || tiles(64, 128) <= 4 * cus)) || short_k || wide ? k64x128 : kWalk;
   return tiles(128, 128) <= 2 * cus || short_k || wide ? k128x128 : kWalk;
 }
 

@@ -388,7 +388,7 @@ def test_experts(sizes, n, k, gated):
 # row tiles of every number of fragments, groups of no rows at both ends, several rounds.
 TILED_SIZES = [([1, 0, 3, 0] * 10, 900, 288), ([300, 1, 0, 256, 257, 2], 2000, 160), ([300, 1, 0, 256, 257, 2], 2000, 288), ([0] * 70 + [3, 0, 130] + [1] * 70, 400, 512),
                ([1, 0, 2, 0, 0, 1] * 50, 200, 544), ([0, 64, 65, 128, 129, 192, 193, 255, 256, 257, 0], 2000, 512), ([2000, 0, 1500, 513], 4096, 768),
-               ([20, 0, 9, 1], 8320, 4096)]
+               ([20, 0, 9, 1], 8320, 4096), ([0] * 70 + [3, 0, 130] + [1] * 70, 1200, 512), ([1, 0, 2, 0, 0, 1] * 50, 800, 544)]
 
 
 @pytest.mark.parametrize("gated", [False, True])
