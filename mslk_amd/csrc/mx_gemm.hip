@@ -451,7 +451,8 @@ hipError_t launch_walk(const MxProblem& p, hipStream_t s) {
 
 enum Way : int {
   kStream,     // few rows, scales that the DMA cannot take: mx_stream.hip
-  k32x32, k32x64, k64x64Long, k64x64, k128x128,
+  k32x32, k32x64, k64x64Long, k64x64,   // the small ones
+  k128x128,
   k64x128,     // groups only
   kWalk,       // 256-column tiles (at least two steps)
 };
@@ -461,8 +462,8 @@ using Tile64x64Long = MxShape<64, 64, 1, 1, 4>;     // one
 using Tile64x64 = MxShape<64, 64, 1, 1, 2>;         // two
 using Tile64x128 = MxShape<64, 128, 2, 2, 1>;       // two
 using Tile128x128 = MxShape<128, 128, 2, 2, 1>;     // two
-// Scales are fetched by 16 bytes.
-bool fetched_in_place(int64_t K, bool scales_aligned) { return K % 512 == 0 && scales_aligned; }
+// Scales are fetched by 16 bytes of a row, by the small tiles by 4.
+bool fetched_in_place(int64_t K, bool small, bool scales_aligned) { return K % (small ? 128 : 512) == 0 && scales_aligned; }
 
 // The smallest tiles of which each CU gets no more than it holds at once, since their steps' loads, not their products, are waited for.  µs:
 //   16 x 4096 x 14336   32x32 8.3, 32x64 11.7, 64x64 14.3
@@ -474,14 +475,14 @@ bool fetched_in_place(int64_t K, bool scales_aligned) { return K % 512 == 0 && s
 //   500 x 8192 x 4096   128x128 16.4, 64x64 22.1, walk 23.1
 //   1000 x 10240 x 8192 walk 55.2, 128x128 64.9
 // Up to 32 rows whose scales would have to be arranged first take the kernel that needs no such launch, if there is a CU for every 32 columns
-// (32 x 8192 x 8448 11.4, arranged 13.6; 16 x 4096 x 4128 8.8 and 11.2).
+// (16 x 4096 x 4128 8.8, arranged 11.2).
 // Groups of few rows on average wait for weights, too: 64x128 tiles (16 groups, 256 rows, 2 x 5120 x 4096 74.0, walk 79.4; 8 groups, 512 rows,
 // 4096 x 14336 77 and 102; 32 groups, 256 rows, 2 x 1024 x 2048 16.4 and 19.1), but for many of a short K the walk, which has no gap between its
 // tiles and no workgroups for tiles that groups might have had (128 groups, 512 rows, 2 x 768 x 2048 35.5, 64x128 41.3).
 Way way_of(int64_t M, int64_t N, int64_t K, int gated, int64_t G, bool grouped, bool scales_aligned) {
   const int64_t cus = device_compute_units(), columns = N * (gated ? 2 : 1);
   auto tiles = [&](int64_t bm, int64_t bn) { return (grouped ? most_row_tiles(M, G, bm) : (M + bm - 1) / bm) * ((columns + bn - 1) / bn); };
-  if (!grouped && M <= 32 && columns <= 32 * cus && !fetched_in_place(K, scales_aligned)) return kStream;
+  if (!grouped && M <= 32 && columns <= 32 * cus && !fetched_in_place(K, true, scales_aligned)) return kStream;
   if (!grouped && tiles(32, 32) <= (M <= 32 ? 2 : 1) * cus) return k32x32;
   if (!grouped && tiles(32, 64) <= cus) return k32x64;
   if (tiles(64, 64) <= 2 * cus) return tiles(64, 64) <= cus ? k64x64Long : k64x64;
@@ -496,7 +497,7 @@ Way way_of(int64_t M, int64_t N, int64_t K, int gated, int64_t G, bool grouped, 
 // 128 x 128 tiles: two of them to a CU, and a long K (600 x 8192, K = 4096 23.2 / 20.8, 8192 36.9 / 36.3, 14336 57.6 / 61.8; 500 x 10240 x 8192 34.7 / 36.7;
 // one to a CU, 256 x 10240 x 14336 47.8 / 46.1).  Smaller tiles wait for codes.
 bool arranges(Way way, int64_t M, int64_t N, int64_t K, int gated, bool scales_aligned) {
-  if (!fetched_in_place(K, scales_aligned)) return true;
+  if (!fetched_in_place(K, way < k128x128, scales_aligned)) return true;
   const int64_t columns = N * (gated ? 2 : 1), cus = device_compute_units();
   if (way == k128x128) return K >= 8192 && (M + 127) / 128 * ((columns + 127) / 128) > cus;
   return way == kWalk && (double)M * (double)columns * (double)K >= 128. * (double)cus * (256 * 256 * 256);

@@ -11,8 +11,8 @@
 // (Loaded into registers instead, the compiler's wait for them would be one for the DMA loads too, which it does not know of.)  As
 // they lie in the tensor, each row's 16 bytes are a line for the L1 and the L2 to look up, and a pair of a 256 x 256 tile 512 lines next to
 // 1024 of codes: up to 0.28 us per step, where power leaves that to be seen.  Large products have them arranged first, 64 rows to a KiB (MxScales).
-// K's end.  Of a last step of fewer than eight blocks the missing chunks are filled with chunk 0, and their scales are 0, 2^-127, in rows
-// that the caller has padded: products of two such blocks are below 2^-243 and vanish in fp32.
+// K's end.  Of a last step of fewer than eight blocks the missing chunks are filled with chunk 0, and their scales are 0, 2^-127, in arranged
+// rows or by a mask: products of two such blocks are below 2^-243 and vanish in fp32.
 // Products.  v_mfma_scale_f32_32x32x64_f8f6f4, W first: lane (i = l & 31, h = l >> 5) gives row i's chunk 4 h + j to product j of a
 // step, and the four bytes of its scales of the step are those of chunks 4 h ... 4 h + 3: the instruction picks byte j.  Any order of
 // K would do that both operands share; this one needs neither shifts nor shuffles of scales.  Out of registers and on quantized normal
@@ -45,13 +45,14 @@ struct MxShape {
   static constexpr int FM = BM / WM / 32, FN = BN / WN / 32;        // fragments of 32 rows per wave
   static constexpr int X_BYTES = BM * kMxStep, W_BYTES = BN * kMxStep;
   static constexpr int LX = BM / 8 / NW, LW = BN / 8 / NW;          // DMA loads per wave and step
-  // scales of two steps: DMA loads per wave (the rows of X, then of W, 64 rows a load; the last ones may have none)
-  static constexpr int S_X = (BM + 63) / 64 * 64, LS = ((S_X + BN + 63) / 64 + NW - 1) / NW;
-  static constexpr int S_BYTES = LS * NW * 1024;
+  // Scales of two steps: DMA loads per wave (the rows of X, then of W, S_ROWS a load; the last ones may have none).  KS > 1: four bytes a lane, for rows
+  // that begin on four bytes; else 16, a fourth of the loads (with four, 16 groups of 64 rows, gated 5120 x 4096, take 2 % more).
+  static constexpr int S_ROWS = KS > 1 ? 16 : 64, LS = ((BM + BN) / S_ROWS + NW - 1) / NW;
+  static constexpr int S_BYTES = LS * NW * S_ROWS * 16;
   static constexpr int PART_BYTES = 2 * (X_BYTES + W_BYTES + S_BYTES);   // of the waves that share steps
   static constexpr int LDS_BYTES = KS * PART_BYTES;
   static_assert(KS == 1 || NW == 1, "steps are shared, or taken in turn");
-  static_assert(BM % (32 * WM) == 0 && (BN % (64 * WN) == 0 || (KS > 1 && BN == 32)) && BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && (BM + BN) % 32 == 0, "whole fragments and loads");
+  static_assert(BM % (32 * WM) == 0 && (BN % (64 * WN) == 0 || (KS > 1 && BN == 32)) && BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && BM % S_ROWS == 0 && BN % S_ROWS == 0, "whole fragments and loads");
 };
 
 // Scales of a tile: row r of it is row `first` + r behind `base`, which is the first of 64.
@@ -85,7 +86,8 @@ MSLK_AMD_DEVINL v8i mx_operand(v4i a) { return v8i{a[0], a[1], a[2], a[3], 0, 0,
 template <typename TS, bool GATED>
 struct MxTile {
   uint32_t x_off[TS::LX], w_off[TS::LW];   // of this lane's chunk of a load, step 0
-  uint32_t s_off[TS::LS];                  // of this lane's 16 bytes of scales, relative to xs or ws
+  uint32_t s_off[TS::LS];                  // of this lane's scales, relative to xs or ws
+  uint32_t s_last;                         // which bytes of a word of scales of the last step are those of its blocks
   MxOperands o;
 
   // Of a wave: its place among those that share a step, and which step of KS it takes.
@@ -116,6 +118,8 @@ struct MxTile {
     o.xs.base = uniform_ptr(o.xs.base);
     o.ws.base = uniform_ptr(o.ws.base);
     const int lane = threadIdx.x & 63, wave = wave_id();
+    const int mine = o.last_chunks - 4 * (lane >> 5);
+    s_last = mine >= 4 ? ~0u : mine <= 0 ? 0u : (1u << (8 * mine)) - 1;
 #pragma unroll
     for (int q = 0; q < TS::LX; ++q) {   // rows beyond the valid ones read the last valid one again: their sums are not stored
       const int r = x_load_row(q) + (lane >> 3);
@@ -130,14 +134,15 @@ struct MxTile {
     }
 #pragma unroll
     for (int i = 0; i < TS::LS; ++i) {   // the list of LDS rows of X, then of W
-      const int r = (wave * TS::LS + i) * 64 + lane;
+      const int r = (wave * TS::LS + i) * TS::S_ROWS + lane * TS::S_ROWS / 64;
       bool up = false;
-      if (r >= TS::S_X) {
-        const int row = min(w_row(min(r - TS::S_X, TS::BN - 1), up), o.rows_w - 1);
+      if (r >= TS::BM) {
+        const int row = min(w_row(min(r - TS::BM, TS::BN - 1), up), o.rows_w - 1);
         s_off[i] = o.ws.offset(row + (up ? (int)o.up_rows : 0));
       } else {
-        s_off[i] = o.xs.offset(min(x_row(min(r, TS::BM - 1)), o.rows_x - 1));
+        s_off[i] = o.xs.offset(min(x_row(r), o.rows_x - 1));
       }
+      if (TS::S_ROWS == 16) s_off[i] += (lane & 3) * 4;
     }
   }
 
@@ -153,12 +158,19 @@ struct MxTile {
     const int chunks = kt + 1 < o.steps ? 8 : o.last_chunks;
     return Adjust{c < chunks ? 0u : (uint32_t)(-16 * c), (c ^ 4) < chunks ? 0u : (uint32_t)(-16 * (c ^ 4))};
   }
-  // Load i of the scales of steps 2 pair and 2 pair + 1 into `stage`.
+  // Load i of the scales of steps 2 pair and 2 pair + 1 into `stage`; lanes of words behind the last block go back to the pair's first word.
   MSLK_AMD_DEVINL void copy_scales(char* stage, int pair, int i) {
     const int64_t from = (int64_t)pair * o.xs.pair_stride;   // (the same for both)
-    const int wave = wave_id();
-    char* dst = stage + (wave * TS::LS + i) * 1024;
-    dma16(uniform_ptr(((wave * TS::LS + i) * 64 >= TS::S_X ? o.ws.base : o.xs.base) + from), s_off[i], dst);
+    const int load = wave_id() * TS::LS + i, word = threadIdx.x & 3, blocks = (o.steps - 1 - 2 * pair) * 8 + o.last_chunks;
+    const uint8_t* base = uniform_ptr((load * TS::S_ROWS >= TS::BM ? o.ws.base : o.xs.base) + from);
+    char* const dst = stage + load * TS::S_ROWS * 16;
+    if constexpr (TS::S_ROWS == 16) dma4(base, s_off[i] + (word * 4 < blocks ? 0u : (uint32_t)(-4 * word)), dst);
+    else dma16(base, s_off[i], dst);
+  }
+  // Global -> LDS copy of four bytes per lane, as dma16().
+  MSLK_AMD_DEVINL static void dma4(const uint8_t* base, uint32_t off, char* lds_wave_base) {
+    const uint32_t dst = (uint32_t)(uintptr_t)(lds_ptr_t)lds_wave_base;
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" : : "v"(off), "s"(base), "s"(dst) : "memory", "m0");
   }
 
   // At most `PENDING` of this wave's youngest loads are in flight and its LDS accesses are done; then the workgroup's barrier.
@@ -190,7 +202,7 @@ struct MxTile {
 #pragma unroll
     for (int tm = 0; tm < TS::FM; ++tm) sx[tm] = *reinterpret_cast<const uint32_t*>(at + (tm * TS::WM + wave / TS::WN) * 512);
 #pragma unroll
-    for (int tn = 0; tn < TS::FN; ++tn) sw[tn] = *reinterpret_cast<const uint32_t*>(at + TS::S_X * 16 + (tn * TS::WN + wave % TS::WN) * 512);
+    for (int tn = 0; tn < TS::FN; ++tn) sw[tn] = *reinterpret_cast<const uint32_t*>(at + TS::BM * 16 + (tn * TS::WN + wave % TS::WN) * 512);
   }
   template <int J>
   MSLK_AMD_DEVINL static void multiply(const v4i& wf, const v4i& xf, uint32_t sw, uint32_t sx, v16f& acc) {
@@ -234,6 +246,13 @@ struct MxTile {
       if (t + 2 < turns) {
         wait<63>();   // for the reads: the stage is free
         fetch(t + 2);
+      }
+      if constexpr (TS::S_ROWS == 16) {
+        const uint32_t there = 2 * (turn_id() + (t >> 1) * TS::KS) + (t & 1) + 1 == o.steps ? s_last : ~0u;
+#pragma unroll
+        for (int tm = 0; tm < TS::FM; ++tm) sx[tm] &= there;
+#pragma unroll
+        for (int tn = 0; tn < TS::FN; ++tn) sw[tn] &= there;
       }
       auto product = [&](auto j) {
         constexpr int J = decltype(j)::value;

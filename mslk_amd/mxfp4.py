@@ -9,8 +9,8 @@ of two.  Codes are bytes [.., K / 2] with the earlier value in the low half (uin
 bytes s [.., K / 32] that stand for 2^(s - 127), 255 for NaN (uint8 or torch.float8_e8m0fnu): the layouts of the OCP microscaling
 specification, so weights quantized elsewhere can be used as they are.  Products take both operands so, sum in fp32 and round once.
 
-Nothing here is differentiable.  Codes have to be contiguous; a K that is no multiple of 512 (and scales that do not begin on 16 bytes)
-costs a copy of the scales in each call.
+Nothing here is differentiable.  Codes have to be contiguous; a K that is no multiple of 512 (for few rows, 128) or scales that do not
+begin on 16 bytes cost a copy of the scales in each call.
 """
 from __future__ import annotations
 

@@ -279,7 +279,8 @@ TILED = [(5, 9000, 288), (32, 8200, 96), (40, 2000, 1280), (128, 1024, 2336), (7
          (1100, 2000, 224), (1100, 2000, 512), (1025, 2056, 1312), (1, 40000, 64), (2600, 7000, 256),
          (1500, 6000, 288), (1472, 6144, 512), (2600, 7000, 544), (4100, 4200, 800), (4240, 4096, 1024), (4050, 4360, 1056), (3, 70000, 512), (40, 66000, 320),
          (8, 300, 8224), (16, 2000, 5152), (32, 100, 12320), (9, 40, 4128),
-         (100, 2600, 1312), (64, 8192, 544), (97, 2621, 2048), (128, 4096, 512), (100, 2602, 64), (32, 16384, 512), (30, 16380, 1056)]   # (then: weights streamed, several rounds of pairs; 32 x 64 tiles again; as many 32 x 32 ones as there can be)
+         (100, 2600, 1312), (64, 8192, 544), (97, 2621, 2048), (128, 4096, 512), (100, 2602, 64), (32, 16384, 512), (30, 16380, 1056),
+         (17, 130, 128), (33, 300, 384), (128, 1024, 2432), (100, 2600, 1408), (300, 1000, 640), (520, 1104, 1920), (2, 2000, 11008)]   # (then: weights streamed, several rounds of pairs; 32 x 64 tiles again; as many 32 x 32 ones as there can be; scales by four bytes, to every end of a pair)
 
 
 @pytest.mark.parametrize("m,n,k", TILED)
