@@ -6,7 +6,10 @@
 //
 // Both are bound by memory.  A lane holds 8 values (16 bytes of 16-bit ones), so that a wave reads and writes whole lines; four
 // neighbouring lanes are a block and find its maximum by data-parallel moves, on the bits, where NaN > infinity > numbers.
-// 8192 x 28672 bf16 values: 134 us there (4.4 TB/s read and written) and 88 back (6.8: the codes are still in the Infinity Cache).
+// Values of half of the Infinity Cache and more go past the caches (STREAM), there and back: 8192 x 28672 bf16 values take 178 us in all instead of 224
+// (6.7 TB/s read and written: the codes stay in the cache between the two), 8192 x 8192 55 instead of 60.  Fewer are left where a reader may find them.
+#include <type_traits>
+
 #include "mx.h"
 #include "quant_math.h"
 
@@ -15,17 +18,36 @@ namespace {
 
 constexpr int kThreads = 256;
 
-template <int DTYPE> struct Elements { typedef uint16_t type; };
-template <> struct Elements<2> { typedef float type; };
+// Words: 16 bytes of elements, which begin on any element.
+template <int DTYPE> struct Elements {
+  typedef uint16_t type;
+  typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(2)));
+};
+template <> struct Elements<2> {
+  typedef float type;
+  typedef uint32_t Words __attribute__((ext_vector_type(4), aligned(4)));
+};
 
-// 8 consecutive values as fp32.  No promise of alignment: the compiler picks the widest load the target allows.
-template <int DTYPE>
+constexpr int64_t kStreamBytes = int64_t(1) << 27;
+
+// 8 consecutive values as fp32.
+template <int DTYPE, bool STREAM>
 MSLK_AMD_DEVINL void load8(const typename Elements<DTYPE>::type* p, float (&v)[8]) {
+  typedef typename Elements<DTYPE>::Words Words;
+  auto load4 = [&](int at) {
+    const Words* from = reinterpret_cast<const Words*>(p) + at;
+    if constexpr (STREAM) return __builtin_nontemporal_load(from);
+    else return *from;
+  };
   if constexpr (DTYPE == 2) {
-    __builtin_memcpy(v, p, 32);
+    const Words lo = load4(0), hi = load4(1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = __uint_as_float(lo[i]);
+      v[4 + i] = __uint_as_float(hi[i]);
+    }
   } else {
-    uint32_t w[4];
-    __builtin_memcpy(w, p, 16);
+    const Words w = load4(0);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       v[2 * i] = Traits<DTYPE>::to_f32(w[i] & 0xFFFFu);
@@ -41,7 +63,7 @@ MSLK_AMD_DEVINL uint32_t max_of_4_lanes(uint32_t m) {
 
 // U vectors of 8 values per lane, kThreads vectors apart, all loads in front of the arithmetic.  Vector v of the launch is vector
 // v % per_row of row v / per_row; FLAT: rows follow one another without a gap.
-template <int DTYPE, int U, bool FLAT>
+template <int DTYPE, int U, bool FLAT, bool STREAM>
 __global__ __launch_bounds__(kThreads) void quantize_kernel(const typename Elements<DTYPE>::type* __restrict__ a, int64_t row_stride, uint32_t per_row,
                                                             int64_t vectors, uint32_t* __restrict__ codes, uint8_t* __restrict__ scales) {
   const int64_t first = (int64_t)blockIdx.x * (kThreads * U) + threadIdx.x;
@@ -55,7 +77,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const typename Eleme
         const uint32_t row = (uint32_t)i / per_row;   // (launches of rows with gaps are cut below 2^32 vectors)
         at = row * row_stride + (int64_t)((uint32_t)i - row * per_row) * 8;
       }
-      load8<DTYPE>(a + at, v[u]);
+      load8<DTYPE, STREAM>(a + at, v[u]);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[u][e] = 0.f;
@@ -84,7 +106,7 @@ __global__ __launch_bounds__(kThreads) void quantize_kernel(const typename Eleme
   }
 }
 
-template <int DTYPE, int U>
+template <int DTYPE, int U, bool STREAM>
 __global__ __launch_bounds__(kThreads) void dequantize_kernel(const uint32_t* __restrict__ codes, const uint8_t* __restrict__ scales, int64_t vectors,
                                                               void* __restrict__ out) {
   const int64_t first = (int64_t)blockIdx.x * (kThreads * U) + threadIdx.x;
@@ -109,25 +131,35 @@ __global__ __launch_bounds__(kThreads) void dequantize_kernel(const uint32_t* __
     two(2, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[u], 1.f, 1));
     two(4, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[u], 1.f, 2));
     two(6, __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c[u], 1.f, 3));
+    typedef uint32_t Words __attribute__((ext_vector_type(4)));
+    auto store4 = [&](int64_t at, Words w) {
+      Words* to = static_cast<Words*>(out) + at;
+      if constexpr (STREAM) __builtin_nontemporal_store(w, to);
+      else *to = w;
+    };
     if constexpr (DTYPE == 2) {
-      float4* o = static_cast<float4*>(out) + 2 * i;
-      o[0] = make_float4(v[0], v[1], v[2], v[3]);
-      o[1] = make_float4(v[4], v[5], v[6], v[7]);
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        store4(2 * i + h, Words{__float_as_uint(v[4 * h]), __float_as_uint(v[4 * h + 1]), __float_as_uint(v[4 * h + 2]), __float_as_uint(v[4 * h + 3])});
     } else {
-      static_cast<uint4*>(out)[i] = make_uint4(pack_out_x2<DTYPE == 1>(v[0], v[1]), pack_out_x2<DTYPE == 1>(v[2], v[3]),
-                                               pack_out_x2<DTYPE == 1>(v[4], v[5]), pack_out_x2<DTYPE == 1>(v[6], v[7]));
+      store4(i, Words{pack_out_x2<DTYPE == 1>(v[0], v[1]), pack_out_x2<DTYPE == 1>(v[2], v[3]), pack_out_x2<DTYPE == 1>(v[4], v[5]),
+                      pack_out_x2<DTYPE == 1>(v[6], v[7])});
     }
   }
 }
 
-// Calls f(first vector, vectors, vectors per lane) for launches that HIP takes (fewer than 2^32 work-items): four vectors per lane
-// keep enough loads in flight, where that still makes a workgroup for every CU.
+// Calls f(first vector, vectors, vectors per lane, whether they are streamed) for launches that HIP takes (fewer than 2^32 work-items): four vectors
+// per lane keep enough loads in flight, where that still makes a workgroup for every CU.  bytes: of all values.
 template <typename F>
-hipError_t in_launches(int64_t vectors, F f) {
+hipError_t in_launches(int64_t vectors, int64_t bytes, F f) {
   constexpr int64_t kMost = int64_t(1) << 31;   // a multiple of all that a launch is divided into
   for (int64_t at = 0; at < vectors; at += kMost) {
     const int64_t n = vectors - at < kMost ? vectors - at : kMost;
-    f(at, n, n > 4 * 256 * kThreads ? 4 : 1);
+    const std::integral_constant<int, 1> one{};
+    const std::integral_constant<int, 4> four{};
+    if (n <= 4 * 256 * kThreads) f(at, n, one, std::false_type{});
+    else if (bytes < kStreamBytes) f(at, n, four, std::false_type{});
+    else f(at, n, four, std::true_type{});
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
   return hipSuccess;
@@ -138,30 +170,27 @@ template <int DTYPE>
 hipError_t quantize(const void* a, int64_t rows, int64_t K, int64_t row_stride, uint32_t* codes, uint8_t* scales, hipStream_t s) {
   typedef typename Elements<DTYPE>::type T;
   const T* x = static_cast<const T*>(a);
-  const int64_t per_row = K / 8;
+  const int64_t per_row = K / 8, bytes = rows * K * (int64_t)sizeof(T);
   if (row_stride == K || rows == 1)
-    return in_launches(rows * per_row, [&](int64_t at, int64_t n, int u) {
-      if (u == 4) quantize_kernel<DTYPE, 4, true><<<blocks(n, 4), kThreads, 0, s>>>(x + at * 8, 0, 1, n, codes + at, scales + at / 4);
-      else quantize_kernel<DTYPE, 1, true><<<blocks(n, 1), kThreads, 0, s>>>(x + at * 8, 0, 1, n, codes + at, scales + at / 4);
+    return in_launches(rows * per_row, bytes, [&](int64_t at, int64_t n, auto u, auto stream) {
+      quantize_kernel<DTYPE, u, true, stream><<<blocks(n, u), kThreads, 0, s>>>(x + at * 8, 0, 1, n, codes + at, scales + at / 4);
     });
   const int64_t most = (int64_t(1) << 31) / per_row;   // rows of a launch; K < 2^31
   for (int64_t r = 0; r < rows; r += most) {
-    const int64_t n = (rows - r < most ? rows - r : most) * per_row, at = r * per_row;
-    if (n > 4 * 256 * kThreads)
-      quantize_kernel<DTYPE, 4, false><<<blocks(n, 4), kThreads, 0, s>>>(x + r * row_stride, row_stride, (uint32_t)per_row, n, codes + at, scales + at / 4);
-    else
-      quantize_kernel<DTYPE, 1, false><<<blocks(n, 1), kThreads, 0, s>>>(x + r * row_stride, row_stride, (uint32_t)per_row, n, codes + at, scales + at / 4);
-    if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
+    const int64_t first = r * per_row;
+    const hipError_t e = in_launches((rows - r < most ? rows - r : most) * per_row, bytes, [&](int64_t, int64_t n, auto u, auto stream) {
+      quantize_kernel<DTYPE, u, false, stream><<<blocks(n, u), kThreads, 0, s>>>(x + r * row_stride, row_stride, (uint32_t)per_row, n, codes + first, scales + first / 4);
+    });
+    if (e != hipSuccess) return e;
   }
   return hipSuccess;
 }
 
 template <int DTYPE>
 hipError_t dequantize(const uint32_t* codes, const uint8_t* scales, int64_t vectors, void* out, hipStream_t s) {
-  return in_launches(vectors, [&](int64_t at, int64_t n, int u) {
-    char* o = static_cast<char*>(out) + at * (DTYPE == 2 ? 32 : 16);
-    if (u == 4) dequantize_kernel<DTYPE, 4><<<blocks(n, 4), kThreads, 0, s>>>(codes + at, scales + at / 4, n, o);
-    else dequantize_kernel<DTYPE, 1><<<blocks(n, 1), kThreads, 0, s>>>(codes + at, scales + at / 4, n, o);
+  const int64_t each = DTYPE == 2 ? 32 : 16;
+  return in_launches(vectors, vectors * each, [&](int64_t at, int64_t n, auto u, auto stream) {
+    dequantize_kernel<DTYPE, u, stream><<<blocks(n, u), kThreads, 0, s>>>(codes + at, scales + at / 4, n, static_cast<char*>(out) + at * each);
   });
 }
 

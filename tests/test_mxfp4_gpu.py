@@ -133,6 +133,19 @@ def test_quantize_more_than_one_vector_per_lane():
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_many_values_at_once_and_in_parts(dtype):
+    """Those of 2^27 bytes and more, which go past the caches, in one piece and with gaps between the rows, against parts of them."""
+    gen = torch.Generator(DEV).manual_seed(6)
+    whole = torch.randn(16500, 4130, generator=gen, device=DEV).to(dtype)
+    for a in (whole[:, :4128].contiguous(), whole[:, 1:4129]):
+        codes, scales = mslk_amd.quantize_mxfp4(a)
+        parts = [mslk_amd.quantize_mxfp4(p) for p in a.split(1500)]
+        assert torch.equal(codes, torch.cat([p[0] for p in parts])) and torch.equal(scales, torch.cat([p[1] for p in parts]))
+    assert torch.equal(mslk_amd.dequantize_mxfp4(codes, scales, dtype), torch.cat([mslk_amd.dequantize_mxfp4(*p, dtype) for p in parts]))
+    check_quantized(a[8000:8050])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("shape", [(1, 32), (7, 96), (300, 8192), (2, 3, 64), (0, 32)])
 def test_dequantize(shape, dtype):
     codes, scales = operand(shape[:-1], shape[-1], rng(11), low=120, high=134)
