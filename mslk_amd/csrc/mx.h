@@ -19,7 +19,8 @@ hipError_t launch_quantize_mxfp4(const void* a, int dtype, int64_t rows, int64_t
 hipError_t launch_dequantize_mxfp4(const void* codes, const void* scales, int64_t rows, int64_t K, void* out, int dtype, hipStream_t s);
 
 // Where scales lie: those of row r, blocks 16 p ... 16 p + 15 are the 16 bytes at data + (r / 64) * block + (r % 64) * row + p * pair_stride,
-// all multiples of 16.  A tensor's own: row = K / 32, block = 64 row, pair_stride = 16.  Arranged: [rows / 64][pairs][64][16], blocks beyond K 0.
+// all multiples of 16 (for the small tiles, of 4).  A tensor's own: row = K / 32, block = 64 row, pair_stride = 16.  Arranged: [rows / 64][pairs][64][16],
+// blocks beyond K 0.
 struct MxScales {
   const uint8_t* data;
   int64_t block;

@@ -474,6 +474,8 @@ bool fetched_in_place(int64_t K, bool small, bool scales_aligned) { return K % (
 //   256 x 8192 x 8192   64x64 of two waves 19.7 (four 24.8), 128x128 27.0
 //   500 x 8192 x 4096   128x128 16.4, 64x64 22.1, walk 23.1
 //   1000 x 10240 x 8192 walk 55.2, 128x128 64.9
+// Two 128x128 tiles to a CU only with a short K: 1000 x 8192 x 1024 8.9 (walk 11.3), 500 x 14336 x 2048 13.6 (15.5), 500 x 10240 x 4096 20.9 (21.1),
+// 500 x 10240 x 8192 37.0 (36.0), 2000 x 4096 x 14336 69.7 (64.7); one to a CU 500 x 8192 x 8192 28.4 (33.0).
 // Up to 32 rows whose scales would have to be arranged first take the kernel that needs no such launch, if there is a CU for every 32 columns
 // (16 x 4096 x 4128 8.8, arranged 11.2).
 // Groups of few rows on average wait for weights, too: 64x128 tiles (16 groups, 256 rows, 2 x 5120 x 4096 74.0, walk 79.4; 8 groups, 512 rows,
@@ -488,19 +490,17 @@ Way way_of(int64_t M, int64_t N, int64_t K, int gated, int64_t G, bool grouped, 
   if (tiles(64, 64) <= 2 * cus) return tiles(64, 64) <= cus ? k64x64Long : k64x64;
   const bool short_k = K <= 256, wide = N >= (1 << 25);   // what the walk does not take
   if (grouped) return M <= 64 || (M <= 64 * G && (K >= 4096 || tiles(64, 128) <= 4 * cus)) || short_k || wide ? k64x128 : kWalk;
-  return tiles(128, 128) <= 2 * cus || short_k || wide ? k128x128 : kWalk;
+  return tiles(128, 128) <= (K < 4096 ? 2 : 1) * cus || short_k || wide ? k128x128 : kWalk;
 }
 
 // Whether the scales are arranged first.  If they can be fetched in place, the launch in front has to be worth it.
 // The walk: from 128 steps of 256 x 256 sums per CU on (arranged / in place, us: 4096 x 4096 x 4096 43.4 / 41.4, 16 experts, 2048 rows, 8192 x 5120
 // 126 / 119, 8192 x 8192 x 2048 92 / 91, 8192 x 8192 x 8192 263 / 265, 16384 x 8192 x 16384 938 / 959, 16 experts, 32768 rows 756 / 774).
-// 128 x 128 tiles: two of them to a CU, and a long K (600 x 8192, K = 4096 23.2 / 20.8, 8192 36.9 / 36.3, 14336 57.6 / 61.8; 500 x 10240 x 8192 34.7 / 36.7;
-// one to a CU, 256 x 10240 x 14336 47.8 / 46.1).  Smaller tiles wait for codes.
+// Tiles of fewer rows wait for codes, or have few steps.
 bool arranges(Way way, int64_t M, int64_t N, int64_t K, int gated, bool scales_aligned) {
   if (!fetched_in_place(K, way < k128x128, scales_aligned)) return true;
-  const int64_t columns = N * (gated ? 2 : 1), cus = device_compute_units();
-  if (way == k128x128) return K >= 8192 && (M + 127) / 128 * ((columns + 127) / 128) > cus;
-  return way == kWalk && (double)M * (double)columns * (double)K >= 128. * (double)cus * (256 * 256 * 256);
+  const double products = (double)M * (double)(N * (gated ? 2 : 1)) * (double)K;
+  return way == kWalk && products >= 128. * device_compute_units() * (256 * 256 * 256);
 }
 
 }  // namespace
