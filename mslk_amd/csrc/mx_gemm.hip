@@ -27,6 +27,24 @@ MSLK_AMD_DEVINL void load_bias(const MxProblem& p, int n, int h, float (&b)[8]) 
   for (int e = 0; e < 8; ++e) b[e] = __uint_as_float(v[e]);
 }
 
+// Columns n ... n + 7 of the bias, which differ from lane to lane and may end; vectors: the bias and its columns in eights lie on 16 bytes.
+MSLK_AMD_DEVINL void load_bias_columns(const MxProblem& p, int n, bool vectors, float (&b)[8]) {
+  if (vectors && p.bias_dtype == 1) {
+    const float4* at = reinterpret_cast<const float4*>(static_cast<const float*>(p.bias) + min(n, p.N - 8));
+    const float4 lo = at[0], hi = at[1];
+    b[0] = lo.x; b[1] = lo.y; b[2] = lo.z; b[3] = lo.w;
+    b[4] = hi.x; b[5] = hi.y; b[6] = hi.z; b[7] = hi.w;
+  } else if (vectors) {
+    const uint4 two = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p.bias) + min(n, p.N - 8));
+    const uint32_t v[4] = {two.x, two.y, two.z, two.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b[e] = bf16_bits_to_f32((v[e >> 1] >> (16 * (e & 1))) & 0xFFFFu);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) b[e] = bias_at(p, min(n + e, p.N - 1));
+  }
+}
+
 // As store16_stream(), at a scalar base and a lane's offset.  (The data registers may be reused behind the statement: its wait states.)
 MSLK_AMD_DEVINL void store16_at(char* base, uint32_t off, uint4 val) {
   const v4i v = {(int)val.x, (int)val.y, (int)val.z, (int)val.w};
@@ -53,10 +71,15 @@ MSLK_AMD_DEVINL void store_tile(const MxProblem& p, const v16f (&acc)[FN][FM], i
   const uint32_t lane_off = 2u * ((uint32_t)row8 * (uint32_t)p.N + (uint32_t)column(0, piece, h));
 #pragma unroll
   for (int t = 0; t < LINES; ++t) {
+    // (Of the large tile's last rows and columns the bias is read where it is added: there are no registers to hold it.)
+    constexpr bool HELD = BIAS && (FULL || FM * FN <= 4);
     float b[4][8];
-    if constexpr (BIAS && FULL) {
+    if constexpr (HELD) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) load_bias(p, first + column(t, r, 0), h, b[r]);
+      for (int r = 0; r < 4; ++r) {
+        if constexpr (FULL) load_bias(p, first + column(t, r, 0), h, b[r]);
+        else load_bias_columns(p, first + column(t, r, h), (p.N & 7) == 0 && (reinterpret_cast<uintptr_t>(p.bias) & 15) == 0, b[r]);
+      }
     }
 #pragma unroll
     for (int tm = 0; tm < FM; ++tm) {
@@ -73,7 +96,7 @@ MSLK_AMD_DEVINL void store_tile(const MxProblem& p, const v16f (&acc)[FN][FM], i
             v[e] = r < PIECES ? gated_value(acc[2 * T][tm][at], acc[2 * T + 1][tm][at]) : 0.f;
           } else {
             v[e] = acc[2 * t + (e >> 2)][tm][4 * r + (e & 3)];
-            if constexpr (BIAS && FULL) v[e] += b[r][e];
+            if constexpr (HELD) v[e] += b[r][e];
             else if constexpr (BIAS) v[e] += bias_at(p, min(first + column(t, r, h) + e, p.N - 1));
           }
         }
