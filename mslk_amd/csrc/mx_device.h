@@ -9,9 +9,22 @@ namespace {
 constexpr int kXcds = 8;
 constexpr int kPanel = 4;   // row tiles that share the weights of a panel in an XCD's L2
 
-// y = silu(gate) * up in fp32.  For gates below -88 exp(-gate) is infinite and the result -0, as it should be; the exponential and the
-// reciprocal are good to about 2 units of fp32, far below the rounding to 16 bits that follows.
-MSLK_AMD_DEVINL float gated_value(float gate, float up) { return gate * __builtin_amdgcn_rcpf(1.f + __expf(-gate)) * up; }
+// y = silu(gate) * up in fp32, silu(gate) = gate / (1 + exp(-gate)).  exp(-gate) is off by |gate| 2^-24 of itself (its argument times log2(e), rounded) and
+// about two units, the reciprocal by one: far below the rounding to 16 bits that follows, as |gate| is below 2^7 here.
+// Below -87 the reciprocal is no normal number any more, and from -88.7 on exp(-gate) is infinite, but up may bring the product back into range (gate -90,
+// up 1e30: -7e-8).  There silu(gate) = gate exp(gate) to the last bit; exp(gate) = 2^n 2^f, |f| <= 1/2, and 2^n is multiplied to up first.
+// FAR: some gate may be that far.  Callers look at all gates of a lane (far_gates()) and make their values again if one of the wave's is.
+template <bool FAR>
+MSLK_AMD_DEVINL float gated_value(float gate, float up) {
+  const float near = gate * __builtin_amdgcn_rcpf(1.f + __expf(-gate)) * up;
+  if constexpr (!FAR) return near;
+  constexpr float kLog2e = 1.44269504088896340736f;
+  const float x = fmaxf(gate, -1000.f), n = rintf(x * kLog2e);   // (what is below -1000 ends at 0 all the same; -infinity times that is NaN)
+  return gate < -87.f ? gate * __builtin_amdgcn_exp2f(fmaf(x, kLog2e, -n)) * ldexpf(up, (int)n) : near;
+}
+// The largest bits of gates seen: those of -87 are below those of every smaller number.
+MSLK_AMD_DEVINL uint32_t farther(uint32_t most, float gate) { return max(most, __float_as_uint(gate)); }
+MSLK_AMD_DEVINL bool far_gates(uint32_t most) { return __builtin_expect(__any(most > 0xC2AE0000u), 0); }
 
 MSLK_AMD_DEVINL float bias_at(const MxProblem& p, int n) {
   return p.bias_dtype == 1 ? static_cast<const float*>(p.bias)[n] : bf16_bits_to_f32(static_cast<const uint16_t*>(p.bias)[n]);

@@ -85,24 +85,29 @@ MSLK_AMD_DEVINL void store_tile(const MxProblem& p, const v16f (&acc)[FN][FM], i
     for (int tm = 0; tm < FM; ++tm) {
       const int row0 = wm * WAVE_ROW + tm * FRAG_ROW;
       if (!FULL && row0 >= rows) break;
-      uint32_t w[4][4];
+      uint32_t w[4][4], gates = 0;
+      auto values = [&](auto far) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float v[8];
+        for (int r = 0; r < 4; ++r) {
+          float v[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if constexpr (GATED) {
-            const int T = t * 2 + (r >> 1), at = 8 * (r & 1) + e;
-            v[e] = r < PIECES ? gated_value(acc[2 * T][tm][at], acc[2 * T + 1][tm][at]) : 0.f;
-          } else {
-            v[e] = acc[2 * t + (e >> 2)][tm][4 * r + (e & 3)];
-            if constexpr (HELD) v[e] += b[r][e];
-            else if constexpr (BIAS) v[e] += bias_at(p, min(first + column(t, r, h) + e, p.N - 1));
+          for (int e = 0; e < 8; ++e) {
+            if constexpr (GATED) {
+              const int T = t * 2 + (r >> 1), at = 8 * (r & 1) + e;
+              v[e] = r < PIECES ? gated_value<decltype(far)::value>(acc[2 * T][tm][at], acc[2 * T + 1][tm][at]) : 0.f;
+              if (r < PIECES) gates = farther(gates, acc[2 * T][tm][at]);
+            } else {
+              v[e] = acc[2 * t + (e >> 2)][tm][4 * r + (e & 3)];
+              if constexpr (HELD) v[e] += b[r][e];
+              else if constexpr (BIAS) v[e] += bias_at(p, min(first + column(t, r, h) + e, p.N - 1));
+            }
           }
-        }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[r][e] = pack_out_x2<F16>(v[2 * e], v[2 * e + 1]);
-      }
+          for (int e = 0; e < 4; ++e) w[r][e] = pack_out_x2<F16>(v[2 * e], v[2 * e + 1]);
+        }
+      };
+      values(std::false_type{});
+      if (GATED && far_gates(gates)) values(std::true_type{});
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
 #pragma unroll
@@ -158,11 +163,19 @@ MSLK_AMD_DEVINL void store_fragment(const MxProblem& p, const v16f& acc, int m0,
     const int n = n0 + 8 * q + 4 * h;
     if (n >= p.N) continue;
     float v[4];
+    uint32_t gates = 0;
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       v[r] = acc[4 * q + r];
-      if constexpr (GATED) v[r] = gated_value(v[r], acc[4 * q + 8 + r]);
+      if constexpr (GATED) {
+        gates = farther(gates, acc[4 * q + r]);
+        v[r] = gated_value<false>(acc[4 * q + r], acc[4 * q + 8 + r]);
+      }
       if constexpr (BIAS) v[r] += bias_at(p, min(n + r, p.N - 1));
+    }
+    if (GATED && far_gates(gates)) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[r] = gated_value<true>(acc[4 * q + r], acc[4 * q + 8 + r]);
     }
     const uint32_t w[2] = {pack_out_x2<F16>(v[0], v[1]), pack_out_x2<F16>(v[2], v[3])};
     uint16_t* dst = p.y + (int64_t)(m0 + m) * p.N + n;

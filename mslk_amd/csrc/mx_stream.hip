@@ -127,9 +127,17 @@ MSLK_AMD_DEVINL void stream_tile(const MxProblem& p, char* lds, int m0, int rows
     if (n >= p.N) continue;
     v4f v = total(m, piece);
     if constexpr (GATED) {
-      const v4f up = total(m, piece + 4);
+      const v4f gate = v, up = total(m, piece + 4);
+      uint32_t gates = 0;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = gated_value(v[r], up[r]);
+      for (int r = 0; r < 4; ++r) {
+        gates = farther(gates, gate[r]);
+        v[r] = gated_value<false>(gate[r], up[r]);
+      }
+      if (far_gates(gates)) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = gated_value<true>(gate[r], up[r]);
+      }
     } else if (p.bias_dtype != 0) {
 #pragma unroll
       for (int r = 0; r < 4; ++r) v[r] += bias_at(p, min(n + r, p.N - 1));
