@@ -397,7 +397,7 @@ int mslk_amd_dequantize_mxfp4(const void* codes, const void* scales, int64_t row
  *   workspace: mslk_amd_mxfp4_mm_workspace_bytes() of it, 16-byte aligned; `aligned` != 0 says that both scale pointers are 16-byte
  *   aligned.  Nothing in it is kept from one call to the next.
  * grouped: row g of the stacked weights wq [G, N or 2 N, K / 2], w_scale [G, N or 2 N, K / 32] belongs to the next m_sizes[g] rows of X
- *   (int64, device memory).  Rows beyond the sum of the sizes are left untouched; sizes below 0 count as 0.
+ *   (int64, device memory); G <= 2^30.  Rows beyond the sum of the sizes are left untouched; sizes below 0 count as 0.
  */
 size_t mslk_amd_mxfp4_mm_workspace_bytes(int64_t M, int64_t N, int64_t K, int gated, int aligned);
 int mslk_amd_mxfp4_mm(const void* xq, const void* wq, const void* x_scale, const void* w_scale, const void* bias, int bias_dtype,

@@ -133,6 +133,7 @@ int check_mx(const char* op, const void* xq, const void* wq, const void* x_scale
   if (M < 0 || N < 0 || K < 0 || G < 0) return fail("%s: negative dimension", op);
   if (K % 32 != 0) return fail("%s: K must be a multiple of 32 (got %lld)", op, (long long)K);
   if (M > kIntMax || N > kIntMax || K >= (int64_t(1) << 24)) return fail("%s: dimension out of range (M, N < 2^31, K < 2^24)", op);
+  if (G > (1 << 30)) return fail("%s: at most 2^30 groups (got %d)", op, G);   // (kernels count them in steps of 64)
   if (gated && (N + 256) * K >= (int64_t(1) << 33)) return fail("%s: gated weights of N = %lld, K = %lld are too large (N K < 2^33)", op, (long long)N, (long long)K);
   if (y_dtype != MSLK_AMD_DTYPE_BF16 && y_dtype != MSLK_AMD_DTYPE_F16) return fail("%s: bf16 or fp16 output expected (dtype code %d)", op, y_dtype);
   if (M == 0 || N == 0 || G == 0) return 0;
