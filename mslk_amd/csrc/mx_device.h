@@ -46,6 +46,8 @@ MSLK_AMD_DEVINL int entry_of(int wg, int total) {
 
 // Group and tile of entry t among the row tiles of all groups (R_g = ceil(size / BM) each) times tiles_n.  Returns false behind the
 // last one.  Every lane takes part.
+template <int BM>
+MSLK_AMD_DEVINL int row_tiles_of(int rows) { return (int)(((uint32_t)rows + (BM - 1)) / BM); }   // (rows may be 2^31 - 1)
 struct GroupTile { int g, row0, rows, tm, tn; };
 template <int BM>
 MSLK_AMD_DEVINL bool find_group_tile(const MxProblem& p, int tiles_n, int wg, GroupTile& out) {
@@ -64,7 +66,7 @@ MSLK_AMD_DEVINL bool find_group_tile(const MxProblem& p, int tiles_n, int wg, Gr
     }
     const int64_t start = rows_before + end - mine;
     int r = (int)max((int64_t)0, min((int64_t)mine, p.M - start));
-    r = (r + BM - 1) / BM;
+    r = row_tiles_of<BM>(r);
 #pragma unroll
     for (int d = 32; d > 0; d /= 2) r += __shfl_xor(r, d, 64);
     tiles += r;
@@ -84,7 +86,7 @@ MSLK_AMD_DEVINL bool find_group_tile(const MxProblem& p, int tiles_n, int wg, Gr
     }
     const int64_t start = rows_before + end - mine;
     const int live = (int)max((int64_t)0, min((int64_t)mine, p.M - start));
-    int last = (live + BM - 1) / BM * tiles_n;   // entries up to and with this group's
+    int last = row_tiles_of<BM>(live) * tiles_n;   // entries up to and with this group's
     const int own = last;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -96,7 +98,7 @@ MSLK_AMD_DEVINL bool find_group_tile(const MxProblem& p, int tiles_n, int wg, Gr
       const int src = __ffsll((unsigned long long)holds) - 1;
       out.g = __builtin_amdgcn_readfirstlane(g0 + src);
       const int row0 = __shfl((int)start, src, 64), size = __shfl(live, src, 64), at = t - (before + __shfl(last - own, src, 64));
-      tile_at(at, (size + BM - 1) / BM, tiles_n, out.tm, out.tn);
+      tile_at(at, row_tiles_of<BM>(size), tiles_n, out.tm, out.tn);
       out.row0 = __builtin_amdgcn_readfirstlane(row0) + out.tm * BM;
       out.rows = min(__builtin_amdgcn_readfirstlane(size) - out.tm * BM, BM);
       return true;

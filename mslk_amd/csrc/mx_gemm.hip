@@ -2,6 +2,7 @@
 #include "kernels.h"
 #include "mx_device.h"
 #include "mx_tile_large.h"
+#include "rows.h"
 
 namespace mslk_amd {
 namespace {
@@ -209,7 +210,7 @@ MSLK_AMD_DEVINL MxOperands operands_of(const MxProblem& p, int m0, int rows, int
   return o;
 }
 
-// One tile per workgroup.
+// One tile per workgroup; the grid goes on along y (rows.h).
 template <typename TS, bool GATED, bool GROUPS, bool BIAS, bool F16>
 __global__ __launch_bounds__(TS::NTHREADS) void mx_kernel(MxProblem p, int tiles_m, int tiles_n) {
   static_assert(TS::LDS_BYTES <= 160 * 1024, "LDS of a CU");
@@ -219,13 +220,13 @@ __global__ __launch_bounds__(TS::NTHREADS) void mx_kernel(MxProblem p, int tiles
   int64_t w_row = 0;
   if constexpr (GROUPS) {
     GroupTile t;
-    if (!find_group_tile<TS::BM>(p, tiles_n, blockIdx.x, t)) return;
+    if (!find_group_tile<TS::BM>(p, tiles_n, (int)row_block(), t)) return;
     m0 = t.row0;
     rows = t.rows;
     tn = t.tn;
     w_row = (int64_t)t.g * p.N * (GATED ? 2 : 1);
   } else {
-    const int t = entry_of(blockIdx.x, tiles_m * tiles_n);
+    const int t = entry_of((int)row_block(), tiles_m * tiles_n);
     if (t < 0) return;
     int tm;
     tile_at(t, tiles_m, tiles_n, tm, tn);
@@ -392,7 +393,7 @@ MSLK_AMD_DEVINL void list_row_tiles(const ListJob& job, const uint32_t* sizes, i
 
 __global__ __launch_bounds__(256) void arrange_scales_kernel(ArrangeJob a, ArrangeJob b, ListJob tiles, int from, int pairs) {
   extern __shared__ __attribute__((aligned(16))) uint4 piece[];   // [row][pair], an odd number of pieces per row
-  int at = blockIdx.x;
+  int at = (int)row_block();
   if (tiles.m_sizes != nullptr && at-- == 0) {
     uint32_t* const sizes = reinterpret_cast<uint32_t*>(piece);
     const int held = min(tiles.G, 64 * 4);
@@ -404,6 +405,7 @@ __global__ __launch_bounds__(256) void arrange_scales_kernel(ArrangeJob a, Arran
   const bool second = at >= a.workgroups;
   const ArrangeJob job = second ? b : a;
   if (second) at -= a.workgroups;
+  if (at >= job.workgroups) return;   // behind the last one, in the grid's last line
   const int slabs = (pairs + kArrangePairs - 1) / kArrangePairs, block = at / slabs, pair0 = (at - block * slabs) * kArrangePairs;
   const int n = min(pairs - pair0, kArrangePairs), rows = (int)min((int64_t)64, job.rows - (int64_t)block * 64);
   const int pitch = n | 1;
@@ -447,11 +449,11 @@ int64_t most_row_tiles(int64_t M, int64_t G, int64_t tile_rows) { return M / til
 template <typename TS, bool GATED, bool GROUPS, bool BIAS, bool F16>
 hipError_t launch_tiles(const MxProblem& p, hipStream_t s) {
   constexpr int COLUMNS = GATED ? TS::BN / 2 : TS::BN;
-  const int64_t tiles_n = (p.N + COLUMNS - 1) / COLUMNS;
-  const int64_t tiles_m = GROUPS ? most_row_tiles(p.M, p.G, TS::BM) : (p.M + TS::BM - 1) / TS::BM;
+  const int64_t tiles_n = ((int64_t)p.N + COLUMNS - 1) / COLUMNS;
+  const int64_t tiles_m = GROUPS ? most_row_tiles(p.M, p.G, TS::BM) : ((int64_t)p.M + TS::BM - 1) / TS::BM;
   const int64_t grid = (tiles_m * tiles_n + kXcds - 1) / kXcds * kXcds;
-  if (grid * TS::NTHREADS >= (int64_t(1) << 32)) return hipErrorInvalidValue;
-  mx_kernel<TS, GATED, GROUPS, BIAS, F16><<<(unsigned)grid, TS::NTHREADS, 0, s>>>(p, (int)tiles_m, (int)tiles_n);
+  if (grid >= (int64_t(1) << 30)) return hipErrorInvalidValue;
+  mx_kernel<TS, GATED, GROUPS, BIAS, F16><<<row_grid(grid), TS::NTHREADS, 0, s>>>(p, (int)tiles_m, (int)tiles_n);
   return hipGetLastError();
 }
 
@@ -471,8 +473,8 @@ template <bool GATED, bool BIAS, bool F16>
 hipError_t launch_walk(const MxProblem& p, hipStream_t s) {
   constexpr int COLUMNS = GATED ? MxLarge::BN / 2 : MxLarge::BN;
   if (p.K <= 256) return hipErrorInvalidValue;   // (the tiles load two steps ahead)
-  const int64_t tiles_n = (p.N + COLUMNS - 1) / COLUMNS;
-  const int64_t tiles_m = p.row_tiles != nullptr ? most_row_tiles(p.M, p.G, MxLarge::BM) : (p.M + MxLarge::BM - 1) / MxLarge::BM;
+  const int64_t tiles_n = ((int64_t)p.N + COLUMNS - 1) / COLUMNS;
+  const int64_t tiles_m = p.row_tiles != nullptr ? most_row_tiles(p.M, p.G, MxLarge::BM) : ((int64_t)p.M + MxLarge::BM - 1) / MxLarge::BM;
   if (tiles_m * tiles_n >= (int64_t(1) << 30)) return hipErrorInvalidValue;
   const int64_t grid = (2 * tiles_m * tiles_n + kXcds - 1) / kXcds * kXcds, cus = device_compute_units();
   mx_walk_kernel<GATED, BIAS, F16><<<(unsigned)(grid < cus ? grid : cus), MxLarge::NTHREADS, 0, s>>>(p, (int)tiles_m, (int)tiles_n);
@@ -571,7 +573,7 @@ hipError_t launch_mx_mm(MxProblem p, void* workspace, bool scales_aligned, hipSt
     s.data = tensor;
     if (!arranged) return true;
     const int64_t wgs = (rows + 63) / 64 * ((pairs + kArrangePairs - 1) / kArrangePairs);
-    if (wgs * 256 >= (int64_t(1) << 31)) return false;
+    if (wgs >= (int64_t(1) << 29)) return false;
     job = ArrangeJob{tensor, room, rows, (int)wgs};
     s.data = room;
     room += arranged_bytes(rows, p.K);
@@ -580,7 +582,7 @@ hipError_t launch_mx_mm(MxProblem p, void* workspace, bool scales_aligned, hipSt
   if (!scales(p.xs, p.M, a) || !scales(p.ws, (int64_t)p.N * (p.gated ? 2 : 1) * (grouped ? p.G : 1), b)) return hipErrorInvalidValue;
   if (listed || arranged) {
     const int most = pairs < kArrangePairs ? pairs : kArrangePairs;
-    arrange_scales_kernel<<<(unsigned)(a.workgroups + b.workgroups + (listed ? 1 : 0)), 256, 64 * (most | 1) * 16, s>>>(a, b, tiles, from, pairs);
+    arrange_scales_kernel<<<row_grid((int64_t)a.workgroups + b.workgroups + (listed ? 1 : 0)), 256, 64 * (most | 1) * 16, s>>>(a, b, tiles, from, pairs);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
   }
   if (way == kWalk) return p.out_f16 ? launch_walk<true>(p, s) : launch_walk<false>(p, s);
