@@ -438,6 +438,12 @@ const char* mslk_amd_debug_grouped_dispatch_name(int layout, int G, int64_t M, i
 const char* mslk_amd_debug_grouped_list_dispatch_name(int G, const int64_t* M, const int64_t* N, const int64_t* K);
 
 /*
+ * The same for mslk_amd_mxfp4_mm (groups 0) and mslk_amd_mxfp4_grouped_mm ("mx_tiles<32,32,waves=1x1x4> workgroups=256",
+ * "arrange_scales + mx_walk tiles=640 workgroups=256", ...); aligned_scales as for their workspace sizes.
+ */
+const char* mslk_amd_debug_mxfp4_dispatch_name(int64_t M, int64_t N, int64_t K, int gated, int groups, int aligned_scales);
+
+/*
  * How the 256 x 256 tiles of row groups are divided inside an XCD: the entry of its slice of `tiles` tiles that workgroup `worker`
  * (of 2 * wgs) works on in `pass`, -1 for none, and which piece of how many of that tile (*piece, *pieces).  Host code; returns -2
  * for arguments out of range.

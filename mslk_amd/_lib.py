@@ -91,6 +91,7 @@ SIGNATURES = {
     "mslk_amd_debug_cast_e4m3fn": (c_int, [c_void_p, c_int64, c_void_p, c_void_p]),
     "mslk_amd_debug_dispatch_name": (c_char_p, [c_int64, c_int64, c_int64, c_int, c_int, c_int, c_int]),
     "mslk_amd_debug_grouped_dispatch_name": (c_char_p, [c_int, c_int, c_int64, c_int64, c_int64]),
+    "mslk_amd_debug_mxfp4_dispatch_name": (c_char_p, [c_int64, c_int64, c_int64, c_int, c_int, c_int]),
     "mslk_amd_debug_grouped_list_dispatch_name": (c_char_p, [c_int, POINTER(c_int64), POINTER(c_int64), POINTER(c_int64)]),
     "mslk_amd_debug_row_walk": (c_int, [c_int, c_int, c_int, c_int, POINTER(c_int), POINTER(c_int)]),
     "mslk_amd_debug_stream_read": (c_int, [c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p]),

@@ -762,6 +762,21 @@ const char* mslk_amd_debug_grouped_list_dispatch_name(int G, const int64_t* M, c
   return result;
 }
 
+const char* mslk_amd_debug_mxfp4_dispatch_name(int64_t M, int64_t N, int64_t K, int gated, int groups, int aligned_scales) {
+  void* const fake = reinterpret_cast<void*>(uintptr_t(1) << 20);
+  const void* const scales = static_cast<const char*>(fake) + (aligned_scales ? 0 : 1);
+  thread_local char result[600];
+  const size_t room = ~size_t(0);
+  dispatch_probe_begin();
+  const int rc = groups != 0 ? mslk_amd_mxfp4_grouped_mm(fake, fake, scales, scales, static_cast<const int64_t*>(fake), groups, gated, fake, MSLK_AMD_DTYPE_BF16,
+                                                         M, N, K, fake, room, nullptr)
+                             : mslk_amd_mxfp4_mm(fake, fake, scales, scales, nullptr, 0, gated, fake, MSLK_AMD_DTYPE_BF16, M, N, K, fake, room, nullptr);
+  const char* text = dispatch_probe_end();
+  if (rc != 0) snprintf(result, sizeof(result), "error: %s", g_err);
+  else snprintf(result, sizeof(result), "%s", text[0] ? text : "nothing to launch");
+  return result;
+}
+
 int mslk_amd_debug_row_walk(int tiles, int wgs, int worker, int pass, int* piece, int* pieces) {
   if (tiles < 0 || tiles > (1 << 28) || wgs <= 0 || wgs > 1024 || worker < 0 || worker >= 2 * wgs || pass < 0 || pass > (1 << 20) || !piece || !pieces) return -2;
   return debug_row_walk(tiles, wgs, worker, pass, piece, pieces);

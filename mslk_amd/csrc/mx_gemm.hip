@@ -453,6 +453,8 @@ hipError_t launch_tiles(const MxProblem& p, hipStream_t s) {
   const int64_t tiles_m = GROUPS ? most_row_tiles(p.M, p.G, TS::BM) : ((int64_t)p.M + TS::BM - 1) / TS::BM;
   const int64_t grid = (tiles_m * tiles_n + kXcds - 1) / kXcds * kXcds;
   if (grid >= (int64_t(1) << 30)) return hipErrorInvalidValue;
+  if (dispatch_probe_record("mx_tiles<%d,%d,waves=%dx%dx%d>%s workgroups=%lld", TS::BM, TS::BN, TS::WM, TS::WN, TS::KS, GROUPS ? " groups" : "", (long long)grid))
+    return hipSuccess;
   mx_kernel<TS, GATED, GROUPS, BIAS, F16><<<row_grid(grid), TS::NTHREADS, 0, s>>>(p, (int)tiles_m, (int)tiles_n);
   return hipGetLastError();
 }
@@ -477,7 +479,9 @@ hipError_t launch_walk(const MxProblem& p, hipStream_t s) {
   const int64_t tiles_m = p.row_tiles != nullptr ? most_row_tiles(p.M, p.G, MxLarge::BM) : ((int64_t)p.M + MxLarge::BM - 1) / MxLarge::BM;
   if (tiles_m * tiles_n >= (int64_t(1) << 30)) return hipErrorInvalidValue;
   const int64_t grid = (2 * tiles_m * tiles_n + kXcds - 1) / kXcds * kXcds, cus = device_compute_units();
-  mx_walk_kernel<GATED, BIAS, F16><<<(unsigned)(grid < cus ? grid : cus), MxLarge::NTHREADS, 0, s>>>(p, (int)tiles_m, (int)tiles_n);
+  const unsigned wgs = (unsigned)(grid < cus ? grid : cus);
+  if (dispatch_probe_record("mx_walk%s tiles=%lld workgroups=%u", p.row_tiles != nullptr ? " groups" : "", (long long)(tiles_m * tiles_n), wgs)) return hipSuccess;
+  mx_walk_kernel<GATED, BIAS, F16><<<wgs, MxLarge::NTHREADS, 0, s>>>(p, (int)tiles_m, (int)tiles_n);
   return hipGetLastError();
 }
 
@@ -580,7 +584,7 @@ hipError_t launch_mx_mm(MxProblem p, void* workspace, bool scales_aligned, hipSt
     return true;
   };
   if (!scales(p.xs, p.M, a) || !scales(p.ws, (int64_t)p.N * (p.gated ? 2 : 1) * (grouped ? p.G : 1), b)) return hipErrorInvalidValue;
-  if (listed || arranged) {
+  if ((listed || arranged) && !dispatch_probe_record(!arranged ? "list_row_tiles" : listed ? "arrange_scales with list_row_tiles" : "arrange_scales")) {
     const int most = pairs < kArrangePairs ? pairs : kArrangePairs;
     arrange_scales_kernel<<<row_grid((int64_t)a.workgroups + b.workgroups + (listed ? 1 : 0)), 256, 64 * (most | 1) * 16, s>>>(a, b, tiles, from, pairs);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;

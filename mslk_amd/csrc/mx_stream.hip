@@ -169,6 +169,7 @@ __global__ __launch_bounds__(S::WAVES * 64) void mx_stream_kernel(MxProblem p) {
 
 template <typename S>
 hipError_t launch(const MxProblem& p, unsigned grid, hipStream_t s) {
+  if (dispatch_probe_record("mx_stream<%d,waves=%d> workgroups=%u", S::XR, S::WAVES, grid)) return hipSuccess;
   if (p.gated) mx_stream_kernel<S, true><<<grid, S::WAVES * 64, 0, s>>>(p);
   else mx_stream_kernel<S, false><<<grid, S::WAVES * 64, 0, s>>>(p);
   return hipGetLastError();

@@ -72,3 +72,9 @@ def grouped_list_kernel(sizes, N: int, K) -> str:
     i64 = lambda v: (ctypes.c_int64 * G)(*v)
     return _lib.lib().mslk_amd_debug_grouped_list_dispatch_name(
         G, i64(sizes), i64([N] * G), i64([K] * G if isinstance(K, int) else K)).decode()
+
+
+def mxfp4_kernel(M: int, N: int, K: int, gated: bool = False, groups: int = 0, aligned: bool = True) -> str:
+    """The launches of an MXFP4 product (groups 0: dense); aligned: both tensors of scales begin on 16 bytes."""
+    from mslk_amd import _lib
+    return _lib.lib().mslk_amd_debug_mxfp4_dispatch_name(M, N, K, gated, groups, aligned).decode()
