@@ -460,7 +460,8 @@ int mslk_amd_debug_row_walk(int tiles, int wgs, int worker, int pass, int* piece
  *   mslk_amd_debug_mfma_loop: `workgroups` x 4 waves each run `iters` iterations of a 128 x 128 x 128 wave tile out of
  *     registers: 64 v_mfma_f32_16x16x128_f8f6f4 (form 0) or 32 v_mfma_f32_32x32x64_f8f6f4 (form 1) per iteration, i.e.
  *     iters * 2 * 128^3 FLOP per wave.  `operands` points at 128 KiB of e4m3 codes (32-byte aligned) that fill the operand
- *     registers once; the rate depends on these values through the power they draw.
+ *     registers once; the rate depends on these values through the power they draw.  Forms 2 and 3 are 0 and 1 on e2m1 codes,
+ *     the first 16 of every 32 bytes, with scales of 1.
  *   mslk_amd_debug_tile_streams: the global -> LDS loads of the 128 x 64 tile kernel's K loop and nothing else (no LDS
  *     reads, no multiplies, no output): tiles_m x tiles_n workgroups in the dense kernels' tile order, each fetching the
  *     128 rows of its row tile from x (tiles_m * 128 rows of K bytes, x_bytes in all) and / or its 64 weight rows from w

@@ -792,7 +792,7 @@ int mslk_amd_debug_stream_read(const void* src, int64_t bytes, int mode, int wor
 }
 
 int mslk_amd_debug_mfma_loop(const void* operands, int form, int iters, int workgroups, void* sink, void* stream) {
-  if (form != 0 && form != 1) return fail("debug_mfma_loop: form must be 0 (16x16x128) or 1 (32x32x64)");
+  if (form < 0 || form > 3) return fail("debug_mfma_loop: form must be 0 (16x16x128) or 1 (32x32x64), of e2m1 codes 2 or 3");
   if (iters < 0 || iters > (1 << 20)) return fail("debug_mfma_loop: iters must be in 0 .. 2^20");
   if (workgroups <= 0 || workgroups > 65536) return fail("debug_mfma_loop: workgroups must be in 1 .. 65536");
   if (!operands || reinterpret_cast<uintptr_t>(operands) % 32 != 0) return fail("debug_mfma_loop: operands must be a 32-byte aligned device pointer to 128 KiB");

@@ -105,6 +105,9 @@ __global__ __launch_bounds__(256) void tile_streams_kernel(const uint8_t* __rest
 // (32x32x64) independent accumulators per wave, the wave tile of the GEMM (128 x 128 x 128 per iteration), one wave per
 // SIMD.  No memory traffic inside the loop: what it sustains is the matrix cores' rate at the clock the power limit grants
 // for these operand values.
+// E2M1: codes of four bits, the first 16 bytes of a fragment, with scales of 1; else e4m3 without scales.
+constexpr int kOnes = 0x7F7F7F7F;
+template <bool E2M1>
 __global__ __launch_bounds__(256) void mfma_16x16x128_kernel(const v8i* __restrict__ src, int iters, float* __restrict__ sink) {
   v8i a[8], b[8];
 #pragma unroll
@@ -122,7 +125,8 @@ __global__ __launch_bounds__(256) void mfma_16x16x128_kernel(const v8i* __restri
     for (int i = 0; i < 8; ++i)
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[i], b[j], acc[i][j], 0, 0, 0, 0, 0, 0);
+        acc[i][j] = E2M1 ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[i], b[j], acc[i][j], 4, 4, 0, kOnes, 0, kOnes)
+                         : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a[i], b[j], acc[i][j], 0, 0, 0, 0, 0, 0);
   }
   float s = 0.f;
 #pragma unroll
@@ -132,6 +136,7 @@ __global__ __launch_bounds__(256) void mfma_16x16x128_kernel(const v8i* __restri
   if (s == 123.456f && sink != nullptr) sink[0] = s;
 }
 
+template <bool E2M1>
 __global__ __launch_bounds__(256) void mfma_32x32x64_kernel(const v8i* __restrict__ src, int iters, float* __restrict__ sink) {
   v8i a[8], b[8];   // 4 blocks of 32 rows x 2 halves of the 128-byte K step
 #pragma unroll
@@ -153,7 +158,8 @@ __global__ __launch_bounds__(256) void mfma_32x32x64_kernel(const v8i* __restric
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i * 2 + h], b[j * 2 + h], acc[i][j], 0, 0, 0, 0, 0, 0);
+          acc[i][j] = E2M1 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i * 2 + h], b[j * 2 + h], acc[i][j], 4, 4, 0, kOnes, 0, kOnes)
+                           : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a[i * 2 + h], b[j * 2 + h], acc[i][j], 0, 0, 0, 0, 0, 0);
   }
   float s = 0.f;
 #pragma unroll
@@ -183,8 +189,12 @@ hipError_t launch_debug_tile_streams(const void* x, const void* w, int K, int ti
 }
 
 hipError_t launch_debug_mfma_loop(const void* operands, int form, int iters, int workgroups, void* sink, hipStream_t s) {
-  if (form == 0) mfma_16x16x128_kernel<<<workgroups, 256, 0, s>>>(static_cast<const v8i*>(operands), iters, static_cast<float*>(sink));
-  else mfma_32x32x64_kernel<<<workgroups, 256, 0, s>>>(static_cast<const v8i*>(operands), iters, static_cast<float*>(sink));
+  const v8i* src = static_cast<const v8i*>(operands);
+  float* out = static_cast<float*>(sink);
+  if (form == 0) mfma_16x16x128_kernel<false><<<workgroups, 256, 0, s>>>(src, iters, out);
+  else if (form == 1) mfma_32x32x64_kernel<false><<<workgroups, 256, 0, s>>>(src, iters, out);
+  else if (form == 2) mfma_16x16x128_kernel<true><<<workgroups, 256, 0, s>>>(src, iters, out);
+  else mfma_32x32x64_kernel<true><<<workgroups, 256, 0, s>>>(src, iters, out);
   return hipGetLastError();
 }
 
