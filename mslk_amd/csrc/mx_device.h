@@ -13,7 +13,8 @@ constexpr int kPanel = 4;   // row tiles that share the weights of a panel in an
 // about two units, the reciprocal by one: far below the rounding to 16 bits that follows, as |gate| is below 2^7 here.
 // Below -87 the reciprocal is no normal number any more, and from -88.7 on exp(-gate) is infinite, but up may bring the product back into range (gate -90,
 // up 1e30: -7e-8).  There silu(gate) = gate exp(gate) to the last bit; exp(gate) = 2^n 2^f, |f| <= 1/2, and 2^n is multiplied to up first.
-// FAR: some gate may be that far.  Callers look at all gates of a lane (far_gates()) and make their values again if one of the wave's is.
+// FAR: some gate may be that far.  Callers look at all gates of a lane (far_gates()) and make their values again if one of the wave's is.  That look is what
+// it costs otherwise: 2047 x (2 x 10000) x 4128 takes 100.5 us in the kernel instead of 99.2, 128 experts of 2 x 768 x 2048 93 instead of 92.
 template <bool FAR>
 MSLK_AMD_DEVINL float gated_value(float gate, float up) {
   const float near = gate * __builtin_amdgcn_rcpf(1.f + __expf(-gate)) * up;

@@ -508,21 +508,22 @@ using Tile128x128 = MxShape<128, 128, 2, 2, 1>;     // two
 bool fetched_in_place(int64_t K, bool small, bool scales_aligned) { return K % (small ? 128 : 512) == 0 && scales_aligned; }
 
 // The smallest tiles of which each CU gets no more than it holds at once, since their steps' loads, not their products, are waited for.  µs:
-//   16 x 4096 x 14336   32x32 8.3, 32x64 11.7, 64x64 14.3
+//   16 x 4096 x 14336   32x32 8.9, 32x64 11.7, 64x64 14.9
 //   64 x 4096 x 14336   32x32 9.5, 32x64 13.0, 64x64 18.0
-//   64 x 8192 x 8192    32x64 9.9, 32x32 11.0, 64x64 13.2 (two waves 14.3), 128x128 25.7
-//   16 x 16384 x 4096   32x32 8.2, 32x64 8.5, 64x64 9.8 (up to 32 rows two of the smallest to a CU, as they read no weights twice)
-//   128 x 8192 x 8192   64x64 13.9 (two waves 15.1), 32x64 17.1, 128x128 26.3
-//   256 x 8192 x 8192   64x64 of two waves 19.7 (four 24.8), 128x128 27.0
-//   500 x 8192 x 4096   128x128 16.4, 64x64 22.1, walk 23.1
-//   1000 x 10240 x 8192 walk 55.2, 128x128 64.9
-// Two 128x128 tiles to a CU only with a short K: 1000 x 8192 x 1024 8.9 (walk 11.3), 500 x 14336 x 2048 13.6 (15.5), 500 x 10240 x 4096 20.9 (21.1),
-// 500 x 10240 x 8192 37.0 (36.0), 2000 x 4096 x 14336 69.7 (64.7); one to a CU 500 x 8192 x 8192 28.4 (33.0).
+//   64 x 8192 x 8192    32x64 9.7, 32x32 10.5, 64x64 12.8 (two waves 14.7), 128x128 26.1
+//   16 x 16384 x 4096   32x32 8.2, 32x64 8.7, 64x64 10.0 (up to 32 rows two of the smallest to a CU, as they read no weights twice)
+//   128 x 8192 x 8192   64x64 13.3 (two waves 15.2), 32x64 16.1, 128x128 26.6
+//   256 x 8192 x 8192   64x64 of two waves 19.3 (four 23.3), 128x128 27.1
+//   500 x 8192 x 4096   128x128 17.0, walk 20.5, 64x64 21.6
+//   1000 x 10240 x 8192 walk 51.8, 128x128 65.0
+// Two 128x128 tiles to a CU only with a short K: 1000 x 8192 x 1024 9.5 (walk 11.7), 500 x 14336 x 2048 13.5 (15.3), 500 x 10240 x 4096 20.9 (21.1),
+// 500 x 10240 x 8192 34.6 (34.7), 2000 x 4096 x 14336 73.7 (66.1); one to a CU 500 x 8192 x 8192 29.2 (32.9).
 // Up to 32 rows whose scales would have to be arranged first take the kernel that needs no such launch, if there is a CU for every 32 columns
-// (16 x 4096 x 4128 8.8, arranged 11.2).
-// Groups of few rows on average wait for weights, too: 64x128 tiles (16 groups, 256 rows, 2 x 5120 x 4096 74.0, walk 79.4; 8 groups, 512 rows,
-// 4096 x 14336 77 and 102; 32 groups, 256 rows, 2 x 1024 x 2048 16.4 and 19.1), but for many of a short K the walk, which has no gap between its
-// tiles and no workgroups for tiles that groups might have had (128 groups, 512 rows, 2 x 768 x 2048 35.5, 64x128 41.3).
+// (16 x 4096 x 4128 6.5, arranged 8.6; 32 x 8192 x 5152 7.9, 11.2).
+// Groups of few rows on average wait for weights, too: 64x128 tiles (16 groups, 256 rows, 2 x 5120 x 4096 74.2, walk 79.5; 8 groups, 512 rows,
+// 4096 x 14336 77.0 and 102.5; 32 groups, 256 rows, 2 x 1024 x 2048 14.0 and 19.1; a few crowded groups of more rows go the other way: 16 groups, 1024 rows,
+// 2 x 5120 x 4096 93.4 and 86.2), but for many of a short K the walk, which has no gap between its tiles and no workgroups for tiles that groups might have
+// had (128 groups, 512 rows, 2 x 768 x 2048 36.9, 64x128 38.6; of four rows each 49.1 and 46.7).
 Way way_of(int64_t M, int64_t N, int64_t K, int gated, int64_t G, bool grouped, bool scales_aligned) {
   const int64_t cus = device_compute_units(), columns = N * (gated ? 2 : 1);
   auto tiles = [&](int64_t bm, int64_t bn) { return (grouped ? most_row_tiles(M, G, bm) : (M + bm - 1) / bm) * ((columns + bn - 1) / bn); };
@@ -536,8 +537,9 @@ Way way_of(int64_t M, int64_t N, int64_t K, int gated, int64_t G, bool grouped, 
 }
 
 // Whether the scales are arranged first.  If they can be fetched in place, the launch in front has to be worth it.
-// The walk: from 128 steps of 256 x 256 sums per CU on (arranged / in place, us: 4096 x 4096 x 4096 43.4 / 41.4, 16 experts, 2048 rows, 8192 x 5120
-// 126 / 119, 8192 x 8192 x 2048 92 / 91, 8192 x 8192 x 8192 263 / 265, 16384 x 8192 x 16384 938 / 959, 16 experts, 32768 rows 756 / 774).
+// The walk: from 128 steps of 256 x 256 sums per CU on (arranged / in place, us: 4096 x 4096 x 4096 41.4 / 39.0, 16 experts, 2048 rows, 8192 x 5120
+// 122 / 116, 8192 x 8192 x 2048 86 / 83, 8192 x 8192 x 4096 139 / 136, 8192 x 8192 x 8192 246 / 243, 16384 x 8192 x 16384 923 / 945, 16 experts, 16384 rows
+// 416 / 425, 32768 rows 793 / 809).
 // Tiles of fewer rows wait for codes, or have few steps.
 bool arranges(Way way, int64_t M, int64_t N, int64_t K, int gated, bool scales_aligned) {
   if (!fetched_in_place(K, way < k128x128, scales_aligned)) return true;

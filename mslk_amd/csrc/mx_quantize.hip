@@ -6,8 +6,8 @@
 //
 // Both are bound by memory.  A lane holds 8 values (16 bytes of 16-bit ones), so that a wave reads and writes whole lines; four
 // neighbouring lanes are a block and find its maximum by data-parallel moves, on the bits, where NaN > infinity > numbers.
-// Values of half of the Infinity Cache and more go past the caches (STREAM), there and back: 8192 x 28672 bf16 values take 178 us in all instead of 224
-// (6.7 TB/s read and written: the codes stay in the cache between the two), 8192 x 8192 55 instead of 60.  Fewer are left where a reader may find them.
+// Values of half of the Infinity Cache and more go past the caches (STREAM), there and back: 8192 x 28672 bf16 values take 177 us in all instead of 224
+// (5.3 TB/s of values: the codes stay in the cache between the two), 8192 x 8192 55 instead of 60.  Fewer are left where a reader may find them.
 #include <type_traits>
 
 #include "mx.h"

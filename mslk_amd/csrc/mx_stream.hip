@@ -1,6 +1,6 @@
 // Products of few rows of X with MXFP4 weights for gfx950 (formats: mx.h), for rows of scales that do not begin on 4 bytes: they go to
 // registers from wherever they lie, and no launch arranges them first.  The weights are read once, and they are what counts: 16 x 4096 x 4128 takes
-// 8.8 us.
+// 6.3 us a call.
 //
 // A workgroup makes 32 columns (gated: 16, from 16 rows of the gate and their 16 partners) of up to 32 rows of X.  Its waves take K's
 // pairs of steps, 512 values, in turn, each with a part of the LDS for itself: no barrier until their sums meet in LDS, and no sums

@@ -16,7 +16,7 @@
 // Products.  v_mfma_scale_f32_32x32x64_f8f6f4, W first: lane (i = l & 31, h = l >> 5) gives row i's chunk 4 h + j to product j of a
 // step, and the four bytes of its scales of the step are those of chunks 4 h ... 4 h + 3: the instruction picks byte j.  Any order of
 // K would do that both operands share; this one needs neither shifts nor shuffles of scales.  Out of registers and on quantized normal
-// numbers these run at 6.66 PFLOP/s, 16x16x128 at 5.96 (on zeros 9.89 and 6.63: the limit on numbers is power).
+// numbers these run at 6.8 PFLOP/s (on zeros 9.8: the limit on numbers is power).  16x16x128 draws less, 7.6 (9.7), but no tile here is built on it.
 // Rows.  LDS row f 32 W + w 32 + i of an operand is row i of fragment f of wave row (column) w, W of them.  Of 32 rows of W a lane receives
 // rows 8 q + 4 h + r (q, r = 0 ... 3); fragment 2 T + t takes columns 64 T + 16 q + 8 h + 4 t + r of the wave's, so that a pair of fragments
 // gives a lane eight neighbouring columns: 16 bytes of a row of Y, stored as they are.

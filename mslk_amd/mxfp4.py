@@ -9,8 +9,9 @@ of two.  Codes are bytes [.., K / 2] with the earlier value in the low half (uin
 bytes s [.., K / 32] that stand for 2^(s - 127), 255 for NaN (uint8 or torch.float8_e8m0fnu): the layouts of the OCP microscaling
 specification, so weights quantized elsewhere can be used as they are.  Products take both operands so, sum in fp32 and round once.
 
-Nothing here is differentiable.  Codes have to be contiguous; a K that is no multiple of 512 (for few rows, 128) or scales that do not
-begin on 16 bytes cost a copy of the scales in each call.
+Nothing here is differentiable.  Codes have to be contiguous.  Both tensors of scales are copied in each call, into another order, where they cannot be
+read as they lie (K no multiple of 512, of 128 for products of few tiles, or scales that do not begin on 16 bytes; up to 32 rows and as many columns as
+32 per compute unit are read from anywhere) and where the product is large enough to gain by it (2 M N K of 1.1e12 operations and more).
 """
 from __future__ import annotations
 
